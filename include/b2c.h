@@ -132,6 +132,80 @@ int b2c_gesv(const float *A, const float *b, float *x, int64_t batch, int k,
 int b2c_qr(const float *A, float *Q, float *R, int64_t batch, int k,
            void *workspace, size_t workspace_bytes, void *stream);
 
+/* Element types of the products below. */
+#define B2C_F32 0
+#define B2C_BF16 1
+#define B2C_F16 2
+
+/* Activations of the products' epilogue. */
+#define B2C_ACT_NONE 0
+#define B2C_ACT_RELU 1
+#define B2C_ACT_GELU 2      /* x Phi(x), Phi through erf */
+#define B2C_ACT_GELU_TANH 3 /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+#define B2C_ACT_SILU 4      /* x / (1 + exp(-x)) */
+
+/* A batch of matrices with free strides, in elements: element (b, r, c) at
+ * ptr[b * batch_stride + r * row_stride + c * col_stride]. Strides may be 0
+ * (a broadcast axis) but not negative. */
+typedef struct b2c_matrix {
+  const void *ptr;
+  int64_t batch_stride, row_stride, col_stride;
+} b2c_matrix;
+
+/* Matrix product with its epilogue,
+ *   pre = alpha * A B + bias,   Y = act(pre) + beta * R,
+ * all of type `dtype`; sums and the epilogue are held in 32 bits and each
+ * output is rounded once.
+ *   A    (batch, M, K), B (batch, K, N)  inputs, any strides (batch_stride 0:
+ *                                        one matrix for the whole batch)
+ *   bias (N,) contiguous, or NULL
+ *   R    (batch, M, N) any strides, or NULL (beta is then unused); may be Y's
+ *        memory where R has Y's strides
+ *   Y    (batch, M, N) contiguous output
+ *   pre  (batch, M, N) contiguous output, or NULL
+ * Other outputs may not overlap the inputs. K = 0 gives A B = 0. Non-finite
+ * inputs give non-finite outputs where the sums meet them, for float32 NaN in
+ * the place of inf too. Each of M, K, N is at most 2^30. No counterpart in
+ * the reference. */
+int b2c_gemm(int dtype, const b2c_matrix *A, const b2c_matrix *B, const void *bias, const b2c_matrix *R, void *Y,
+             void *pre, int64_t batch, int64_t M, int64_t K, int64_t N, float alpha, float beta, int activation,
+             void *workspace, size_t workspace_bytes, void *stream);
+
+/* Scratch bytes of b2c_gemm for these operands (their alignment and strides
+ * count; A->ptr and B->ptr are not read). */
+size_t b2c_gemm_workspace_size(int dtype, const b2c_matrix *A, const b2c_matrix *B, int64_t batch, int64_t M,
+                               int64_t K, int64_t N);
+
+/* Gradient of that epilogue: dP = dY * act'(pre), dbias = the sum of dP's
+ * rows over the whole batch, dR = beta * dY. Any of the three outputs may be
+ * NULL. The products' gradients are then b2c_gemm calls,
+ * dA = alpha dP B^T and dB = alpha A^T dP.
+ *   dY, pre (batch, M, N) any strides; pre NULL with B2C_ACT_NONE only
+ *   dP, dR  (batch, M, N) contiguous; dbias (N,)
+ * The sums take dP before it is rounded, in a fixed order. No counterpart in
+ * the reference. */
+int b2c_gemm_dact(int dtype, const b2c_matrix *dY, const b2c_matrix *pre, int activation, float beta, void *dP,
+                  void *dbias, void *dR, int64_t batch, int64_t M, int64_t N, void *workspace,
+                  size_t workspace_bytes, void *stream);
+size_t b2c_gemm_dact_workspace_size(int64_t batch, int64_t M, int64_t N);
+
+/* Newton-Schulz orthogonalisation (the step that the Muon optimiser takes on
+ * an update): X = G / (|G|_F + eps), then `steps` times
+ *   X <- a X + (b S + c S S) X,  S = X X^T
+ * on the smaller side of G, (a, b, c) = coefficients[3 t .. 3 t + 2] in step
+ * t (a host array). With suitable coefficients the singular values of the
+ * result lie near 1. Every matrix of the batch has a norm of its own; one of
+ * zeros gives zeros, one with a non-finite entry gives NaN.
+ *   G   (batch, m, n) any strides; out (batch, m, n) contiguous, may be G's
+ *       memory where G is contiguous
+ * The polynomials have to keep |p(s)| <= 3.5 over the singular values that
+ * they can meet, starting from [0, 1]: B2C_ERR_INVALID_ARGUMENT otherwise.
+ * m, n at most 2^20. No counterpart in the reference. */
+int b2c_orthogonalize(int dtype, const b2c_matrix *G, void *out, int64_t batch, int64_t m, int64_t n,
+                      const double *coefficients, int steps, double eps, void *workspace, size_t workspace_bytes,
+                      void *stream);
+size_t b2c_orthogonalize_workspace_size(int dtype, const b2c_matrix *G, int64_t batch, int64_t m, int64_t n);
+
 /* Device-accessible address of pinned, mapped host memory (the address a
  * kernel may dereference; equal to host_ptr under unified addressing).
  * Returns B2C_ERR_CUDA, leaving *device_ptr NULL, when host_ptr is not

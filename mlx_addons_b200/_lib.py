@@ -23,8 +23,20 @@ B2C_ERR_CUDA = 4
 
 OP_POSV, OP_POTRF, OP_TRSM, OP_SLOGDET, OP_GESV, OP_QR = 0, 1, 2, 3, 4, 5
 
+F32, BF16, F16 = 0, 1, 2
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+class Matrix(ctypes.Structure):
+    """b2c_matrix: a batch of matrices with free strides, in elements."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("col_stride", ctypes.c_int64)]
+
+
 # Every symbol include/b2c.h declares, with its ctypes signature.
 _vp, _i64, _ci, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+_f, _d, _mp, _dp = ctypes.c_float, ctypes.c_double, ctypes.POINTER(Matrix), ctypes.POINTER(ctypes.c_double)
 SIGNATURES = {
     "b2c_version": (_ci, []),
     "b2c_last_error": (ctypes.c_char_p, []),
@@ -36,6 +48,12 @@ SIGNATURES = {
     "b2c_gesv": (_ci, [_vp, _vp, _vp, _i64, _ci, _ci, _vp, _sz, _vp]),
     "b2c_qr": (_ci, [_vp, _vp, _vp, _i64, _ci, _vp, _sz, _vp]),
     "b2c_posv_static_scratch": (_ci, [_vp, _vp, _vp, _vp, _i64, _ci, _ci, _vp]),
+    "b2c_gemm": (_ci, [_ci, _mp, _mp, _vp, _mp, _vp, _vp, _i64, _i64, _i64, _i64, _f, _f, _ci, _vp, _sz, _vp]),
+    "b2c_gemm_workspace_size": (_sz, [_ci, _mp, _mp, _i64, _i64, _i64, _i64]),
+    "b2c_gemm_dact": (_ci, [_ci, _mp, _mp, _ci, _f, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "b2c_gemm_dact_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "b2c_orthogonalize": (_ci, [_ci, _mp, _vp, _i64, _i64, _i64, _dp, _ci, _d, _vp, _sz, _vp]),
+    "b2c_orthogonalize_workspace_size": (_sz, [_ci, _mp, _i64, _i64, _i64]),
     "b2c_host_device_pointer": (_ci, [_vp, ctypes.POINTER(ctypes.c_void_p)]),
     "b2c_take_device_fault": (_ci, [ctypes.POINTER(ctypes.c_uint)]),
 }

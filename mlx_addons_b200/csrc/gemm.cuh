@@ -1,0 +1,148 @@
+// Matrix products with an epilogue: types and device helpers shared by
+// gemm_simt.cu, gemm_tc.cu, gemm_dact.cu and polar.cu.
+//
+// Every product is written as D[i, j] = sum_k P[i, k] Q[j, k] on two operands
+// with free strides; the caller of b2c_gemm has P = A, Q = B^T, or the other
+// way round where B's columns are the longer side.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "b2c.h"
+#include "b2c_common.cuh"
+
+namespace b2c {
+
+// One operand: element (b, r, k) at p[b * bs + r * rs + k * ks].
+struct GemmOperand {
+  const void* p;
+  int64_t bs, rs, ks;
+};
+
+// An addend or output in the coordinates of D.
+struct GemmView {
+  void* p;
+  int64_t bs, is, js;
+};
+
+// out = act(alpha * D + bias) + beta * res; pre = alpha * D + bias.
+struct GemmEpilogue {
+  GemmView y, pre, res;  // pre.p / res.p null where absent; all of the product's type
+  const void* bias;      // null where absent
+  int bias_on_i;         // bias[i] (1) or bias[j] (0)
+  int act;               // B2C_ACT_*
+  float alpha, beta;
+};
+
+struct GemmProblem {
+  int dtype;             // B2C_F32, B2C_BF16 or B2C_F16: operands, addends and outputs
+  GemmOperand P, Q;
+  int64_t batch;
+  int64_t I, J, K;
+  GemmEpilogue e;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+
+// Rounds to nearest even; a half result past the type's range becomes inf.
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+constexpr float kGeluC = 0.7978845608028654f;   // sqrt(2 / pi)
+constexpr float kGeluK = 0.044715f;
+constexpr float kRsqrt2 = 0.7071067811865476f;
+constexpr float kRsqrt2Pi = 0.3989422804014327f;  // 1 / sqrt(2 pi)
+
+__device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + expf(-x)); }
+
+// act(x). NaN stays NaN.
+__device__ __forceinline__ float act_f32(float x, int act) {
+  switch (act) {
+    case B2C_ACT_RELU: return x < 0.f ? 0.f : x;
+    case B2C_ACT_GELU: return 0.5f * x * (1.f + erff(x * kRsqrt2));
+    // 0.5 x (1 + tanh u) = x sigmoid(2 u)
+    case B2C_ACT_GELU_TANH: return x * sigmoid_f32(2.f * kGeluC * (x + kGeluK * x * x * x));
+    case B2C_ACT_SILU: return x * sigmoid_f32(x);
+    default: return x;
+  }
+}
+
+// d act(x) / dx, given the pre-activation.
+__device__ __forceinline__ float act_slope_f32(float x, int act) {
+  switch (act) {
+    case B2C_ACT_RELU: return x > 0.f ? 1.f : 0.f;
+    case B2C_ACT_GELU: return 0.5f * (1.f + erff(x * kRsqrt2)) + x * expf(-0.5f * x * x) * kRsqrt2Pi;
+    case B2C_ACT_GELU_TANH: {
+      const float s = sigmoid_f32(2.f * kGeluC * (x + kGeluK * x * x * x));
+      return s + x * s * (1.f - s) * 2.f * kGeluC * (1.f + 3.f * kGeluK * x * x);
+    }
+    case B2C_ACT_SILU: {
+      const float s = sigmoid_f32(x);
+      return s * (1.f + x * (1.f - s));
+    }
+    default: return 1.f;
+  }
+}
+
+// One element of the epilogue.
+template <typename T>
+__device__ __forceinline__ void epilogue_store(const GemmEpilogue& e, int64_t b, int64_t i, int64_t j, float acc) {
+  float v = e.alpha * acc;
+  if (e.bias) v += to_f32(static_cast<const T*>(e.bias)[e.bias_on_i ? i : j]);
+  if (e.pre.p) static_cast<T*>(e.pre.p)[b * e.pre.bs + i * e.pre.is + j * e.pre.js] = from_f32<T>(v);
+  v = act_f32(v, e.act);
+  if (e.res.p) v = fmaf(e.beta, to_f32(static_cast<const T*>(e.res.p)[b * e.res.bs + i * e.res.is + j * e.res.js]), v);
+  static_cast<T*>(e.y.p)[b * e.y.bs + i * e.y.is + j * e.y.js] = from_f32<T>(v);
+}
+
+// Launchers. gemm_simt.cu
+cudaError_t launch_gemm_simt(const GemmProblem& g, cudaStream_t s);
+
+// dP = dY act'(pre) (rounded to the type once), and the column sums of the
+// unrounded dP. gemm_dact.cu
+struct DactParams {
+  int dtype, act;
+  const void* dY;      // (batch, M, N), strides below
+  int64_t dy_bs, dy_rs, dy_cs;
+  const void* pre;     // null where act is none
+  int64_t pre_bs, pre_rs, pre_cs;
+  void* dP;            // (batch, M, N) contiguous, null where only the sums are wanted
+  void* dbias;         // (N,), null where unwanted
+  void* dR;            // beta dY, contiguous, null where unwanted
+  float beta;
+  int64_t batch, M, N;
+  float* ws;           // dact_ws_floats() floats where dbias is wanted
+};
+size_t dact_ws_floats(int64_t batch, int64_t M, int64_t N);
+cudaError_t launch_gemm_dact(const DactParams& p, cudaStream_t s);
+
+// polar.cu
+struct PolarParams {
+  int dtype;
+  const void* G;       // (batch, m, n), strides below
+  int64_t bs, rs, cs;
+  void* out;           // (batch, m, n) contiguous
+  int64_t batch, m, n;
+  const float* coef;   // host, steps x 3
+  int steps;
+  double eps;
+  void* ws;
+};
+size_t polar_ws_bytes(const PolarParams& p);
+cudaError_t launch_polar(const PolarParams& p, cudaStream_t s);
+
+}  // namespace b2c

@@ -1,0 +1,205 @@
+// extern "C" boundary of the products with an epilogue and of the
+// Newton-Schulz orthogonalisation (declared in include/b2c.h).
+#include <cmath>
+#include <cstdio>
+
+#include "b2c_kernels.cuh"
+#include "gemm.cuh"
+
+namespace {
+
+using namespace b2c;
+
+constexpr int64_t kMaxDim = (int64_t)1 << 30;
+constexpr int64_t kMaxPolarDim = (int64_t)1 << 20;
+constexpr int kMaxSteps = 64;
+constexpr double kMaxSigma = 3.5;
+
+int err(int code, const char* name, const char* what) {
+  char buf[256];
+  snprintf(buf, sizeof(buf), "%s: %s", name, what);
+  return set_error(code, buf);
+}
+
+int cuda_err(cudaError_t e, const char* name) {
+  if (e == cudaErrorInvalidConfiguration) return err(B2C_ERR_UNSUPPORTED, name, "more tiles than one launch holds");
+  char buf[256];
+  snprintf(buf, sizeof(buf), "%s (%s)", cudaGetErrorName(e), cudaGetErrorString(e));
+  return err(B2C_ERR_CUDA, name, buf);
+}
+
+bool dtype_ok(int dtype) { return dtype >= B2C_F32 && dtype <= B2C_F16; }
+bool strides_ok(const b2c_matrix& m) { return m.batch_stride >= 0 && m.row_stride >= 0 && m.col_stride >= 0; }
+
+GemmProblem problem(int dtype, const b2c_matrix* A, const b2c_matrix* B, int64_t batch, int64_t M, int64_t K, int64_t N) {
+  GemmProblem g{};
+  g.dtype = dtype;
+  g.batch = batch;
+  g.I = M;
+  g.J = N;
+  g.K = K;
+  g.P = GemmOperand{A->ptr, A->batch_stride, A->row_stride, A->col_stride};
+  g.Q = GemmOperand{B->ptr, B->batch_stride, B->col_stride, B->row_stride};
+  return g;
+}
+
+// The largest |a s + b s^3 + c s^5| over s in [0, hi].
+double poly_bound(double a, double b, double c, double hi) {
+  auto at = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
+  double best = at(hi);
+  // stationary points: a + 3 b t + 5 c t^2 = 0 with t = s^2
+  double roots[2];
+  int n = 0;
+  if (c != 0.0) {
+    const double disc = 9 * b * b - 20 * a * c;
+    if (disc >= 0) {
+      const double q = sqrt(disc);
+      roots[n++] = (-3 * b + q) / (10 * c);
+      roots[n++] = (-3 * b - q) / (10 * c);
+    }
+  } else if (b != 0.0) {
+    roots[n++] = -a / (3 * b);
+  }
+  for (int i = 0; i < n; ++i)
+    if (roots[i] > 0 && sqrt(roots[i]) < hi) best = fmax(best, at(sqrt(roots[i])));
+  return best;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b2c_gemm_workspace_size(int dtype, const b2c_matrix* A, const b2c_matrix* B, int64_t batch, int64_t M,
+                               int64_t K, int64_t N) {
+  (void)dtype, (void)A, (void)B, (void)batch, (void)M, (void)K, (void)N;
+  return 0;
+}
+
+int b2c_gemm(int dtype, const b2c_matrix* A, const b2c_matrix* B, const void* bias, const b2c_matrix* R, void* Y,
+             void* pre, int64_t batch, int64_t M, int64_t K, int64_t N, float alpha, float beta, int activation,
+             void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "b2c_gemm";
+  (void)workspace, (void)workspace_bytes;
+  if (!dtype_ok(dtype)) return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown dtype");
+  if (activation < B2C_ACT_NONE || activation > B2C_ACT_SILU)
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown activation");
+  if (batch < 0 || M < 0 || K < 0 || N < 0) return err(B2C_ERR_INVALID_ARGUMENT, name, "sizes must be >= 0");
+  if (M > kMaxDim || K > kMaxDim || N > kMaxDim) return err(B2C_ERR_UNSUPPORTED, name, "M, K and N are limited to 2^30");
+  if (!A || !B) return err(B2C_ERR_INVALID_ARGUMENT, name, "A and B must be non-NULL");
+  if (!strides_ok(*A) || !strides_ok(*B) || (R && !strides_ok(*R)))
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "strides must be >= 0");
+  if (batch == 0 || M == 0 || N == 0) return set_error(B2C_OK, "");
+  if (!Y || (K > 0 && (!A->ptr || !B->ptr)) || (R && !R->ptr))
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "A, B, R and Y must point to data");
+  GemmProblem g = problem(dtype, A, B, batch, M, K, N);
+  g.e.y = GemmView{Y, M * N, N, 1};
+  g.e.pre = GemmView{pre, M * N, N, 1};
+  if (R) g.e.res = GemmView{const_cast<void*>(R->ptr), R->batch_stride, R->row_stride, R->col_stride};
+  g.e.bias = bias;
+  g.e.alpha = alpha;
+  g.e.beta = beta;
+  g.e.act = activation;
+  const cudaError_t e = launch_gemm_simt(g, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
+}
+
+size_t b2c_gemm_dact_workspace_size(int64_t batch, int64_t M, int64_t N) {
+  if (batch <= 0 || M <= 0 || N <= 0 || M > kMaxDim || N > kMaxDim) return 0;
+  return dact_ws_floats(batch, M, N) * sizeof(float);
+}
+
+int b2c_gemm_dact(int dtype, const b2c_matrix* dY, const b2c_matrix* pre, int activation, float beta, void* dP,
+                  void* dbias, void* dR, int64_t batch, int64_t M, int64_t N, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  const char* name = "b2c_gemm_dact";
+  if (!dtype_ok(dtype)) return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown dtype");
+  if (activation < B2C_ACT_NONE || activation > B2C_ACT_SILU)
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown activation");
+  if (batch < 0 || M < 0 || N < 0) return err(B2C_ERR_INVALID_ARGUMENT, name, "sizes must be >= 0");
+  if (M > kMaxDim || N > kMaxDim) return err(B2C_ERR_UNSUPPORTED, name, "M and N are limited to 2^30");
+  if (!dY || !strides_ok(*dY) || (pre && !strides_ok(*pre)))
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "dY must be non-NULL and strides >= 0");
+  if (activation != B2C_ACT_NONE && !pre)
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "an activation's gradient needs pre");
+  if (N == 0 || (!dP && !dbias && !dR)) return set_error(B2C_OK, "");
+  const bool empty = batch == 0 || M == 0;
+  if (empty && !dbias) return set_error(B2C_OK, "");
+  if (!empty && (!dY->ptr || (activation != B2C_ACT_NONE && !pre->ptr)))
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "dY and pre must point to data");
+  DactParams p{};
+  p.dtype = dtype;
+  p.act = activation;
+  p.dY = dY->ptr;
+  p.dy_bs = dY->batch_stride, p.dy_rs = dY->row_stride, p.dy_cs = dY->col_stride;
+  if (activation != B2C_ACT_NONE) {
+    p.pre = pre->ptr;
+    p.pre_bs = pre->batch_stride, p.pre_rs = pre->row_stride, p.pre_cs = pre->col_stride;
+  }
+  p.dP = dP;
+  p.dbias = dbias;
+  p.dR = dR;
+  p.beta = beta;
+  p.batch = batch;
+  p.M = M;
+  p.N = N;
+  p.ws = static_cast<float*>(workspace);
+  const size_t need = dbias ? dact_ws_floats(batch, M, N) * sizeof(float) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return err(B2C_ERR_WORKSPACE, name, "workspace too small");
+  const cudaError_t e = launch_gemm_dact(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
+}
+
+static PolarParams polar_params(int dtype, const b2c_matrix* G, int64_t batch, int64_t m, int64_t n) {
+  PolarParams p{};
+  p.dtype = dtype;
+  p.G = G->ptr;
+  p.bs = G->batch_stride, p.rs = G->row_stride, p.cs = G->col_stride;
+  p.batch = batch;
+  p.m = m;
+  p.n = n;
+  return p;
+}
+
+size_t b2c_orthogonalize_workspace_size(int dtype, const b2c_matrix* G, int64_t batch, int64_t m, int64_t n) {
+  if (!dtype_ok(dtype) || !G || batch <= 0 || m <= 0 || n <= 0 || m > kMaxPolarDim || n > kMaxPolarDim) return 0;
+  return polar_ws_bytes(polar_params(dtype, G, batch, m, n));
+}
+
+int b2c_orthogonalize(int dtype, const b2c_matrix* G, void* out, int64_t batch, int64_t m, int64_t n,
+                      const double* coefficients, int steps, double eps, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  const char* name = "b2c_orthogonalize";
+  if (!dtype_ok(dtype)) return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown dtype");
+  if (batch < 0 || m < 0 || n < 0) return err(B2C_ERR_INVALID_ARGUMENT, name, "sizes must be >= 0");
+  if (m > kMaxPolarDim || n > kMaxPolarDim) return err(B2C_ERR_UNSUPPORTED, name, "m and n are limited to 2^20");
+  if (steps < 1 || steps > kMaxSteps) return err(B2C_ERR_INVALID_ARGUMENT, name, "steps must be 1 to 64");
+  if (!coefficients) return err(B2C_ERR_INVALID_ARGUMENT, name, "coefficients must be non-NULL");
+  if (!(eps >= 0.0) || std::isinf(eps)) return err(B2C_ERR_INVALID_ARGUMENT, name, "eps must be finite and >= 0");
+  if (!G || !strides_ok(*G)) return err(B2C_ERR_INVALID_ARGUMENT, name, "G must be non-NULL and its strides >= 0");
+  float coef[3 * kMaxSteps];
+  double hi = 1.0;
+  for (int t = 0; t < steps; ++t) {
+    const double *c = coefficients + 3 * t;
+    for (int i = 0; i < 3; ++i) {
+      if (!std::isfinite(c[i])) return err(B2C_ERR_INVALID_ARGUMENT, name, "coefficients must be finite");
+      coef[3 * t + i] = (float)c[i];
+    }
+    hi = poly_bound(c[0], c[1], c[2], hi);
+    if (!(hi <= kMaxSigma))
+      return err(B2C_ERR_INVALID_ARGUMENT, name, "the coefficients let singular values grow past 3.5");
+  }
+  if (batch == 0 || m == 0 || n == 0) return set_error(B2C_OK, "");
+  if (!G->ptr || !out) return err(B2C_ERR_INVALID_ARGUMENT, name, "G and out must point to data");
+  PolarParams p = polar_params(dtype, G, batch, m, n);
+  p.out = out;
+  p.coef = coef;
+  p.steps = steps;
+  p.eps = eps;
+  p.ws = workspace;
+  const size_t need = polar_ws_bytes(p);
+  if (need && (!workspace || workspace_bytes < need)) return err(B2C_ERR_WORKSPACE, name, "workspace too small");
+  const cudaError_t e = launch_polar(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
+}
+
+}  // extern "C"

@@ -17,6 +17,13 @@ batched Cholesky path:
     TruncatedSVD        and its sklearn-style wrapper (_svd.py)
     solve_cholesky      alias of solve (the reference's small-kernel solve)
 
+products with an epilogue, their gradients, and the orthogonalisation that is
+built of them (float32, bfloat16 or float16; no counterpart in the reference):
+
+    gemm(A, B, ...)     act(alpha A B + bias) + beta residual
+    gemm_grad(dY, ...)  its gradients
+    orthogonalize(G)    Newton-Schulz iteration towards G's polar factor
+
 plus one fused extension, ``cho_solve_logdet(A, b, return_L=False)``, which
 returns x and logdet (and L) from ONE pass over A — the reference needs a
 separate factorisation for each of cholesky, solve and logdet_spd.
@@ -46,7 +53,7 @@ from .. import _lib
 
 __all__ = [
     "solve", "cholesky", "solve_cholesky", "solve_lu", "qr", "tril_solve", "triu_solve", "det", "slogdet", "logdet_spd",
-    "cho_solve_logdet", "randomized_svd", "TruncatedSVD", "MAX_GPU_K", "SHARED_K_MAX",
+    "cho_solve_logdet", "gemm", "gemm_grad", "orthogonalize", "randomized_svd", "TruncatedSVD", "MAX_GPU_K", "SHARED_K_MAX",
 ]
 
 # Reference constants (src/mlx_addons/linalg/_metal_kernels.py:19-20). They
@@ -415,4 +422,6 @@ def det(A):
     return sign * torch.exp(lad)
 
 
+from ._gemm import gemm, gemm_grad  # noqa: E402
+from ._polar import orthogonalize  # noqa: E402
 from ._svd import TruncatedSVD, randomized_svd  # noqa: E402  (uses the device helpers above)
