@@ -4,7 +4,7 @@
 #include <cstdio>
 
 #include "b2c_kernels.cuh"
-#include "gemm.cuh"
+#include "gemm_tc.cuh"
 
 namespace {
 
@@ -16,7 +16,7 @@ constexpr int kMaxSteps = 64;
 constexpr double kMaxSigma = 3.5;
 
 int err(int code, const char* name, const char* what) {
-  char buf[256];
+  char buf[400];
   snprintf(buf, sizeof(buf), "%s: %s", name, what);
   return set_error(code, buf);
 }
@@ -41,6 +41,54 @@ GemmProblem problem(int dtype, const b2c_matrix* A, const b2c_matrix* B, int64_t
   g.P = GemmOperand{A->ptr, A->batch_stride, A->row_stride, A->col_stride};
   g.Q = GemmOperand{B->ptr, B->batch_stride, B->col_stride, B->row_stride};
   return g;
+}
+
+// Which kernel takes a product, and what has to be copied for it.
+struct GemmChoice {
+  GemmProblem g;
+  bool tc;
+  PackPlan pack_p, pack_q;
+  size_t ws() const { return tc ? (size_t)(pack_p.bytes + pack_q.bytes) : 0; }
+};
+
+GemmChoice choose(const GemmProblem& in) {
+  GemmChoice c{};
+  c.g = in;
+  if (in.I <= 64 && in.J > in.I) {  // the longer side takes the 128 rows of a tile
+    GemmProblem& g = c.g;
+    g.P = in.Q, g.Q = in.P;
+    g.I = in.J, g.J = in.I;
+    for (GemmView* v : {&g.e.y, &g.e.pre, &g.e.res}) {
+      const int64_t t = v->is;
+      v->is = v->js, v->js = t;
+    }
+    g.e.bias_on_i = !in.e.bias_on_i;
+  }
+  c.tc = in.K >= 32 && (double)in.I * (double)in.J * (double)in.K * (double)in.batch > 1048576.0;
+  if (c.tc) {
+    c.pack_p = plan_pack(in.dtype, c.g.P, in.batch, c.g.I, in.K);
+    c.pack_q = plan_pack(in.dtype, c.g.Q, in.batch, c.g.J, in.K);
+  }
+  return c;
+}
+
+cudaError_t launch_gemm(const GemmChoice& c, void* ws, cudaStream_t s) {
+  const GemmProblem& g = c.g;
+  if (!c.tc) return launch_gemm_simt(g, s);
+  TcProblem t{};
+  cudaError_t e;
+  char* w = static_cast<char*>(ws);
+  if (!c.pack_p.needed) tc_direct(g.P, g.batch, g.I, g.K, &t.P);
+  else if ((e = launch_pack(g.dtype, g.P, c.pack_p, w, &t.P, s)) != cudaSuccess) return e;
+  if (!c.pack_q.needed) tc_direct(g.Q, g.batch, g.J, g.K, &t.Q);
+  else if ((e = launch_pack(g.dtype, g.Q, c.pack_q, w + c.pack_p.bytes, &t.Q, s)) != cudaSuccess) return e;
+  t.kind = g.dtype == B2C_F32 ? kThirds : kOne;
+  t.f16 = g.dtype == B2C_F16;
+  t.batch = g.batch;
+  t.I = g.I, t.J = g.J, t.K = g.K;
+  t.e = g.e;
+  t.out = t.res = g.dtype;
+  return launch_gemm_tc(t, s);
 }
 
 // The largest |a s + b s^3 + c s^5| over s in [0, hi].
@@ -71,15 +119,16 @@ extern "C" {
 
 size_t b2c_gemm_workspace_size(int dtype, const b2c_matrix* A, const b2c_matrix* B, int64_t batch, int64_t M,
                                int64_t K, int64_t N) {
-  (void)dtype, (void)A, (void)B, (void)batch, (void)M, (void)K, (void)N;
-  return 0;
+  if (!dtype_ok(dtype) || !A || !B || !strides_ok(*A) || !strides_ok(*B) || batch <= 0 || M <= 0 || K <= 0 || N <= 0 ||
+      M > kMaxDim || K > kMaxDim || N > kMaxDim)
+    return 0;
+  return choose(problem(dtype, A, B, batch, M, K, N)).ws();
 }
 
 int b2c_gemm(int dtype, const b2c_matrix* A, const b2c_matrix* B, const void* bias, const b2c_matrix* R, void* Y,
              void* pre, int64_t batch, int64_t M, int64_t K, int64_t N, float alpha, float beta, int activation,
              void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "b2c_gemm";
-  (void)workspace, (void)workspace_bytes;
   if (!dtype_ok(dtype)) return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown dtype");
   if (activation < B2C_ACT_NONE || activation > B2C_ACT_SILU)
     return err(B2C_ERR_INVALID_ARGUMENT, name, "unknown activation");
@@ -99,7 +148,10 @@ int b2c_gemm(int dtype, const b2c_matrix* A, const b2c_matrix* B, const void* bi
   g.e.alpha = alpha;
   g.e.beta = beta;
   g.e.act = activation;
-  const cudaError_t e = launch_gemm_simt(g, static_cast<cudaStream_t>(stream));
+  const GemmChoice c = choose(g);
+  if (c.ws() && (!workspace || workspace_bytes < c.ws() || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return err(B2C_ERR_WORKSPACE, name, "workspace missing, too small or not on 16 bytes");
+  const cudaError_t e = launch_gemm(c, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
 }
 

@@ -1,0 +1,97 @@
+// Copies of operands for the tensor-core products: rows padded to a multiple
+// of 8 elements, so that every row starts on 16 bytes, and float32 values as
+// three bf16 planes.
+//
+// Bound by HBM. The axis with the smaller stride stays the inner one (the
+// product reads either order), so reads and writes both run along it; a
+// thread takes 8 neighbouring elements and writes each plane's as 16 bytes.
+#include "b2c_kernels.cuh"
+#include "gemm_tc.cuh"
+
+namespace b2c {
+
+namespace {
+
+struct PackParams {
+  const void* src;
+  int64_t bs, os, is;            // strides of batch, outer, inner
+  int64_t batch, outer, inner, pitch, plane;
+  uint16_t* dst;
+};
+
+// Rounds to bf16; a finite value whose nearest is infinite is cut off instead.
+__device__ __forceinline__ uint16_t bf16_finite(float x) {
+  const uint16_t r = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  return (r & 0x7fff) == 0x7f80 ? (uint16_t)(__float_as_uint(x) >> 16) : r;
+}
+__device__ __forceinline__ float bf16_value(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+
+// x as hi + mid + lo, each bf16: the remainders are exact, so the three hold
+// all 24 bits. A non-finite x is its hi plane alone.
+__device__ __forceinline__ void thirds(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
+  if (isfinite(x)) {
+    hi = bf16_finite(x);
+    const float r = x - bf16_value(hi);
+    mid = bf16_finite(r);
+    lo = bf16_finite(r - bf16_value(mid));
+  } else {
+    hi = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+    mid = lo = 0;
+  }
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(256) gemm_pack_kernel(const PackParams p) {
+  const int64_t units = (p.inner + 7) / 8, total = p.batch * p.outer * units;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t row = t / units, u = t - row * units, b = row / p.outer, o = row - b * p.outer;
+    const int64_t src = b * p.bs + o * p.os + u * 8 * p.is, dst = row * p.pitch + u * 8;
+    const int n = (int)(p.inner - u * 8 < 8 ? p.inner - u * 8 : 8);
+    if constexpr (F32) {
+      const float* s = static_cast<const float*>(p.src) + src;
+      __align__(16) uint16_t h[8], m[8], l[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) thirds(c < n ? s[c * p.is] : 0.f, h[c], m[c], l[c]);
+      *reinterpret_cast<uint4*>(p.dst + dst) = *reinterpret_cast<const uint4*>(h);
+      *reinterpret_cast<uint4*>(p.dst + p.plane + dst) = *reinterpret_cast<const uint4*>(m);
+      *reinterpret_cast<uint4*>(p.dst + 2 * p.plane + dst) = *reinterpret_cast<const uint4*>(l);
+    } else {
+      const uint16_t* s = static_cast<const uint16_t*>(p.src) + src;
+      __align__(16) uint16_t h[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) h[c] = c < n ? s[c * p.is] : (uint16_t)0;
+      *reinterpret_cast<uint4*>(p.dst + dst) = *reinterpret_cast<const uint4*>(h);
+    }
+  }
+}
+
+}  // namespace
+
+PackPlan plan_pack(int dtype, const GemmOperand& o, int64_t batch, int64_t rows, int64_t K) {
+  PackPlan r{};
+  TcOperand direct;
+  r.needed = dtype == B2C_F32 || !tc_direct(o, batch, rows, K, &direct);
+  if (!r.needed) return r;
+  const int64_t rs = rows == 1 ? INT64_MAX : o.rs, ks = K == 1 ? INT64_MAX : o.ks;
+  r.rows_inner = rs < ks || (rs == ks && rows > K);
+  r.batch = o.bs == 0 ? 1 : batch;
+  r.outer = r.rows_inner ? K : rows;
+  r.inner = r.rows_inner ? rows : K;
+  r.pitch = (r.inner + 7) / 8 * 8;
+  r.plane = r.batch * r.outer * r.pitch;
+  r.bytes = (r.plane * 2 * (dtype == B2C_F32 ? 3 : 1) + 255) / 256 * 256;
+  return r;
+}
+
+cudaError_t launch_pack(int dtype, const GemmOperand& o, const PackPlan& plan, void* dst, TcOperand* out, cudaStream_t s) {
+  const PackParams p{o.p, o.bs, plan.rows_inner ? o.ks : o.rs, plan.rows_inner ? o.rs : o.ks, plan.batch, plan.outer,
+                     plan.inner, plan.pitch, plan.plane, static_cast<uint16_t*>(dst)};
+  const int64_t total = plan.batch * plan.outer * ((plan.inner + 7) / 8), blocks = (total + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+  if (dtype == B2C_F32) gemm_pack_kernel<true><<<grid, 256, 0, s>>>(p);
+  else gemm_pack_kernel<false><<<grid, 256, 0, s>>>(p);
+  *out = TcOperand{dst, plan.outer * plan.pitch, plan.pitch, plan.plane, plan.rows_inner, plan.batch == 1};
+  return cudaGetLastError();
+}
+
+}  // namespace b2c

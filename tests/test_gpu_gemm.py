@@ -64,6 +64,19 @@ def _plain(A, B):
     return y, ey
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ta,tb", [(False, False), (False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("M,K,N,batch", [(1700, 328, 1608, 0), (2048, 64, 2048, 0), (1601, 200, 1793, 0), (300, 136, 520, 13),
+                                         (256, 512, 256, 60)])
+def test_many_tiles(M, K, N, batch, ta, tb, dtype):
+    """Sizes that fill the GPU with the largest tiles, their edges ragged."""
+    A, B, bias, R = _problem(M, K, N, dtype, (batch,) if batch else (), shared=not batch, trans_a=ta, trans_b=tb)
+    Y, pre = la.gemm(A, B, bias, "gelu", R, return_pre=True)
+    y, p, ey, ep = gemm64(A, B, bias, "gelu", R)
+    check(pre, p, ep, "pre", K)
+    check(Y, y, ey, "Y", K)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N", [(1, 96), (70, 40), (160, 144)])
