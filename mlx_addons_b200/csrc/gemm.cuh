@@ -142,6 +142,8 @@ struct PolarParams {
   double eps;
   void* ws;
 };
+// The largest |a v + b v^3 + c v^5| over v in [0, hi].
+double polar_poly_bound(double a, double b, double c, double hi);
 size_t polar_ws_bytes(const PolarParams& p);
 cudaError_t launch_polar(const PolarParams& p, cudaStream_t s);
 

@@ -91,28 +91,6 @@ cudaError_t launch_gemm(const GemmChoice& c, void* ws, cudaStream_t s) {
   return launch_gemm_tc(t, s);
 }
 
-// The largest |a s + b s^3 + c s^5| over s in [0, hi].
-double poly_bound(double a, double b, double c, double hi) {
-  auto at = [&](double s) { return fabs(s * (a + s * s * (b + c * s * s))); };
-  double best = at(hi);
-  // stationary points: a + 3 b t + 5 c t^2 = 0 with t = s^2
-  double roots[2];
-  int n = 0;
-  if (c != 0.0) {
-    const double disc = 9 * b * b - 20 * a * c;
-    if (disc >= 0) {
-      const double q = sqrt(disc);
-      roots[n++] = (-3 * b + q) / (10 * c);
-      roots[n++] = (-3 * b - q) / (10 * c);
-    }
-  } else if (b != 0.0) {
-    roots[n++] = -a / (3 * b);
-  }
-  for (int i = 0; i < n; ++i)
-    if (roots[i] > 0 && sqrt(roots[i]) < hi) best = fmax(best, at(sqrt(roots[i])));
-  return best;
-}
-
 }  // namespace
 
 extern "C" {
@@ -236,7 +214,7 @@ int b2c_orthogonalize(int dtype, const b2c_matrix* G, void* out, int64_t batch, 
       if (!std::isfinite(c[i])) return err(B2C_ERR_INVALID_ARGUMENT, name, "coefficients must be finite");
       coef[3 * t + i] = (float)c[i];
     }
-    hi = poly_bound(c[0], c[1], c[2], hi);
+    hi = polar_poly_bound(c[0], c[1], c[2], hi);
     if (!(hi <= kMaxSigma))
       return err(B2C_ERR_INVALID_ARGUMENT, name, "the coefficients let singular values grow past 3.5");
   }
@@ -249,7 +227,8 @@ int b2c_orthogonalize(int dtype, const b2c_matrix* G, void* out, int64_t batch, 
   p.eps = eps;
   p.ws = workspace;
   const size_t need = polar_ws_bytes(p);
-  if (need && (!workspace || workspace_bytes < need)) return err(B2C_ERR_WORKSPACE, name, "workspace too small");
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return err(B2C_ERR_WORKSPACE, name, "workspace missing, too small or not on 16 bytes");
   const cudaError_t e = launch_polar(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
 }

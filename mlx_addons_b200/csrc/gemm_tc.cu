@@ -40,7 +40,9 @@ namespace {
 constexpr int BM = 128;          // rows of D per CTA
 constexpr int BK = 64;           // depth of a slice: 128 bytes
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kThreads = (kEpiWarps + 4) * 32;  // the last warpgroup: loads, products, two idle warps
+// Registers: 384 x 168 at launch = 128 x 72 + 256 x 216 after the split.
+constexpr int kRegsFew = 72, kRegsMany = 216;
 constexpr int kMaxStages = 8;
 constexpr int kChunk = 4;        // slices of k per joined accumulator
 constexpr int kMaxSeg = 6;
@@ -444,65 +446,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
   volatile int* gu = &gave_up;
 
-  if (warp == kEpiWarps && lane == 0) {
-    // ---- loads ----
-    const uint32_t lead_full0 = CG == 2 ? map_rank(full0, 0) : full0;
-    uint32_t s = 0, phase = 0;
-    for (int64_t t = first; t < p.tiles && !*gu; t += step) {
-      const Tile o = tile_at<CG>(p, t);
-      const int i0 = (int)(o.i + rank * BM), j0 = (int)(o.j + rank * p.share);
-      const int bp = p.p_bcast ? 0 : (int)o.b, bq = p.q_bcast ? 0 : (int)o.b;
-      for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
-        const int c1 = min(c0 + p.chunk, p.kblocks);
-        for (int g = 0; g < p.nseg; ++g) {
-          for (int kb = c0; kb < c1; ++kb) {
-            if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit)) break;
-            if (rank == 0) bar_expect(full0 + 8 * s, CG * stage_bytes);
-            const uint32_t bar = lead_full0 + 8 * s, a = smem_u32(ring + s * stage_bytes), q = a + p.a_bytes;
-            if (p.p_inner) {
-              tma_load<CG>(a, &map_p, i0, kb * BK, bp, p.seg_p[g], bar);
-              tma_load<CG>(a + 8192, &map_p, i0 + 64, kb * BK, bp, p.seg_p[g], bar);
-            } else {
-              tma_load<CG>(a, &map_p, kb * BK, i0, bp, p.seg_p[g], bar);
-            }
-            if (p.q_inner) {
-              for (int h = 0; h < p.b_bytes / 8192; ++h)
-                tma_load<CG>(q + h * 8192, &map_q, j0 + 64 * h, kb * BK, bq, p.seg_q[g], bar);
-            } else {
-              tma_load<CG>(q, &map_q, kb * BK, j0, bq, p.seg_q[g], bar);
-            }
-            if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
-          }
-        }
-      }
-    }
-  } else if (warp == kEpiWarps + 1 && rank == 0 && lane == 0) {
-    // ---- products ----
-    uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
-    const uint32_t step_p = p.p_inner ? 2048 >> 4 : 32 >> 4, step_q = p.q_inner ? 2048 >> 4 : 32 >> 4;
-    for (int64_t t = first; t < p.tiles && !*gu; t += step) {
-      for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
-        const int n = (min(c0 + p.chunk, p.kblocks) - c0) * p.nseg;
-        if (!bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit)) break;
-        fence_after();
-        const uint32_t d = tmem + buf * 256;
-        for (int it = 0; it < n; ++it) {
-          if (!bar_wait(full0 + 8 * s, phase, gu, limit)) break;
-          fence_after();
-          const uint32_t a = smem_u32(ring + s * stage_bytes);
-          const uint64_t da = tile_desc(a, p.p_inner), dq = tile_desc(a + p.a_bytes, p.q_inner);
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            mma<CG>(d, da + kk * step_p, dq + kk * step_q, p.idesc, it > 0 || kk > 0);
-          commit<CG>(empty0 + 8 * s);
-          if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
-        }
-        if (*gu) break;
-        commit<CG>(tfull0 + 8 * buf);
-        if (++buf == 2) buf = 0, tphase ^= 1;
-      }
-    }
-  } else if (warp < kEpiWarps) {
+  if (warp < kEpiWarps) {
+    if constexpr (JOIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     // ---- epilogue: warps w and w + 4 share the rows 32 (w % 4).., and take every other 32 columns ----
     const int quad = warp & 3, half = warp >> 2;
     const uint32_t lead_tempty0 = CG == 2 ? map_rank(tempty0, 0) : tempty0;
@@ -570,6 +515,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (half * 32 >= p.BN && lane == 0) bar_arrive_cluster(lead_tempty0 + 8 * buf);
         if (++buf == 2) buf = 0, tphase ^= 1;
+      }
+    }
+  } else {
+    if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+    if (warp == kEpiWarps && lane == 0) {
+      // ---- loads ----
+      const uint32_t lead_full0 = CG == 2 ? map_rank(full0, 0) : full0;
+      uint32_t s = 0, phase = 0;
+      for (int64_t t = first; t < p.tiles && !*gu; t += step) {
+        const Tile o = tile_at<CG>(p, t);
+        const int i0 = (int)(o.i + rank * BM), j0 = (int)(o.j + rank * p.share);
+        const int bp = p.p_bcast ? 0 : (int)o.b, bq = p.q_bcast ? 0 : (int)o.b;
+        for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
+          const int c1 = min(c0 + p.chunk, p.kblocks);
+          for (int g = 0; g < p.nseg; ++g) {
+            for (int kb = c0; kb < c1; ++kb) {
+              if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit)) break;
+              if (rank == 0) bar_expect(full0 + 8 * s, CG * stage_bytes);
+              const uint32_t bar = lead_full0 + 8 * s, a = smem_u32(ring + s * stage_bytes), q = a + p.a_bytes;
+              if (p.p_inner) {
+                tma_load<CG>(a, &map_p, i0, kb * BK, bp, p.seg_p[g], bar);
+                tma_load<CG>(a + 8192, &map_p, i0 + 64, kb * BK, bp, p.seg_p[g], bar);
+              } else {
+                tma_load<CG>(a, &map_p, kb * BK, i0, bp, p.seg_p[g], bar);
+              }
+              if (p.q_inner) {
+                for (int h = 0; h < p.b_bytes / 8192; ++h)
+                  tma_load<CG>(q + h * 8192, &map_q, j0 + 64 * h, kb * BK, bq, p.seg_q[g], bar);
+              } else {
+                tma_load<CG>(q, &map_q, kb * BK, j0, bq, p.seg_q[g], bar);
+              }
+              if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
+            }
+          }
+        }
+      }
+    } else if (warp == kEpiWarps + 1 && rank == 0 && lane == 0) {
+      // ---- products ----
+      uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
+      const uint32_t step_p = p.p_inner ? 2048 >> 4 : 32 >> 4, step_q = p.q_inner ? 2048 >> 4 : 32 >> 4;
+      for (int64_t t = first; t < p.tiles && !*gu; t += step) {
+        for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
+          const int n = (min(c0 + p.chunk, p.kblocks) - c0) * p.nseg;
+          if (!bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit)) break;
+          fence_after();
+          const uint32_t d = tmem + buf * 256;
+          for (int it = 0; it < n; ++it) {
+            if (!bar_wait(full0 + 8 * s, phase, gu, limit)) break;
+            fence_after();
+            const uint32_t a = smem_u32(ring + s * stage_bytes);
+            const uint64_t da = tile_desc(a, p.p_inner), dq = tile_desc(a + p.a_bytes, p.q_inner);
+  #pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk)
+              mma<CG>(d, da + kk * step_p, dq + kk * step_q, p.idesc, it > 0 || kk > 0);
+            commit<CG>(empty0 + 8 * s);
+            if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
+          }
+          if (*gu) break;
+          commit<CG>(tfull0 + 8 * buf);
+          if (++buf == 2) buf = 0, tphase ^= 1;
+        }
       }
     }
   }

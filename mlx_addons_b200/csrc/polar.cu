@@ -5,13 +5,16 @@
 // taken on the smaller side (for a tall G, S = X^T X and X <- a X + X (b S +
 // c S S)), so S has min(m, n) rows. Each step is three products with an
 // epilogue: S; P = c S S + b S; X' = P X + a X.
+#include <cmath>
+
 #include "b2c_kernels.cuh"
-#include "gemm.cuh"
+#include "gemm_tc.cuh"
 
 namespace b2c {
 
 namespace {
 
+constexpr float kScaleX = 16384.f;
 constexpr int kNormThreads = 256;
 constexpr int kNormParts = 64;  // partial sums of a matrix, added in a fixed order
 
@@ -48,35 +51,64 @@ __global__ void __launch_bounds__(kNormThreads) polar_norm_kernel(const PolarIn 
   }
 }
 
-template <typename T>
+// X = G / (|G|_F + eps) times 2^14, as one or two f16 planes.
+template <typename T, bool HALVES>
 __global__ void __launch_bounds__(kNormThreads) polar_scale_kernel(const PolarIn in, const double* part, int parts,
-                                                                   double eps, float* X) {
+                                                                   double eps, __half* X, int64_t pitch, int64_t plane) {
   const int64_t total = in.m * in.n;
   for (int64_t b = blockIdx.y; b < in.batch; b += gridDim.y) {
-  const T* base = static_cast<const T*>(in.G) + b * in.bs;
-  double s = 0.0;
-  for (int i = 0; i < parts; ++i) s += part[b * kNormParts + i];
-  const double inv = 1.0 / (sqrt(s) + eps);
-  for (int64_t e = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kNormThreads) {
-    const int64_t r = e / in.n, c = e - r * in.n;
-    X[b * total + e] = (float)((double)to_f32(base[r * in.rs + c * in.cs]) * inv);
-  }
+    const T* base = static_cast<const T*>(in.G) + b * in.bs;
+    double s = 0.0;
+    for (int i = 0; i < parts; ++i) s += part[b * kNormParts + i];
+    const double inv = kScaleX / (sqrt(s) + eps);
+    for (int64_t e = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; e < total;
+         e += (int64_t)gridDim.x * kNormThreads) {
+      const int64_t r = e / in.n, c = e - r * in.n, at = (b * in.m + r) * pitch + c;
+      const float x = (float)((double)to_f32(base[r * in.rs + c * in.cs]) * inv);
+      const __half hi = __float2half_rn(x);
+      X[at] = hi;
+      if constexpr (HALVES) X[plane + at] = __float2half_rn(x - __half2float(hi));
+    }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) polar_round_kernel(const float* X, void* out, int64_t total) {
-  for (int64_t e = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kNormThreads)
-    static_cast<T*>(out)[e] = from_f32<T>(X[e]);
+// Scratch of the product form: norms, two X, S and P.
+struct PolarLayout {
+  int64_t side, pitch_x, pitch_s, x_plane, s_plane, x_bytes, s_bytes, part_bytes;
+  int planes;
+};
+
+PolarLayout polar_layout(const PolarParams& p) {
+  PolarLayout l;
+  l.side = p.m < p.n ? p.m : p.n;
+  l.planes = p.dtype == B2C_BF16 ? 1 : 2;
+  l.pitch_x = (p.n + 7) / 8 * 8;
+  l.pitch_s = (l.side + 7) / 8 * 8;
+  l.x_plane = p.batch * p.m * l.pitch_x;
+  l.s_plane = p.batch * l.side * l.pitch_s;
+  l.x_bytes = (l.x_plane * l.planes * 2 + 255) / 256 * 256;
+  l.s_bytes = (l.s_plane * l.planes * 2 + 255) / 256 * 256;
+  l.part_bytes = (p.batch * kNormParts * (int64_t)sizeof(double) + 255) / 256 * 256;
+  return l;
+}
+
+// The largest power of two that keeps values up to `bound` within f16's 2^15.
+float scale_for(double bound) {
+  const double b = bound < 1e-3 ? 1e-3 : bound;
+  return (float)exp2(floor(log2(32768.0 / b)));
 }
 
 template <typename T>
 cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
-  const int64_t mn = p.m * p.n, side = p.m < p.n ? p.m : p.n, ss = side * side;
+  const PolarLayout l = polar_layout(p);
+  const int64_t mn = p.m * p.n, side = l.side;
   char* w = static_cast<char*>(p.ws);
   double* part = reinterpret_cast<double*>(w);
-  float* X0 = reinterpret_cast<float*>(w + p.batch * kNormParts * sizeof(double));
-  float *X1 = X0 + p.batch * mn, *S = X1 + p.batch * mn, *P = S + p.batch * ss;
+  w += l.part_bytes;
+  __half* X0 = reinterpret_cast<__half*>(w);
+  __half* X1 = reinterpret_cast<__half*>(w + l.x_bytes);
+  __half* S = reinterpret_cast<__half*>(w + 2 * l.x_bytes);
+  __half* P = reinterpret_cast<__half*>(w + 2 * l.x_bytes + l.s_bytes);
   const PolarIn in{p.G, p.bs, p.rs, p.cs, p.batch, p.m, p.n};
   int64_t blocks = (mn + kNormThreads - 1) / kNormThreads;
   const int parts = (int)(blocks < kNormParts ? blocks : kNormParts);
@@ -84,59 +116,94 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   const unsigned by = (unsigned)(p.batch < 65535 ? p.batch : 65535);
   const dim3 gn((unsigned)parts, by), gs((unsigned)blocks, by);
   polar_norm_kernel<T><<<gn, kNormThreads, 0, s>>>(in, part);
-  polar_scale_kernel<T><<<gs, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0);
+  constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
+  polar_scale_kernel<T, kTwo><<<gs, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0, l.pitch_x, l.x_plane);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
+
   const bool wide = p.m <= p.n;
-  const int64_t n = p.n;
-  for (int t = 0; t < p.steps; ++t) {
-    const float a = p.coef[3 * t], b = p.coef[3 * t + 1], c = p.coef[3 * t + 2];
-    GemmProblem g{};
-    g.dtype = B2C_F32;
-    g.batch = p.batch;
-    g.I = g.J = side;
-    g.K = wide ? p.n : p.m;
-    g.P = wide ? GemmOperand{X0, mn, n, 1} : GemmOperand{X0, mn, 1, n};
-    g.Q = g.P;
-    g.e.y = GemmView{S, ss, side, 1};
-    g.e.alpha = 1.f;
-    if ((e = launch_gemm_simt(g, s)) != cudaSuccess) return e;
-    g.K = side;
-    g.P = g.Q = GemmOperand{S, ss, side, 1};
-    g.e.y = GemmView{P, ss, side, 1};
-    g.e.res = GemmView{S, ss, side, 1};
-    g.e.alpha = c;
-    g.e.beta = b;
-    if ((e = launch_gemm_simt(g, s)) != cudaSuccess) return e;
-    g.I = p.m;
-    g.J = p.n;
-    // P is symmetric: either index may be the contracted one
-    if (wide) {
-      g.P = GemmOperand{P, ss, side, 1};
-      g.Q = GemmOperand{X0, mn, 1, n};
-    } else {
-      g.P = GemmOperand{X0, mn, n, 1};
-      g.Q = GemmOperand{P, ss, side, 1};
-    }
-    g.e.y = GemmView{X1, mn, n, 1};
-    g.e.res = GemmView{X0, mn, n, 1};
-    g.e.alpha = 1.f;
-    g.e.beta = a;
-    if ((e = launch_gemm_simt(g, s)) != cudaSuccess) return e;
-    float* sw = X0;
+  const int inner = kTwo ? kOutHalves : B2C_F16;
+  TcProblem t{};
+  t.kind = kTwo ? kHalves : kOne;
+  t.f16 = 1;
+  t.batch = p.batch;
+  const int bcast = p.batch == 1;
+  const int64_t sx = side * l.pitch_s, xx = p.m * l.pitch_x;
+  const TcOperand s_op{S, sx, l.pitch_s, l.s_plane, 0, bcast}, p_op{P, sx, l.pitch_s, l.s_plane, 0, bcast};
+  double hi = 1.0;
+  for (int step = 0; step < p.steps; ++step) {
+    const double a = p.coef[3 * step], b = p.coef[3 * step + 1], c = p.coef[3 * step + 2], t2 = hi * hi;
+    const float ss = scale_for(t2), sp = scale_for(fabs(b) * t2 + fabs(c) * t2 * t2);
+    const TcOperand x_rows{X0, xx, l.pitch_x, l.x_plane, 0, bcast}, x_cols{X0, xx, l.pitch_x, l.x_plane, 1, bcast};
+    // S = X X^T (X^T X), the lower half of its tiles
+    t.I = t.J = side;
+    t.K = wide ? p.n : p.m;
+    t.P = t.Q = wide ? x_rows : x_cols;
+    t.sym = 1;
+    t.e = GemmEpilogue{};
+    t.e.y = GemmView{S, sx, l.pitch_s, 1};
+    t.e.alpha = ss / (kScaleX * kScaleX);
+    t.out = t.res = inner;
+    t.y_plane = t.res_plane = l.s_plane;
+    if ((e = launch_gemm_tc(t, s)) != cudaSuccess) return e;
+    // P = c S S + b S
+    t.K = side;
+    t.P = t.Q = s_op;
+    t.e.y.p = P;
+    t.e.res = GemmView{S, sx, l.pitch_s, 1};
+    t.e.alpha = (float)(c * sp / ((double)ss * ss));
+    t.e.beta = (float)(b * sp / ss);
+    if ((e = launch_gemm_tc(t, s)) != cudaSuccess) return e;
+    // X' = P X + a X (X P + a X); P is symmetric, so either of its indices may be contracted
+    const bool last = step == p.steps - 1;
+    const float so = last ? 1.f : kScaleX;
+    t.I = p.m;
+    t.J = p.n;
+    t.P = wide ? p_op : x_rows;
+    t.Q = wide ? x_cols : p_op;
+    t.sym = 0;
+    t.e.y = last ? GemmView{p.out, mn, p.n, 1} : GemmView{X1, xx, l.pitch_x, 1};
+    t.e.res = GemmView{X0, xx, l.pitch_x, 1};
+    t.e.alpha = so / (sp * kScaleX);
+    t.e.beta = (float)(a * so / kScaleX);
+    t.out = last ? p.dtype : inner;
+    t.y_plane = last ? 0 : l.x_plane;
+    t.res_plane = l.x_plane;
+    if ((e = launch_gemm_tc(t, s)) != cudaSuccess) return e;
+    __half* sw = X0;
     X0 = X1;
     X1 = sw;
+    hi = polar_poly_bound(a, b, c, hi);
   }
-  const int64_t total = p.batch * mn, rb = (total + kNormThreads - 1) / kNormThreads;
-  polar_round_kernel<T><<<(unsigned)(rb < 8192 ? rb : 8192), kNormThreads, 0, s>>>(X0, p.out, total);
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 }  // namespace
 
+double polar_poly_bound(double a, double b, double c, double hi) {
+  auto at = [&](double v) { return fabs(v * (a + v * v * (b + c * v * v))); };
+  double best = at(hi);
+  // stationary points: a + 3 b t + 5 c t^2 = 0 with t = v^2
+  double roots[2];
+  int n = 0;
+  if (c != 0.0) {
+    const double disc = 9 * b * b - 20 * a * c;
+    if (disc >= 0) {
+      const double q = sqrt(disc);
+      roots[n++] = (-3 * b + q) / (10 * c);
+      roots[n++] = (-3 * b - q) / (10 * c);
+    }
+  } else if (b != 0.0) {
+    roots[n++] = -a / (3 * b);
+  }
+  for (int i = 0; i < n; ++i)
+    if (roots[i] > 0 && sqrt(roots[i]) < hi) best = fmax(best, at(sqrt(roots[i])));
+  return best;
+}
+
 size_t polar_ws_bytes(const PolarParams& p) {
-  const int64_t mn = p.m * p.n, side = p.m < p.n ? p.m : p.n;
-  return (size_t)p.batch * kNormParts * sizeof(double) + (size_t)p.batch * (2 * mn + 2 * side * side) * sizeof(float);
+  const PolarLayout l = polar_layout(p);
+  return (size_t)(l.part_bytes + 2 * l.x_bytes + 2 * l.s_bytes);
 }
 
 cudaError_t launch_polar(const PolarParams& p, cudaStream_t s) {
