@@ -67,31 +67,65 @@ constexpr float kGeluK = 0.044715f;
 constexpr float kRsqrt2 = 0.7071067811865476f;
 constexpr float kRsqrt2Pi = 0.3989422804014327f;  // 1 / sqrt(2 pi)
 
-__device__ __forceinline__ float sigmoid_f32(float x) { return 1.f / (1.f + expf(-x)); }
+// Activations come in two forms: FAST for 16-bit results, on the exponential
+// and reciprocal units (a few 2^-22 relative, far below a 16-bit rounding),
+// and one on the accurate functions for float32.
+template <bool FAST>
+__device__ __forceinline__ float exp_f32(float x) {
+  return FAST ? __expf(x) : expf(x);
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_f32(float x) {
+  return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
+}
+
+// Normal distribution function; bell receives exp(-x^2 / 2). The fast form is
+// Abramowitz and Stegun's 7.1.26 for erfc(|x| / sqrt 2), off by 1.5e-7 at most.
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float x, float& bell) {
+  bell = exp_f32<FAST>(-0.5f * x * x);
+  if constexpr (!FAST) return 0.5f * (1.f + erff(x * kRsqrt2));
+  const float t = __fdividef(1.f, fmaf(0.3275911f * kRsqrt2, fabsf(x), 1.f));
+  float q = fmaf(1.061405429f, t, -1.453152027f);
+  q = fmaf(q, t, 1.421413741f);
+  q = fmaf(q, t, -0.284496736f);
+  q = fmaf(q, t, 0.254829592f);
+  const float tail = 0.5f * q * t * bell;
+  return x < 0.f ? tail : 1.f - tail;
+}
 
 // act(x). NaN stays NaN.
+template <bool FAST>
 __device__ __forceinline__ float act_f32(float x, int act) {
   switch (act) {
     case B2C_ACT_RELU: return x < 0.f ? 0.f : x;
-    case B2C_ACT_GELU: return 0.5f * x * (1.f + erff(x * kRsqrt2));
+    case B2C_ACT_GELU: {
+      float bell;
+      return x * normal_cdf<FAST>(x, bell);
+    }
     // 0.5 x (1 + tanh u) = x sigmoid(2 u)
-    case B2C_ACT_GELU_TANH: return x * sigmoid_f32(2.f * kGeluC * (x + kGeluK * x * x * x));
-    case B2C_ACT_SILU: return x * sigmoid_f32(x);
+    case B2C_ACT_GELU_TANH: return x * sigmoid_f32<FAST>(2.f * kGeluC * (x + kGeluK * x * x * x));
+    case B2C_ACT_SILU: return x * sigmoid_f32<FAST>(x);
     default: return x;
   }
 }
 
 // d act(x) / dx, given the pre-activation.
+template <bool FAST>
 __device__ __forceinline__ float act_slope_f32(float x, int act) {
   switch (act) {
     case B2C_ACT_RELU: return x > 0.f ? 1.f : 0.f;
-    case B2C_ACT_GELU: return 0.5f * (1.f + erff(x * kRsqrt2)) + x * expf(-0.5f * x * x) * kRsqrt2Pi;
+    case B2C_ACT_GELU: {
+      float bell;
+      const float cdf = normal_cdf<FAST>(x, bell);
+      return fmaf(x * kRsqrt2Pi, bell, cdf);
+    }
     case B2C_ACT_GELU_TANH: {
-      const float s = sigmoid_f32(2.f * kGeluC * (x + kGeluK * x * x * x));
+      const float s = sigmoid_f32<FAST>(2.f * kGeluC * (x + kGeluK * x * x * x));
       return s + x * s * (1.f - s) * 2.f * kGeluC * (1.f + 3.f * kGeluK * x * x);
     }
     case B2C_ACT_SILU: {
-      const float s = sigmoid_f32(x);
+      const float s = sigmoid_f32<FAST>(x);
       return s * (1.f + x * (1.f - s));
     }
     default: return 1.f;
@@ -104,7 +138,7 @@ __device__ __forceinline__ void epilogue_store(const GemmEpilogue& e, int64_t b,
   float v = e.alpha * acc;
   if (e.bias) v += to_f32(static_cast<const T*>(e.bias)[e.bias_on_i ? i : j]);
   if (e.pre.p) static_cast<T*>(e.pre.p)[b * e.pre.bs + i * e.pre.is + j * e.pre.js] = from_f32<T>(v);
-  v = act_f32(v, e.act);
+  v = act_f32<sizeof(T) == 2>(v, e.act);
   if (e.res.p) v = fmaf(e.beta, to_f32(static_cast<const T*>(e.res.p)[b * e.res.bs + i * e.res.is + j * e.res.js]), v);
   static_cast<T*>(e.y.p)[b * e.y.bs + i * e.y.is + j * e.y.js] = from_f32<T>(v);
 }
@@ -135,7 +169,8 @@ struct PolarParams {
   int dtype;
   const void* G;       // (batch, m, n), strides below
   int64_t bs, rs, cs;
-  void* out;           // (batch, m, n) contiguous
+  void* out;           // (batch, m, n), contiguous for the caller's m and n
+  int64_t out_rs, out_cs;  // set by launch_polar, which may take G as its transpose
   int64_t batch, m, n;
   const float* coef;   // host, steps x 3
   int steps;

@@ -1,9 +1,10 @@
 // Gradient of a product's epilogue: dP = dY act'(pre), its column sums (the
 // bias gradient) and beta dY (the residual's), in one pass over dY and pre.
 //
-// Bound by HBM: it reads dY and pre and writes dP once. A CTA takes 32
-// columns (one per lane) of a band of rows; its 8 warps walk the band and
-// their float32 column sums join in shared memory, one partial row per band.
+// Bound by HBM: it reads dY and pre and writes dP once. A CTA takes 256
+// columns (8 per lane, as 16-byte accesses where alignment allows) of a band
+// of rows; its 8 warps walk the band and their float32 column sums join in
+// shared memory, one partial row per band.
 // A second kernel adds the bands in a fixed order, so the sums do not depend
 // on which CTA ran first. The sums take dP before it is rounded; dP itself is
 // rounded once to the product's type, since it is an operand of the two
@@ -16,7 +17,8 @@ namespace b2c {
 namespace {
 
 constexpr int kDactWarps = 8;
-constexpr int kMaxBands = 1024;
+constexpr int kCols = 256;      // columns of a CTA: 8 per lane
+constexpr int kMaxBands = 256;
 
 int64_t dact_band_rows(int64_t rows) {
   int64_t band = 64;
@@ -24,35 +26,89 @@ int64_t dact_band_rows(int64_t rows) {
   return band;
 }
 
-template <typename T>
+// VEC: every row of every array starts on 16 bytes and N is a multiple of 8;
+// a lane takes 8 neighbouring columns. Otherwise it takes every 32nd.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const void* p, int64_t off, int64_t cs, int64_t c, int64_t N, float (&v)[8]) {
+  const T* q = static_cast<const T*>(p) + off;
+  if constexpr (VEC) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 8 / PER; ++u) {
+      const uint4 w = *reinterpret_cast<const uint4*>(q + c + u * PER);
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[u * PER + k] = to_f32(e[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + 32 * k < N ? to_f32(q[(c + 32 * k) * cs]) : 0.f;
+  }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(void* p, int64_t off, int64_t c, int64_t N, const float (&v)[8]) {
+  T* q = static_cast<T*>(p) + off;
+  if constexpr (VEC) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 8 / PER; ++u) {
+      uint4 w;
+      T* e = reinterpret_cast<T*>(&w);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) e[k] = from_f32<T>(v[u * PER + k]);
+      *reinterpret_cast<uint4*>(q + c + u * PER) = w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + 32 * k < N) q[c + 32 * k] = from_f32<T>(v[k]);
+  }
+}
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kDactWarps * 32) gemm_dact_kernel(const DactParams p, int64_t band) {
-  __shared__ float part[kDactWarps][32];
+  __shared__ float part[kDactWarps][kCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t rows = p.batch * p.M, c = (int64_t)blockIdx.x * 32 + lane, r0 = (int64_t)blockIdx.y * band;
-  const int64_t r1 = r0 + band < rows ? r0 + band : rows;
-  float sum = 0.f;
+  const int64_t rows = p.batch * p.M, c0 = (int64_t)blockIdx.x * kCols, r0 = (int64_t)blockIdx.y * band;
+  const int64_t c = c0 + (VEC ? lane * 8 : lane), r1 = r0 + band < rows ? r0 + band : rows;
+  float sum[8] = {};
   if (c < p.N) {
+    int64_t b = (r0 + warp) / p.M, i = (r0 + warp) - b * p.M;
     for (int64_t r = r0 + warp; r < r1; r += kDactWarps) {
-      const int64_t b = r / p.M, i = r - b * p.M;
-      const float dy = to_f32(static_cast<const T*>(p.dY)[b * p.dy_bs + i * p.dy_rs + c * p.dy_cs]);
-      float d = dy;
+      float dy[8], d[8];
+      load8<T, VEC>(p.dY, b * p.dy_bs + i * p.dy_rs, p.dy_cs, c, p.N, dy);
       if (p.pre) {
-        const float x = to_f32(static_cast<const T*>(p.pre)[b * p.pre_bs + i * p.pre_rs + c * p.pre_cs]);
-        d = p.act == B2C_ACT_RELU ? (x > 0.f ? dy : 0.f) : dy * act_slope_f32(x, p.act);
+        float x[8];
+        load8<T, VEC>(p.pre, b * p.pre_bs + i * p.pre_rs, p.pre_cs, c, p.N, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          d[k] = p.act == B2C_ACT_RELU ? (x[k] > 0.f ? dy[k] : 0.f) : dy[k] * act_slope_f32<sizeof(T) == 2>(x[k], p.act);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k] = dy[k];
       }
-      if (p.dP) static_cast<T*>(p.dP)[r * p.N + c] = from_f32<T>(d);
-      if (p.dR) static_cast<T*>(p.dR)[r * p.N + c] = from_f32<T>(p.beta * dy);
-      sum += d;
+      if (p.dP) store8<T, VEC>(p.dP, r * p.N, c, p.N, d);
+      if (p.dR) {
+        float q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = p.beta * dy[k];
+        store8<T, VEC>(p.dR, r * p.N, c, p.N, q);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum[k] += d[k];
+      for (i += kDactWarps; i >= p.M; i -= p.M) ++b;
     }
   }
   if (!p.dbias) return;
-  part[warp][lane] = sum;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) part[warp][VEC ? lane * 8 + k : lane + 32 * k] = sum[k];
   __syncthreads();
-  if (warp == 0 && c < p.N) {
+  if (c0 + threadIdx.x < p.N) {
     float t = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDactWarps; ++w) t += part[w][lane];
-    p.ws[(int64_t)blockIdx.y * p.N + c] = t;
+    for (int w = 0; w < kDactWarps; ++w) t += part[w][threadIdx.x];
+    p.ws[(int64_t)blockIdx.y * p.N + c0 + threadIdx.x] = t;
   }
 }
 
@@ -66,12 +122,22 @@ __global__ void __launch_bounds__(256) gemm_dbias_kernel(const float* ws, void* 
 }
 
 template <typename T>
+bool rows_on_16(const void* p, int64_t bs, int64_t rs, int64_t cs) {
+  constexpr int64_t PER = 16 / sizeof(T);
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && cs == 1 && bs % PER == 0 && rs % PER == 0;
+}
+
+template <typename T>
 cudaError_t launch_t(const DactParams& p, cudaStream_t s) {
   const int64_t rows = p.batch * p.M, band = dact_band_rows(rows);
   const int bands = (int)((rows + band - 1) / band);
   if (bands > 0) {
-    const dim3 grid((unsigned)((p.N + 31) / 32), (unsigned)bands);
-    gemm_dact_kernel<T><<<grid, kDactWarps * 32, 0, s>>>(p, band);
+    const dim3 grid((unsigned)((p.N + kCols - 1) / kCols), (unsigned)bands);
+    const bool vec = p.N % 8 == 0 && rows_on_16<T>(p.dY, p.dy_bs, p.dy_rs, p.dy_cs) &&
+                     rows_on_16<T>(p.pre, p.pre_bs, p.pre_rs, p.pre ? p.pre_cs : 1) && rows_on_16<T>(p.dP, 0, 0, 1) &&
+                     rows_on_16<T>(p.dR, 0, 0, 1);
+    if (vec) gemm_dact_kernel<T, true><<<grid, kDactWarps * 32, 0, s>>>(p, band);
+    else gemm_dact_kernel<T, false><<<grid, kDactWarps * 32, 0, s>>>(p, band);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }

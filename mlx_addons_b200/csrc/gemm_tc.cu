@@ -22,14 +22,13 @@
 // cores truncate when they add to an accumulator, so such a product's
 // accumulator is joined in float32 registers every kChunk values of k
 // (JOIN): without that the truncations, all towards zero, add up along k.
-#include <cuda.h>
-
 #include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
 #include "b2c_kernels.cuh"
 #include "gemm_tc.cuh"
+#include "tcgen05.cuh"
 
 namespace b2c {
 
@@ -46,7 +45,6 @@ constexpr int kRegsFew = 72, kRegsMany = 216;
 constexpr int kMaxStages = 8;
 constexpr int kChunk = 4;        // slices of k per joined accumulator
 constexpr int kMaxSeg = 6;
-constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kSmemMax = 232448;
 
 struct TcParams {
@@ -62,133 +60,6 @@ struct TcParams {
   int64_t y_plane, res_plane;
   int inject;
 };
-
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 10000;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-// Waits for the phase of the given parity. False once the CTA has given up,
-// or after `limit` ns, which gives the CTA up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, uint64_t limit) {
-  if (bar_try(bar, parity)) return true;
-  const uint64_t t0 = now_ns();
-  for (;;) {
-    if (bar_try(bar, parity)) return true;
-    if (*gave_up) return false;
-    if (now_ns() - t0 > limit) {
-      *gave_up = 1;
-      atomicOr(&g_gemm_fault, 1u);
-      return false;
-    }
-  }
-}
-
-template <int CG>
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
-  if constexpr (CG == 2) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-  } else {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-  }
-}
-
-// Shared-memory descriptor of a 128-byte swizzled tile: version 1, swizzle 2.
-// K-major rows lie 128 bytes apart (groups of 8 rows: SBO 1024). MN-major
-// blocks of 64 rows x 64 k lie 8192 bytes apart (LBO), 8 k of them 1024 (SBO).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, int inner) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(inner ? (8192u >> 4) : 1u) << 16) |
-         ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-template <int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  if constexpr (CG == 2) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-  }
-}
-// Arrives on `bar` (in both CTAs of a pair) once every MMA issued so far is done.
-template <int CG>
-__device__ __forceinline__ void commit(uint32_t bar) {
-  if constexpr (CG == 2) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
-        : "memory");
-  } else {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-  }
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 32 columns of this lane's row of the accumulator.
-__device__ __forceinline__ void tmem_row32(uint32_t addr, float (&d)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr)
-      : "memory");
-#pragma unroll
-  for (int c = 0; c < 32; ++c) d[c] = __uint_as_float(r[c]);
-}
 
 // ---------------------------------------------------------------------------
 // epilogue of one lane's 32 columns
@@ -284,23 +155,24 @@ __device__ __forceinline__ void add_res(float (&v)[32], const T* base, int64_t j
   }
 }
 
+template <bool FAST>
 __device__ __forceinline__ void apply_act(float (&v)[32], int act) {
   switch (act) {
     case B2C_ACT_RELU:
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = act_f32(v[c], B2C_ACT_RELU);
+      for (int c = 0; c < 32; ++c) v[c] = act_f32<FAST>(v[c], B2C_ACT_RELU);
       break;
     case B2C_ACT_GELU:
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = act_f32(v[c], B2C_ACT_GELU);
+      for (int c = 0; c < 32; ++c) v[c] = act_f32<FAST>(v[c], B2C_ACT_GELU);
       break;
     case B2C_ACT_GELU_TANH:
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = act_f32(v[c], B2C_ACT_GELU_TANH);
+      for (int c = 0; c < 32; ++c) v[c] = act_f32<FAST>(v[c], B2C_ACT_GELU_TANH);
       break;
     case B2C_ACT_SILU:
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = act_f32(v[c], B2C_ACT_SILU);
+      for (int c = 0; c < 32; ++c) v[c] = act_f32<FAST>(v[c], B2C_ACT_SILU);
       break;
     default: break;
   }
@@ -330,7 +202,7 @@ __device__ __forceinline__ void epilogue32(float (&v)[32], const TcParams& p, in
       }
     }
     if (e.pre.p) store_tile<T>(v, e.pre, b, i, j, rows, cols, p.pre_vec, stage, lane);
-    apply_act(v, e.act);
+    apply_act<sizeof(T) == 2>(v, e.act);
   }
   if (e.res.p && lane < rows) {
     const int64_t off = b * e.res.bs + (i + lane) * e.res.is + j * e.res.js;
@@ -456,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t buf = 0, tphase = 0;
     bool ok = true;
     const float bad = __int_as_float(0x7fffffff);
-    if (p.inject && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, limit));
+    if (p.inject && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, limit, &g_gemm_fault));
     for (int64_t t = first; t < p.tiles; t += step) {
       const Tile o = tile_at<CG>(p, t);
       const int64_t i = o.i + rank * BM + quad * 32;
@@ -468,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[q][c] = 0.f;
         for (int c0 = 0; c0 < p.kblocks; c0 += p.chunk) {
-          ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit));
+          ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
           fence_after();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -497,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit));
+        ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
         fence_after();
         for (int col = half * 32; col < p.BN; col += 64) {
           float v[32];
@@ -531,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int c1 = min(c0 + p.chunk, p.kblocks);
           for (int g = 0; g < p.nseg; ++g) {
             for (int kb = c0; kb < c1; ++kb) {
-              if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit)) break;
+              if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_gemm_fault)) break;
               if (rank == 0) bar_expect(full0 + 8 * s, CG * stage_bytes);
               const uint32_t bar = lead_full0 + 8 * s, a = smem_u32(ring + s * stage_bytes), q = a + p.a_bytes;
               if (p.p_inner) {
@@ -558,11 +430,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int64_t t = first; t < p.tiles && !*gu; t += step) {
         for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
           const int n = (min(c0 + p.chunk, p.kblocks) - c0) * p.nseg;
-          if (!bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit)) break;
+          if (!bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
           fence_after();
           const uint32_t d = tmem + buf * 256;
           for (int it = 0; it < n; ++it) {
-            if (!bar_wait(full0 + 8 * s, phase, gu, limit)) break;
+            if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
             fence_after();
             const uint32_t a = smem_u32(ring + s * stage_bytes);
             const uint64_t da = tile_desc(a, p.p_inner), dq = tile_desc(a + p.a_bytes, p.q_inner);
@@ -752,9 +624,7 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   p.sym = t.sym;
   p.a_bytes = BM * BK * 2;
   p.b_bytes = (p.q_inner ? (p.share + 63) / 64 * 64 : p.share) * BK * 2;
-  const uint32_t type = t.f16 ? 0u : 1u;
-  p.idesc = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)p.p_inner << 15) | ((uint32_t)p.q_inner << 16) |
-            ((uint32_t)(p.BN >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
+  p.idesc = mma_idesc(t.f16, p.p_inner, p.q_inner, BM * CG, p.BN);
   p.e = t.e;
   p.res_kind = t.res;
   p.y_plane = t.y_plane;

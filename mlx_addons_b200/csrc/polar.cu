@@ -16,60 +16,120 @@ namespace {
 
 constexpr float kScaleX = 16384.f;
 constexpr int kNormThreads = 256;
-constexpr int kNormParts = 64;  // partial sums of a matrix, added in a fixed order
+constexpr int kNormParts = kNormThreads;  // most partial sums of a matrix
 
 struct PolarIn {
   const void* G;
   int64_t bs, rs, cs, batch, m, n;
+  int vec;  // rows of unit stride on 16-byte boundaries
 };
 
-// Sum of squares of one slice of one matrix, held in 64 bits: squares of any
-// float32 neither overflow nor vanish there.
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) polar_norm_kernel(const PolarIn in, double* part) {
-  __shared__ double red[kNormThreads / 32];
-  const int64_t total = in.m * in.n;
-  for (int64_t b = blockIdx.y; b < in.batch; b += gridDim.y) {
-  const T* base = static_cast<const T*>(in.G) + b * in.bs;
-  double s = 0.0;
-  for (int64_t e = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kNormThreads) {
-    const int64_t r = e / in.n, c = e - r * in.n;
-    const double v = (double)to_f32(base[r * in.rs + c * in.cs]);
-    s += v * v;
-  }
+// Sum of a block's values in a fixed order; every thread gets it.
+__device__ __forceinline__ double block_sum(double s, double* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
+  s = 0.0;
 #pragma unroll
-    for (int w = 0; w < kNormThreads / 32; ++w) t += red[w];
-    part[b * kNormParts + blockIdx.x] = t;
+  for (int w = 0; w < kNormThreads / 32; ++w) s += red[w];
+  return s;
+}
+
+// Walks a matrix in units of 8 neighbouring elements of a row: this thread's
+// next one is `blocks` blocks of threads further. One division at the start.
+struct Walk {
+  int64_t r, u, units, dr, du;
+  __device__ __forceinline__ Walk(int64_t n, int64_t blocks, int64_t block) {
+    units = (n + 7) / 8;
+    const int64_t first = block * kNormThreads + threadIdx.x, step = blocks * kNormThreads;
+    r = first / units, u = first - r * units;
+    dr = step / units, du = step - dr * units;
   }
-  __syncthreads();
+  __device__ __forceinline__ void next() {
+    r += dr, u += du;
+    if (u >= units) u -= units, ++r;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_unit(const PolarIn& in, const T* row, int64_t c, float (&v)[8]) {
+  if (in.vec && c + 8 <= in.n) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < 8 / PER; ++q) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + c + q * PER);
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[q * PER + k] = to_f32(e[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < in.n ? to_f32(row[(c + k) * in.cs]) : 0.f;
   }
 }
 
-// X = G / (|G|_F + eps) times 2^14, as one or two f16 planes.
-template <typename T, bool HALVES>
-__global__ void __launch_bounds__(kNormThreads) polar_scale_kernel(const PolarIn in, const double* part, int parts,
-                                                                   double eps, __half* X, int64_t pitch, int64_t plane) {
-  const int64_t total = in.m * in.n;
+// Sum of squares of one slice of one matrix, held in 64 bits: squares of any
+// float32 neither overflow nor vanish there. Bound by HBM (2 or 4 bytes an
+// element; the 64-bit additions take about as long).
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads) polar_norm_kernel(const PolarIn in, double* part) {
+  __shared__ double red[kNormThreads / 32];
   for (int64_t b = blockIdx.y; b < in.batch; b += gridDim.y) {
     const T* base = static_cast<const T*>(in.G) + b * in.bs;
     double s = 0.0;
-    for (int i = 0; i < parts; ++i) s += part[b * kNormParts + i];
-    const double inv = kScaleX / (sqrt(s) + eps);
-    for (int64_t e = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; e < total;
-         e += (int64_t)gridDim.x * kNormThreads) {
-      const int64_t r = e / in.n, c = e - r * in.n, at = (b * in.m + r) * pitch + c;
-      const float x = (float)((double)to_f32(base[r * in.rs + c * in.cs]) * inv);
-      const __half hi = __float2half_rn(x);
-      X[at] = hi;
-      if constexpr (HALVES) X[plane + at] = __float2half_rn(x - __half2float(hi));
+    for (Walk w(in.n, gridDim.x, blockIdx.x); w.r < in.m; w.next()) {
+      float v[8];
+      load_unit<T>(in, base + w.r * in.rs, w.u * 8, v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
+    }
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) part[b * kNormParts + blockIdx.x] = s;
+  }
+}
+
+// X = G / (|G|_F + eps) times 2^14, as one or two f16 planes, rows padded to
+// units of 8.
+template <typename T, bool HALVES>
+__global__ void __launch_bounds__(kNormThreads) polar_scale_kernel(const PolarIn in, const double* part, int parts,
+                                                                   double eps, __half* X, int64_t pitch, int64_t plane) {
+  __shared__ double red[kNormThreads / 32];
+  for (int64_t b = blockIdx.y; b < in.batch; b += gridDim.y) {
+    const T* base = static_cast<const T*>(in.G) + b * in.bs;
+    const double sum = block_sum((int)threadIdx.x < parts ? part[b * kNormParts + threadIdx.x] : 0.0, red);
+    const double inv = kScaleX / (sqrt(sum) + eps);
+    for (Walk w(in.n, gridDim.x, blockIdx.x); w.r < in.m; w.next()) {
+      float v[8];
+      load_unit<T>(in, base + w.r * in.rs, w.u * 8, v);
+      __align__(16) __half hi[8], lo[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float x = (float)((double)v[k] * inv);
+        hi[k] = __float2half_rn(x);
+        lo[k] = __float2half_rn(x - __half2float(hi[k]));
+      }
+      const int64_t at = (b * in.m + w.r) * pitch + w.u * 8;
+      *reinterpret_cast<uint4*>(X + at) = *reinterpret_cast<const uint4*>(hi);
+      if constexpr (HALVES) *reinterpret_cast<uint4*>(X + plane + at) = *reinterpret_cast<const uint4*>(lo);
     }
   }
+}
+
+// The iteration on G^T gives the transposed result: a matrix whose columns lie
+// closer together than its rows is taken as its transpose, so that reads run
+// along memory.
+PolarParams along_rows(const PolarParams& in) {
+  PolarParams p = in;
+  p.out_rs = p.n;
+  p.out_cs = 1;
+  if (p.m > 1 && p.n > 1 ? p.rs < p.cs : p.n == 1) {
+    p.m = in.n, p.n = in.m;
+    p.rs = in.cs, p.cs = in.rs;
+    p.out_rs = 1, p.out_cs = in.n;
+  }
+  return p;
 }
 
 // Scratch of the product form: norms, two X, S and P.
@@ -109,15 +169,17 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   __half* X1 = reinterpret_cast<__half*>(w + l.x_bytes);
   __half* S = reinterpret_cast<__half*>(w + 2 * l.x_bytes);
   __half* P = reinterpret_cast<__half*>(w + 2 * l.x_bytes + l.s_bytes);
-  const PolarIn in{p.G, p.bs, p.rs, p.cs, p.batch, p.m, p.n};
-  int64_t blocks = (mn + kNormThreads - 1) / kNormThreads;
-  const int parts = (int)(blocks < kNormParts ? blocks : kNormParts);
-  if (blocks > 4096) blocks = 4096;
-  const unsigned by = (unsigned)(p.batch < 65535 ? p.batch : 65535);
-  const dim3 gn((unsigned)parts, by), gs((unsigned)blocks, by);
-  polar_norm_kernel<T><<<gn, kNormThreads, 0, s>>>(in, part);
+  constexpr int64_t PER = 16 / sizeof(T);
+  const PolarIn in{p.G, p.bs, p.rs, p.cs, p.batch, p.m, p.n,
+                   (reinterpret_cast<uintptr_t>(p.G) & 15) == 0 && p.cs == 1 && p.rs % PER == 0 && p.bs % PER == 0};
+  const int64_t units = p.m * ((p.n + 7) / 8);
+  int64_t blocks = (units + 4 * kNormThreads - 1) / (4 * kNormThreads);
+  if (blocks > kNormParts) blocks = kNormParts;
+  const int parts = (int)blocks;
+  const dim3 grid((unsigned)blocks, (unsigned)(p.batch < 65535 ? p.batch : 65535));
+  polar_norm_kernel<T><<<grid, kNormThreads, 0, s>>>(in, part);
   constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
-  polar_scale_kernel<T, kTwo><<<gs, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0, l.pitch_x, l.x_plane);
+  polar_scale_kernel<T, kTwo><<<grid, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0, l.pitch_x, l.x_plane);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
 
@@ -162,7 +224,7 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
     t.P = wide ? p_op : x_rows;
     t.Q = wide ? x_cols : p_op;
     t.sym = 0;
-    t.e.y = last ? GemmView{p.out, mn, p.n, 1} : GemmView{X1, xx, l.pitch_x, 1};
+    t.e.y = last ? GemmView{p.out, mn, p.out_rs, p.out_cs} : GemmView{X1, xx, l.pitch_x, 1};
     t.e.res = GemmView{X0, xx, l.pitch_x, 1};
     t.e.alpha = so / (sp * kScaleX);
     t.e.beta = (float)(a * so / kScaleX);
@@ -201,12 +263,14 @@ double polar_poly_bound(double a, double b, double c, double hi) {
   return best;
 }
 
-size_t polar_ws_bytes(const PolarParams& p) {
+size_t polar_ws_bytes(const PolarParams& in) {
+  const PolarParams p = along_rows(in);
   const PolarLayout l = polar_layout(p);
   return (size_t)(l.part_bytes + 2 * l.x_bytes + 2 * l.s_bytes);
 }
 
-cudaError_t launch_polar(const PolarParams& p, cudaStream_t s) {
+cudaError_t launch_polar(const PolarParams& in, cudaStream_t s) {
+  const PolarParams p = along_rows(in);
   switch (p.dtype) {
     case B2C_F32: return launch_t<float>(p, s);
     case B2C_BF16: return launch_t<__nv_bfloat16>(p, s);

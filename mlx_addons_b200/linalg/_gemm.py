@@ -12,21 +12,25 @@ without a copy. The reference has no counterpart; its products are MLX's own.
 
 from __future__ import annotations
 
-import ctypes
+import contextlib
+import sys
 from typing import Optional
 
 import torch
 
 from .. import _lib
 
+_pkg = sys.modules[__package__]  # the helpers of linalg/__init__.py, which imports this module at its end
+_NO_GUARD = contextlib.nullcontext()
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 def _native(x, what, name):
     """Any accepted array as a torch tensor of one of the three types."""
-    from . import _as_tensor
-
-    t, kind = _as_tensor(x, name)
+    if isinstance(x, torch.Tensor):
+        t, kind = x, "torch"
+    else:
+        t, kind = _pkg._as_tensor(x, name)
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: {what} requires a gradient, which {name} does not record; detach it or call under "
                          "torch.no_grad() (gemm_grad computes the gradients of gemm)")
@@ -45,55 +49,57 @@ def _same_type(name, first, **others):
 
 def _on_device(tensors):
     """Host tensors go to the current CUDA device, others to the first one's."""
-    from . import _require_cuda
-
-    if tensors[0].is_cuda:
-        dev = tensors[0].device
-    else:
-        _require_cuda()
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        _pkg._require_cuda()
         dev = torch.device("cuda", torch.cuda.current_device())
     return dev, [t if t is None or t.device == dev else t.to(dev) for t in tensors]
 
 
+def _guard(dev):
+    """The device as the current one, at no cost where it is."""
+    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
 def _matrix(t):
-    """b2c_matrix of a tensor (batch, rows, cols) or (rows, cols); a negative
-    stride cannot occur in torch."""
-    if t.dim() == 2:
-        return _lib.Matrix(t.data_ptr(), 0, t.stride(0), t.stride(1))
-    return _lib.Matrix(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
-
-
-def _ref(m):
-    return None if m is None else ctypes.byref(m)
+    """b2c_matrix of a tensor (batch, rows, cols) or (rows, cols); torch has no
+    negative strides."""
+    s = t.stride()
+    return _lib.Matrix(t.data_ptr(), 0 if len(s) == 2 else s[-3], s[-2], s[-1])
 
 
 def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _call(what, fn, args, ws_fn, ws_args, dev):
+    """fn(*args, workspace, bytes, stream); a call that needs scratch says so
+    before it launches anything."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    rc = fn(*args, None, 0, stream)
+    if rc == _lib.B2C_ERR_WORKSPACE:
+        n = ws_fn(*ws_args)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        rc = fn(*args, ws.data_ptr(), n, stream)
+    if rc:
+        _lib.check(rc, what)
 
 
 def _gemm_dev(A, B, bias, act, R, alpha, beta, want_pre):
-    """A (batch, M, K), B (batch, K, N) or (K, N), on one device."""
-    from . import _stream
-
+    """A (batch, M, K) or (M, K), B (batch, K, N) or (K, N), on one device."""
     lib = _lib.load()
     dev = A.device
-    batch, M, K = A.shape
+    M, K = A.shape[-2:]
     N = B.shape[-1]
-    Y = torch.empty((batch, M, N), dtype=A.dtype, device=dev)
+    batch = A.shape[0] if A.dim() == 3 else 1
+    Y = torch.empty((batch, M, N) if A.dim() == 3 else (M, N), dtype=A.dtype, device=dev)
     pre = torch.empty_like(Y) if want_pre else None
-    code = _DTYPES[A.dtype]
-    a, b = _matrix(A), _matrix(B)
+    code, a, b = _DTYPES[A.dtype], _matrix(A), _matrix(B)
     r = None if R is None else _matrix(R)
-    with torch.cuda.device(dev):
-        ws_bytes = int(lib.b2c_gemm_workspace_size(code, _ref(a), _ref(b), batch, M, K, N))
-        ws = _workspace(ws_bytes, dev)
-        rc = lib.b2c_gemm(code, _ref(a), _ref(b), _addr(bias), _ref(r), Y.data_ptr(), _addr(pre), batch, M, K, N,
-                          alpha, beta, act, _addr(ws), ws_bytes, _stream(dev))
-    _lib.check(rc, "b2c_gemm")
+    with _guard(dev):
+        _call("b2c_gemm", lib.b2c_gemm,
+              (code, a, b, _addr(bias), r, Y.data_ptr(), _addr(pre), batch, M, K, N, alpha, beta, act),
+              lib.b2c_gemm_workspace_size, (code, a, b, batch, M, K, N), dev)
     return Y, pre
 
 
@@ -114,15 +120,19 @@ def _check_product(A, B, name):
 
 def _flat(t, lead, shared):
     """(..., M, K) as one matrix of all rows (a shared B) or a batch of them."""
+    if not lead or (len(lead) == 1 and not shared):
+        return t
     rows, cols = t.shape[-2:]
     n = 1
     for d in lead:
         n *= d
-    return t.reshape((1, n * rows, cols) if shared else (n, rows, cols))
+    return t.reshape((n * rows, cols) if shared else (n, rows, cols))
 
 
 def _back(out, kind, host):
-    out = tuple(None if o is None else o.cpu() if host else o for o in out)
+    if not host:
+        return out
+    out = tuple(None if o is None else o.cpu() for o in out)
     if kind == "numpy":
         out = tuple(None if o is None else o.numpy() for o in out)
     return out
@@ -177,8 +187,6 @@ def gemm_grad(dY, A, B, pre=None, activation: Optional[str] = None, *, alpha: fl
     dimensions) gets the sum over A's leading dimensions. dP is rounded to the
     operands' type once, as an operand of the two products; dbias takes it
     before that. Every sum runs in a fixed order."""
-    from . import _stream
-
     name = "gemm_grad"
     act = _activation(activation, name)
     dYt, _ = _native(dY, "dY", name)
@@ -199,23 +207,22 @@ def gemm_grad(dY, A, B, pre=None, activation: Optional[str] = None, *, alpha: fl
     dev, (At, Bt, dYt, pt) = _on_device([At, Bt, dYt, pt])
     A3, dY3 = _flat(At, lead, shared), _flat(dYt, lead, shared)
     B3 = Bt if shared else _flat(Bt, lead, False)
-    batch, rows = A3.shape[0], A3.shape[1]
+    batch, rows = A3.shape[0] if A3.dim() == 3 else 1, A3.shape[-2]
+    full = tuple(A3.shape[:-1]) + (N,)
     dP, dbias, dR = dY3, None, None
     if act:
-        dP = torch.empty((batch, rows, N), dtype=At.dtype, device=dev)
+        dP = torch.empty(full, dtype=At.dtype, device=dev)
     if need_bias:
         dbias = torch.empty((N,), dtype=At.dtype, device=dev)
     if need_residual:
-        dR = torch.empty((batch, rows, N), dtype=At.dtype, device=dev)
+        dR = torch.empty(full, dtype=At.dtype, device=dev)
     if act or need_bias or need_residual:
         lib = _lib.load()
         dy, p = _matrix(dY3), None if pt is None else _matrix(_flat(pt, lead, shared))
-        with torch.cuda.device(dev):
-            ws_bytes = int(lib.b2c_gemm_dact_workspace_size(batch, rows, N)) if need_bias else 0
-            ws = _workspace(ws_bytes, dev)
-            rc = lib.b2c_gemm_dact(_DTYPES[At.dtype], _ref(dy), _ref(p), act, float(beta), _addr(dP) if act else None,
-                                   _addr(dbias), _addr(dR), batch, rows, N, _addr(ws), ws_bytes, _stream(dev))
-        _lib.check(rc, "b2c_gemm_dact")
+        with _guard(dev):
+            _call("b2c_gemm_dact", lib.b2c_gemm_dact,
+                  (_DTYPES[At.dtype], dy, p, act, float(beta), _addr(dP) if act else None, _addr(dbias), _addr(dR), batch,
+                   rows, N), lib.b2c_gemm_dact_workspace_size, (batch, rows, N), dev)
     dA, _ = _gemm_dev(dP, B3.mT, None, 0, None, float(alpha), 1.0, False)
     dB, _ = _gemm_dev(A3.mT, dP, None, 0, None, float(alpha), 1.0, False)
     out = (dA.reshape(lead + (M, K)), dB.reshape((K, N) if shared else lead + (K, N)), dbias,

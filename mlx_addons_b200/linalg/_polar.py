@@ -8,6 +8,7 @@ import ctypes
 import torch
 
 from .. import _lib
+from ._gemm import _DTYPES, _back, _call, _guard, _matrix, _native, _on_device
 
 _COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -41,9 +42,6 @@ def orthogonalize(G, steps: int = 5, coefficients=_COEFFICIENTS, eps: float = 1e
     sums and norms are held in 32 bits or more and the result is rounded once to
     G's type. A matrix of zeros gives zeros; one with a NaN or an infinity
     gives NaN. Records no gradient."""
-    from . import _stream
-    from ._gemm import _DTYPES, _addr, _back, _matrix, _native, _on_device, _ref, _workspace
-
     name = "orthogonalize"
     Gt, kind = _native(G, "G", name)
     if Gt.dim() < 2:
@@ -58,14 +56,12 @@ def orthogonalize(G, steps: int = 5, coefficients=_COEFFICIENTS, eps: float = 1e
     batch = 1
     for d in Gt.shape[:-2]:
         batch *= d
-    G3 = Gt.reshape((batch, m, n))
-    out = torch.empty((batch, m, n), dtype=Gt.dtype, device=dev)
+    G3 = Gt if Gt.dim() <= 3 else Gt.reshape((batch, m, n))
+    out = torch.empty(Gt.shape, dtype=Gt.dtype, device=dev)
     lib = _lib.load()
     g, code = _matrix(G3), _DTYPES[Gt.dtype]
-    with torch.cuda.device(dev):
-        ws_bytes = int(lib.b2c_orthogonalize_workspace_size(code, _ref(g), batch, m, n))
-        ws = _workspace(ws_bytes, dev)
-        rc = lib.b2c_orthogonalize(code, _ref(g), out.data_ptr(), batch, m, n, (ctypes.c_double * len(coef))(*coef),
-                                   steps, float(eps), _addr(ws), ws_bytes, _stream(dev))
-    _lib.check(rc, "b2c_orthogonalize")
-    return _back((out.reshape(Gt.shape),), kind, host)[0]
+    with _guard(dev):
+        _call("b2c_orthogonalize", lib.b2c_orthogonalize,
+              (code, g, out.data_ptr(), batch, m, n, (ctypes.c_double * len(coef))(*coef), steps, float(eps)),
+              lib.b2c_orthogonalize_workspace_size, (code, g, batch, m, n), dev)
+    return _back((out,), kind, host)[0]
