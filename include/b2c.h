@@ -195,7 +195,7 @@ size_t b2c_gemm_dact_workspace_size(int64_t batch, int64_t M, int64_t N);
  * on the smaller side of G, (a, b, c) = coefficients[3 t .. 3 t + 2] in step
  * t (a host array). With suitable coefficients the singular values of the
  * result lie near 1. Every matrix of the batch has a norm of its own; one of
- * zeros gives zeros, one with a non-finite entry gives NaN.
+ * zeros gives zeros (NaN where eps is 0), one with a non-finite entry NaN.
  *   G   (batch, m, n) any strides; out (batch, m, n) contiguous, may be G's
  *       memory where G is contiguous
  * The polynomials have to keep |p(s)| <= 3.5 over the singular values that

@@ -48,6 +48,8 @@ cudaError_t dag_take_fault(unsigned int* fault);
 cudaError_t blocked_take_fault(unsigned int* fault);
 // Reads and clears the tensor-core products' fault flag. gemm_tc.cu
 cudaError_t gemm_take_fault(unsigned int* fault);
+// Reads and clears the small orthogonalisation's fault flag. polar_cta.cu
+cudaError_t polar_take_fault(unsigned int* fault);
 cudaError_t launch_posv_blocked2(const PosvParams& p, int grid, cudaStream_t s);
 
 // Triangular solves, any k. posv_blocked.cu

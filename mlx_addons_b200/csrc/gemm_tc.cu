@@ -43,7 +43,7 @@ constexpr int kThreads = (kEpiWarps + 4) * 32;  // the last warpgroup: loads, pr
 // Registers: 384 x 168 at launch = 128 x 72 + 256 x 216 after the split.
 constexpr int kRegsFew = 72, kRegsMany = 216;
 constexpr int kMaxStages = 8;
-constexpr int kChunk = 4;        // slices of k per joined accumulator
+constexpr int kChunk = 2;        // slices of k per joined accumulator
 constexpr int kMaxSeg = 6;
 constexpr int kSmemMax = 232448;
 
@@ -56,6 +56,7 @@ struct TcParams {
   int p_inner, q_inner, p_bcast, q_bcast, sym;
   uint32_t idesc;
   GemmEpilogue e;
+  TcPolar polar;
   int res_kind, y_vec, pre_vec, res_vec;
   int64_t y_plane, res_plane;
   int inject;
@@ -137,21 +138,22 @@ __device__ __forceinline__ void store_tile(const float (&v)[32], const GemmView&
   else store_cols<T>(v, base, o.js, rows, cols, lane);
 }
 
+// r[c] += 32 columns of an addend's row.
 template <typename T>
-__device__ __forceinline__ void add_res(float (&v)[32], const T* base, int64_t js, float beta, int cols, int vec) {
-  if (vec && js == 1 && cols >= 32) {
+__device__ __forceinline__ void load_res(float (&r)[32], const T* base, int64_t js, int cols, int vec) {
+  if (vec && cols >= 32) {
     constexpr int PER = 16 / sizeof(T);
 #pragma unroll
     for (int u = 0; u < 32 / PER; ++u) {
       const uint4 w = *reinterpret_cast<const uint4*>(base + u * PER);
       const T* q = reinterpret_cast<const T*>(&w);
 #pragma unroll
-      for (int c = 0; c < PER; ++c) v[u * PER + c] = fmaf(beta, to_f32(q[c]), v[u * PER + c]);
+      for (int c = 0; c < PER; ++c) r[u * PER + c] += to_f32(q[c]);
     }
   } else {
 #pragma unroll
     for (int c = 0; c < 32; ++c)
-      if (c < cols) v[c] = fmaf(beta, to_f32(base[(int64_t)c * js]), v[c]);
+      if (c < cols) r[c] += to_f32(base[(int64_t)c * js]);
   }
 }
 
@@ -175,6 +177,49 @@ __device__ __forceinline__ void apply_act(float (&v)[32], int act) {
       for (int c = 0; c < 32; ++c) v[c] = act_f32<FAST>(v[c], B2C_ACT_SILU);
       break;
     default: break;
+  }
+}
+
+// v = alpha D, r = the addend; see TcPolarMode.
+__device__ __forceinline__ void polar_epilogue(float (&v)[32], const float (&r)[32], const TcPolar& q, const GemmEpilogue& e,
+                                               int64_t b, int64_t i, int64_t j, int rows, int cols, int lane) {
+  const float f = q.r ? q.r[b] : 1.f;
+  const float* d = q.d_in + b * q.side;
+  const int64_t diag = i + lane - j;  // the column of this row's diagonal element
+  if (q.mode == kPolarS) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] *= f * f;
+    if (diag >= 0 && diag < 32 && lane < rows) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (c == diag) {
+          q.d_out[b * q.side + i + lane] = v[c] * q.k;
+          v[c] = 0.f;
+        }
+    }
+    return;
+  }
+  const float di = q.mode != kPolarXj && lane < rows ? d[i + lane] : 0.f;
+  const float dj = q.mode != kPolarXi && lane < cols ? d[j + lane] : 0.f;
+  if (q.mode == kPolarP) {
+    const float w = fmaf(q.k, di, e.beta);
+    const bool here = diag >= 0 && diag < 32 && lane < rows;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      const float x = fmaf(q.k, __shfl_sync(kFull, dj, c), w);
+      if (here && c == diag) {
+        q.d_out[b * q.side + i + lane] = fmaf(q.k2, v[c], di * fmaf(q.k3, di, q.k4));
+        v[c] = 0.f;
+      } else {
+        v[c] = fmaf(x, r[c], v[c]);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const float x = q.k + (q.mode == kPolarXi ? di : __shfl_sync(kFull, dj, c));
+    v[c] = f * fmaf(e.beta * x, r[c], v[c]);
   }
 }
 
@@ -204,16 +249,25 @@ __device__ __forceinline__ void epilogue32(float (&v)[32], const TcParams& p, in
     if (e.pre.p) store_tile<T>(v, e.pre, b, i, j, rows, cols, p.pre_vec, stage, lane);
     apply_act<sizeof(T) == 2>(v, e.act);
   }
+  float r[32] = {};
   if (e.res.p && lane < rows) {
     const int64_t off = b * e.res.bs + (i + lane) * e.res.is + j * e.res.js;
     switch (p.res_kind) {
-      case B2C_F32: add_res(v, static_cast<const float*>(e.res.p) + off, e.res.js, e.beta, cols, p.res_vec); break;
-      case B2C_BF16: add_res(v, static_cast<const __nv_bfloat16*>(e.res.p) + off, e.res.js, e.beta, cols, p.res_vec); break;
+      case B2C_F32: load_res(r, static_cast<const float*>(e.res.p) + off, e.res.js, cols, p.res_vec); break;
+      case B2C_BF16: load_res(r, static_cast<const __nv_bfloat16*>(e.res.p) + off, e.res.js, cols, p.res_vec); break;
       default:
-        add_res(v, static_cast<const __half*>(e.res.p) + off, e.res.js, e.beta, cols, p.res_vec);
         if (p.res_kind == kOutHalves)
-          add_res(v, static_cast<const __half*>(e.res.p) + p.res_plane + off, e.res.js, e.beta, cols, p.res_vec);
+          load_res(r, static_cast<const __half*>(e.res.p) + p.res_plane + off, e.res.js, cols, p.res_vec);
+        load_res(r, static_cast<const __half*>(e.res.p) + off, e.res.js, cols, p.res_vec);
     }
+  }
+  if (p.polar.mode == kPolarNone) {
+    if (e.res.p) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = fmaf(e.beta, r[c], v[c]);
+    }
+  } else {
+    polar_epilogue(v, r, p.polar, e, b, i, j, rows, cols, lane);
   }
   const GemmView flip{e.y.p, e.y.bs, e.y.js, e.y.is};
   if constexpr (std::is_same<OUT, Halves>::value) {
@@ -626,6 +680,7 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   p.b_bytes = (p.q_inner ? (p.share + 63) / 64 * 64 : p.share) * BK * 2;
   p.idesc = mma_idesc(t.f16, p.p_inner, p.q_inner, BM * CG, p.BN);
   p.e = t.e;
+  p.polar = t.polar;
   p.res_kind = t.res;
   p.y_plane = t.y_plane;
   p.res_plane = t.res_plane;

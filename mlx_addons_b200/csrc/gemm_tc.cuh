@@ -23,6 +23,24 @@ struct TcOperand {
   int bcast;             // one matrix for the whole batch
 };
 
+// The epilogues of an orthogonalisation step (polar.cu). S and P are stored
+// without their diagonals, which are kept as float32 vectors: near the end of
+// the iteration the diagonal is most of them, and so most of what f16 would
+// round away.
+//   kPolarS     y = alpha r^2 D off the diagonal, d_out = k r^2 D on it
+//   kPolarP     y = alpha D + (beta + k (d_i + d_j)) res off it,
+//               d_out = k2 D + k3 d^2 + k4 d on it
+//   kPolarXi/j  y = r (alpha D + beta (k + d_i or d_j) res)
+enum TcPolarMode { kPolarNone = 0, kPolarS, kPolarP, kPolarXi, kPolarXj };
+struct TcPolar {
+  int mode;
+  const float* r;     // one factor a matrix, or null (1)
+  const float* d_in;  // (batch, side)
+  float* d_out;       // (batch, side)
+  int64_t side;
+  float k, k2, k3, k4;
+};
+
 struct TcProblem {
   TcOperand P, Q;
   int kind;              // TcKind of both operands
@@ -32,6 +50,7 @@ struct TcProblem {
   int out;               // B2C_F32 / B2C_BF16 / B2C_F16 with e.y, e.pre and e.bias of that type, or kOutHalves
   int res;               // the type of e.res, or kOutHalves
   int64_t y_plane, res_plane;  // plane strides, elements, where kOutHalves
+  TcPolar polar;
   int sym;               // D is symmetric (P and Q the same, or commuting symmetric): compute the lower tiles, mirror them
 };
 constexpr int kOutHalves = 3;

@@ -9,12 +9,12 @@
 
 #include "b2c_kernels.cuh"
 #include "gemm_tc.cuh"
+#include "polar.cuh"
 
 namespace b2c {
 
 namespace {
 
-constexpr float kScaleX = 16384.f;
 constexpr int kNormThreads = 256;
 constexpr int kNormParts = kNormThreads;  // most partial sums of a matrix
 
@@ -90,23 +90,27 @@ __global__ void __launch_bounds__(kNormThreads) polar_norm_kernel(const PolarIn 
   }
 }
 
-// X = G / (|G|_F + eps) times 2^14, as one or two f16 planes, rows padded to
-// units of 8.
+// G times the power of two that puts |G|_F + eps in [2^13, 2^14), as one or two
+// f16 planes, rows padded to units of 8; r = 2^14 X / that, in [1, 2], is left
+// to the first step. So a bfloat16 G is held without a rounding, which the
+// iteration would amplify by up to 3.4445^steps in its smallest directions.
 template <typename T, bool HALVES>
 __global__ void __launch_bounds__(kNormThreads) polar_scale_kernel(const PolarIn in, const double* part, int parts,
-                                                                   double eps, __half* X, int64_t pitch, int64_t plane) {
+                                                                   double eps, __half* X, int64_t pitch, int64_t plane,
+                                                                   float* r) {
   __shared__ double red[kNormThreads / 32];
   for (int64_t b = blockIdx.y; b < in.batch; b += gridDim.y) {
     const T* base = static_cast<const T*>(in.G) + b * in.bs;
     const double sum = block_sum((int)threadIdx.x < parts ? part[b * kNormParts + threadIdx.x] : 0.0, red);
-    const double inv = kScaleX / (sqrt(sum) + eps);
+    const PolarNorm norm = polar_norm(sqrt(sum) + eps);
+    if (blockIdx.x == 0 && threadIdx.x == 0) r[b] = norm.r;
     for (Walk w(in.n, gridDim.x, blockIdx.x); w.r < in.m; w.next()) {
       float v[8];
       load_unit<T>(in, base + w.r * in.rs, w.u * 8, v);
       __align__(16) __half hi[8], lo[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float x = (float)((double)v[k] * inv);
+        const float x = (float)((double)v[k] * norm.scale);
         hi[k] = __float2half_rn(x);
         lo[k] = __float2half_rn(x - __half2float(hi[k]));
       }
@@ -134,7 +138,7 @@ PolarParams along_rows(const PolarParams& in) {
 
 // Scratch of the product form: norms, two X, S and P.
 struct PolarLayout {
-  int64_t side, pitch_x, pitch_s, x_plane, s_plane, x_bytes, s_bytes, part_bytes;
+  int64_t side, pitch_x, pitch_s, x_plane, s_plane, x_bytes, s_bytes, part_bytes, vec_bytes;
   int planes;
 };
 
@@ -149,13 +153,8 @@ PolarLayout polar_layout(const PolarParams& p) {
   l.x_bytes = (l.x_plane * l.planes * 2 + 255) / 256 * 256;
   l.s_bytes = (l.s_plane * l.planes * 2 + 255) / 256 * 256;
   l.part_bytes = (p.batch * kNormParts * (int64_t)sizeof(double) + 255) / 256 * 256;
+  l.vec_bytes = (p.batch * l.side * (int64_t)sizeof(float) + 255) / 256 * 256;
   return l;
-}
-
-// The largest power of two that keeps values up to `bound` within f16's 2^15.
-float scale_for(double bound) {
-  const double b = bound < 1e-3 ? 1e-3 : bound;
-  return (float)exp2(floor(log2(32768.0 / b)));
 }
 
 template <typename T>
@@ -170,6 +169,10 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   __half* S = reinterpret_cast<__half*>(w + 2 * l.x_bytes);
   __half* P = reinterpret_cast<__half*>(w + 2 * l.x_bytes + l.s_bytes);
   constexpr int64_t PER = 16 / sizeof(T);
+  w += 2 * l.x_bytes + 2 * l.s_bytes;
+  float* ds = reinterpret_cast<float*>(w);  // diagonals of S and P
+  float* dp = reinterpret_cast<float*>(w + l.vec_bytes);
+  float* r = reinterpret_cast<float*>(w + 2 * l.vec_bytes);
   const PolarIn in{p.G, p.bs, p.rs, p.cs, p.batch, p.m, p.n,
                    (reinterpret_cast<uintptr_t>(p.G) & 15) == 0 && p.cs == 1 && p.rs % PER == 0 && p.bs % PER == 0};
   const int64_t units = p.m * ((p.n + 7) / 8);
@@ -179,7 +182,7 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   const dim3 grid((unsigned)blocks, (unsigned)(p.batch < 65535 ? p.batch : 65535));
   polar_norm_kernel<T><<<grid, kNormThreads, 0, s>>>(in, part);
   constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
-  polar_scale_kernel<T, kTwo><<<grid, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0, l.pitch_x, l.x_plane);
+  polar_scale_kernel<T, kTwo><<<grid, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0, l.pitch_x, l.x_plane, r);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
 
@@ -195,7 +198,7 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   double hi = 1.0;
   for (int step = 0; step < p.steps; ++step) {
     const double a = p.coef[3 * step], b = p.coef[3 * step + 1], c = p.coef[3 * step + 2], t2 = hi * hi;
-    const float ss = scale_for(t2), sp = scale_for(fabs(b) * t2 + fabs(c) * t2 * t2);
+    const float ss = polar_scale_for(t2), sp = polar_scale_for(fabs(b) * t2 + fabs(c) * t2 * t2);
     const TcOperand x_rows{X0, xx, l.pitch_x, l.x_plane, 0, bcast}, x_cols{X0, xx, l.pitch_x, l.x_plane, 1, bcast};
     // S = X X^T (X^T X), the lower half of its tiles
     t.I = t.J = side;
@@ -204,7 +207,13 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
     t.sym = 1;
     t.e = GemmEpilogue{};
     t.e.y = GemmView{S, sx, l.pitch_s, 1};
-    t.e.alpha = ss / (kScaleX * kScaleX);
+    t.e.alpha = ss / (kPolarScale * kPolarScale);
+    t.polar = TcPolar{};
+    t.polar.mode = kPolarS;
+    t.polar.r = step ? nullptr : r;
+    t.polar.d_in = t.polar.d_out = ds;
+    t.polar.side = side;
+    t.polar.k = 1.f / ss;
     t.out = t.res = inner;
     t.y_plane = t.res_plane = l.s_plane;
     if ((e = launch_gemm_tc(t, s)) != cudaSuccess) return e;
@@ -215,10 +224,17 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
     t.e.res = GemmView{S, sx, l.pitch_s, 1};
     t.e.alpha = (float)(c * sp / ((double)ss * ss));
     t.e.beta = (float)(b * sp / ss);
+    t.polar.mode = kPolarP;
+    t.polar.r = nullptr;
+    t.polar.d_out = dp;
+    t.polar.k = (float)(c * sp / ss);
+    t.polar.k2 = 1.f / sp;
+    t.polar.k3 = (float)c;
+    t.polar.k4 = (float)b;
     if ((e = launch_gemm_tc(t, s)) != cudaSuccess) return e;
     // X' = P X + a X (X P + a X); P is symmetric, so either of its indices may be contracted
     const bool last = step == p.steps - 1;
-    const float so = last ? 1.f : kScaleX;
+    const float so = last ? 1.f : kPolarScale;
     t.I = p.m;
     t.J = p.n;
     t.P = wide ? p_op : x_rows;
@@ -226,8 +242,12 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
     t.sym = 0;
     t.e.y = last ? GemmView{p.out, mn, p.out_rs, p.out_cs} : GemmView{X1, xx, l.pitch_x, 1};
     t.e.res = GemmView{X0, xx, l.pitch_x, 1};
-    t.e.alpha = so / (sp * kScaleX);
-    t.e.beta = (float)(a * so / kScaleX);
+    t.e.alpha = so / (sp * kPolarScale);
+    t.e.beta = so / kPolarScale;
+    t.polar.mode = wide ? kPolarXi : kPolarXj;
+    t.polar.r = step ? nullptr : r;
+    t.polar.d_in = dp;
+    t.polar.k = (float)a;
     t.out = last ? p.dtype : inner;
     t.y_plane = last ? 0 : l.x_plane;
     t.res_plane = l.x_plane;
@@ -265,12 +285,19 @@ double polar_poly_bound(double a, double b, double c, double hi) {
 
 size_t polar_ws_bytes(const PolarParams& in) {
   const PolarParams p = along_rows(in);
+  if (polar_cta_fits(p)) return 0;
   const PolarLayout l = polar_layout(p);
-  return (size_t)(l.part_bytes + 2 * l.x_bytes + 2 * l.s_bytes);
+  return (size_t)(l.part_bytes + 2 * l.x_bytes + 2 * l.s_bytes + 3 * l.vec_bytes);
 }
 
 cudaError_t launch_polar(const PolarParams& in, cudaStream_t s) {
   const PolarParams p = along_rows(in);
+  if (polar_cta_fits(p)) {
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return e == cudaSuccess ? launch_polar_cta(p, sms, s) : e;
+  }
   switch (p.dtype) {
     case B2C_F32: return launch_t<float>(p, s);
     case B2C_BF16: return launch_t<__nv_bfloat16>(p, s);

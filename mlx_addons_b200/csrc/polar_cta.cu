@@ -1,0 +1,471 @@
+// Newton-Schulz orthogonalisation of small matrices, the whole iteration in
+// one CTA: X (smaller side `side` <= 128, longer side L) stays in shared
+// memory as f16 planes, S and P share a second buffer, the sums are in tensor
+// memory, and the matrix is read and written once.
+//
+// A CTA stacks g = 128 / side matrices (fewer where that would leave SMs
+// idle) into the 128 rows of the tensor-core tile. S of the stack is block
+// diagonal: only the diagonal blocks are written to shared memory, the rest of
+// that buffer stays zero, and so P and P X keep the matrices apart. A matrix
+// with a non-finite entry is left out (zeros) and written as NaN, since 0 * NaN
+// would reach its neighbours.
+//
+// The buffer of X serves as three operands without a copy. Its layout, blocks
+// of 64 columns with 128-byte swizzled rows, is K-major for S = X X^T and, read
+// the other way, MN-major for P X.
+//
+// Bound by the phases of a step in turn (product, conversion of the sums to
+// the next operand, barrier): two CTAs share an SM and fill each other's gaps.
+#include <cstdlib>
+#include <cstring>
+
+#include "b2c_kernels.cuh"
+#include "gemm_tc.cuh"
+#include "polar.cuh"
+#include "tcgen05.cuh"
+
+namespace b2c {
+
+__device__ unsigned int g_polar_fault;
+
+namespace {
+
+constexpr int kThreadsC = 256;
+constexpr int kBlockBytes = 16384;  // 128 rows x 64 columns of f16
+constexpr int kMaxStepsC = 64;
+constexpr int kSmemMaxC = 232448 - 4096;
+
+// S is stored times ss, P times sp; the sums of S are 2^28 S, of P ss^2 S S,
+// of P X 2^14 sp P X.
+struct CtaStep {
+  float k1, k2, k3, k4, kp;  // ss / 2^28, c sp / ss^2, b sp / 2^28, 1 / sp, sp / 2^28
+  float a, b, c;
+};
+constexpr float kUnitS = 1.f / (kPolarScale * kPolarScale);
+
+struct CtaParams {
+  const void* G;
+  int64_t bs, sr, sl;     // strides of batch, small index, long index
+  void* out;
+  int64_t obs, orr, ol;
+  int64_t batch;
+  int side, L, g, xblocks, sblocks, kk, steps, along_l, lanes_per_row, vec_in, vec_out, inject;
+  double eps;
+  CtaStep step[kMaxStepsC];
+};
+
+// Byte offset of 8 columns (16 bytes) of a row in a 128-byte swizzled buffer
+// of 64-column blocks.
+__device__ __forceinline__ int unit_off(int row, int col8) {
+  return (col8 >> 3) * kBlockBytes + row * 128 + (((col8 & 7) ^ (row & 7)) << 4);
+}
+
+__device__ __forceinline__ uint64_t block_desc(uint32_t addr, int inner) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(inner ? (kBlockBytes >> 4) : 1) << 16) |
+         ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int PLANES>
+__device__ __forceinline__ void store_unit(unsigned char* buf, int plane_bytes, int off, const float (&v)[8]) {
+  __align__(16) __half h[8], l[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    h[k] = __float2half_rn(v[k]);
+    if constexpr (PLANES == 2) l[k] = __float2half_rn(v[k] - __half2float(h[k]));
+  }
+  *reinterpret_cast<uint4*>(buf + off) = *reinterpret_cast<const uint4*>(h);
+  if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(buf + plane_bytes + off) = *reinterpret_cast<const uint4*>(l);
+}
+
+// 8 elements of a row, zeros past its end.
+template <typename T>
+__device__ __forceinline__ void load_unit8(const T* row, int64_t stride, int c, int n, int vec, float (&v)[8]) {
+  if (vec && c + 8 <= n) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < 8 / PER; ++q) {
+      const uint4 w = *reinterpret_cast<const uint4*>(row + c + q * PER);
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[q * PER + k] = to_f32(e[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < n ? to_f32(row[(c + k) * stride]) : 0.f;
+  }
+}
+
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_constant__ CtaParams p) {
+  extern __shared__ unsigned char raw[];
+  __shared__ double rowsum[256], factor[128];
+  __shared__ float first_r[128], sdiag[128], pdiag[128];
+  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* X = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
+  const int x_plane = p.xblocks * kBlockBytes, s_plane = p.sblocks * kBlockBytes;
+  unsigned char* S = X + PLANES * x_plane;
+  const uint32_t done = smem_u32(bars), never = done + 8;
+  const uint64_t limit = p.inject ? 1000000ull : kWaitNs;
+  volatile int* gu = &gave_up;
+
+  if (tid == 0) {
+    gave_up = 0;
+    bar_init(done, 1);
+    bar_init(never, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    fence_before();
+  }
+  // ---- norms ----
+  const int64_t m0 = (int64_t)blockIdx.x * p.g;
+  const int have = (int)(p.batch - m0 < p.g ? p.batch - m0 : p.g), rows = have * p.side;
+  const T* G = static_cast<const T*>(p.G) + m0 * p.bs;
+  for (int e = tid * 16; e < PLANES * (x_plane + s_plane); e += kThreadsC * 16)
+    *reinterpret_cast<uint4*>(X + e) = make_uint4(0, 0, 0, 0);
+  // rows of X: `lpr` lanes take the 8-element units of a row in turn (its neighbours lie along the lanes), or, where the
+  // small index has the smaller stride, two threads share a row and the lanes run along the rows
+  const int units = (p.L + 7) / 8, lpr = p.lanes_per_row;
+  if (p.along_l) {
+    const int per = 32 / lpr, sub = lane / lpr, u0 = lane % lpr;
+    for (int r0 = warp * per; r0 < rows; r0 += 8 * per) {
+      const int r = r0 + sub, m = r / p.side;
+      const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
+      double s = 0.0;
+      if (r < rows) {
+#pragma unroll 2
+        for (int u = u0; u < units; u += lpr) {
+          float v[8];
+          load_unit8<T>(row, p.sl, u * 8, p.L, p.vec_in, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
+        }
+      }
+      for (int o = lpr / 2; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+      if (u0 == 0 && r < rows) rowsum[r] = s, rowsum[r + 128] = 0.0;
+    }
+  } else {
+    const int r = tid & 127, m = r / p.side;
+    const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
+    double s = 0.0;
+    if (r < rows) {
+      for (int u = tid >> 7; u < units; u += 2) {
+        float v[8];
+        load_unit8<T>(row, p.sl, u * 8, p.L, 0, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
+      }
+    }
+    rowsum[tid] = s;
+  }
+  __syncthreads();
+  if (tid < have) {
+    double s = 0.0;
+    for (int r = 0; r < p.side; ++r) s += rowsum[tid * p.side + r] + rowsum[tid * p.side + r + 128];
+    const PolarNorm n = polar_norm(sqrt(s) + p.eps);
+    factor[tid] = n.scale;
+    first_r[tid] = n.r;
+  }
+  __syncthreads();
+  // ---- X = G / (|G| + eps), up to the factor r ----
+  if (p.along_l) {
+    const int per = 32 / lpr, sub = lane / lpr, u0 = lane % lpr;
+    for (int r = warp * per + sub; r < rows; r += 8 * per) {
+      const int m = r / p.side;
+      const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
+      const double f = factor[m];
+      if (f == 0.0) continue;
+#pragma unroll 2
+      for (int u = u0; u < units; u += lpr) {
+        float v[8];
+        load_unit8<T>(row, p.sl, u * 8, p.L, p.vec_in, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)((double)v[e] * f);
+        store_unit<PLANES>(X, x_plane, unit_off(r, u), v);
+      }
+    }
+  } else {
+    const int r = tid & 127, m = r / p.side;
+    const double f = r < rows ? factor[m] : 0.0;
+    if (f != 0.0) {
+      const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
+      for (int u = tid >> 7; u < units; u += 2) {
+        float v[8];
+        load_unit8<T>(row, p.sl, u * 8, p.L, 0, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)((double)v[e] * f);
+        store_unit<PLANES>(X, x_plane, unit_off(r, u), v);
+      }
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot, xa = smem_u32(X), sa = smem_u32(S);
+  const uint32_t idesc_s = mma_idesc(1, 0, 0, 128, p.kk);
+  constexpr int SEGS = PLANES == 2 ? 3 : 1;
+  const int seg_p[3] = {PLANES - 1, 0, 0}, seg_q[3] = {0, PLANES - 1, 0};  // small products first
+  uint32_t phase = 0;
+  if (p.inject && blockIdx.x == 0) bar_wait(never, 0, gu, limit, &g_polar_fault);
+  auto wait = [&] {
+    bar_wait(done, phase, gu, limit, &g_polar_fault);
+    phase ^= 1;
+    fence_after();
+  };
+
+  // this lane's row, its matrix and where that matrix lies among the columns of S
+  const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+  const int mine = row / p.side, lo = mine * p.side, hi = mine < p.g ? lo + p.side : lo;
+  const int first = quad * 32 / p.side * p.side, last = min((quad * 32 + 31) / p.side * p.side + p.side, p.kk);
+  const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+
+  const float r0 = row < rows && factor[mine] != 0.0 ? first_r[mine] : 1.f;
+  // with one plane, S and P are held without their diagonals, which stay in float32 (see polar.cu)
+  constexpr bool kSplitDiag = PLANES == 1;
+  for (int t = 0; t < p.steps; ++t) {
+    const CtaStep k = p.step[t];
+    const float f1 = t ? 1.f : r0, f2 = f1 * f1;
+    // ---- S = X X^T ----
+    if (tid == 0) {
+      for (int s = 0; s < SEGS; ++s)
+        for (int b = 0; b < p.xblocks; ++b)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            mma<1>(tmem, block_desc(xa + seg_p[s] * x_plane + b * kBlockBytes + q * 32, 0),
+                   block_desc(xa + seg_q[s] * x_plane + b * kBlockBytes + q * 32, 0), idesc_s, s + b + q > 0);
+      commit<1>(done);
+    }
+    wait();
+    for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
+      if (((c0 >> 5) & 1) != half) continue;
+      float v[32];
+      tmem_row32(lanes + c0, v);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int c = c0 + u * 8 + e;
+          const float x = v[u * 8 + e] * f2;
+          if (kSplitDiag && c == row) sdiag[row] = x * kUnitS;
+          w[e] = c >= lo && c < hi && !(kSplitDiag && c == row) ? x * k.k1 : 0.f;
+        }
+        if (c0 + u * 8 < p.kk) store_unit<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), w);
+      }
+    }
+    fence_before();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    fence_after();
+    // ---- P = c S S + b S ----
+    if (tid == 0) {
+      for (int s = 0; s < SEGS; ++s)
+        for (int q = 0; q < p.kk / 16; ++q) {
+          const int off = (q >> 2) * kBlockBytes + (q & 3) * 32;
+          mma<1>(tmem + 128, block_desc(sa + seg_p[s] * s_plane + off, 0), block_desc(sa + seg_q[s] * s_plane + off, 0),
+                 idesc_s, s + q > 0);
+        }
+      commit<1>(done);
+    }
+    wait();
+    const float di = kSplitDiag && row < p.kk ? sdiag[row] : 0.f;
+    for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
+      if (((c0 >> 5) & 1) != half) continue;
+      float v[32], w[32];
+      tmem_row32(lanes + c0, v);
+      tmem_row32(lanes + 128 + c0, w);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int c = c0 + u * 8 + e;
+          const float o = v[u * 8 + e] * f2, oo = w[u * 8 + e] * k.k2;
+          if constexpr (kSplitDiag) {
+            const float b = fmaf(k.c, di + sdiag[c], k.b) * k.kp;
+            x[e] = c >= lo && c < hi && c != row ? fmaf(o, b, oo) : 0.f;
+            if (c == row) pdiag[row] = fmaf(oo, k.k4, di * fmaf(k.c, di, k.b));
+          } else {
+            x[e] = c >= lo && c < hi ? fmaf(o, k.k3, oo) : 0.f;
+          }
+        }
+        if (c0 + u * 8 < p.kk) store_unit<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), x);
+      }
+    }
+    fence_before();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    fence_after();
+    const float ka = kSplitDiag ? k.a + (row < p.kk ? pdiag[row] : 0.f) : k.a;
+    // ---- X <- P X + a X, up to 256 columns at a time ----
+    for (int b0 = 0; b0 < p.xblocks; b0 += 4) {
+      const int nb = min(4, p.xblocks - b0);
+      if (tid == 0) {
+        const uint32_t idesc_x = mma_idesc(1, 0, 1, 128, nb * 64);
+        for (int s = 0; s < SEGS; ++s)
+          for (int q = 0; q < p.kk / 16; ++q)
+            mma<1>(tmem, block_desc(sa + seg_p[s] * s_plane + (q >> 2) * kBlockBytes + (q & 3) * 32, 0),
+                   block_desc(xa + seg_q[s] * x_plane + b0 * kBlockBytes + q * 2048, 1), idesc_x, s + q > 0);
+        commit<1>(done);
+      }
+      wait();
+      for (int c0 = half * 32; c0 < nb * 64; c0 += 64) {
+        float v[32];
+        tmem_row32(lanes + c0, v);
+        const int c = b0 * 64 + c0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int off = unit_off(row, (c >> 3) + u);
+          const uint4 xh = *reinterpret_cast<const uint4*>(X + off);
+          const __half* h = reinterpret_cast<const __half*>(&xh);
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = __half2float(h[e]);
+          if constexpr (PLANES == 2) {
+            const uint4 xl = *reinterpret_cast<const uint4*>(X + x_plane + off);
+            const __half* l = reinterpret_cast<const __half*>(&xl);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] += __half2float(l[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u * 8 + e] = f1 * fmaf(ka, w[e], v[u * 8 + e] * k.k4);
+          if (t < p.steps - 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = v[u * 8 + e];
+            store_unit<PLANES>(X, x_plane, off, w);
+          }
+        }
+        if (t == p.steps - 1 && row < rows) {
+          const float nan = __int_as_float(0x7fffffff);
+          const float f = factor[mine] == 0.0 || *gu ? nan : 1.f / kPolarScale;
+          T* o = static_cast<T*>(p.out) + (m0 + mine) * p.obs + (row - lo) * p.orr + c * p.ol;
+          constexpr int PER = 16 / sizeof(T);
+          if (p.vec_out && c + 32 <= p.L) {
+#pragma unroll
+            for (int u = 0; u < 32 / PER; ++u) {
+              uint4 w;
+              T* q = reinterpret_cast<T*>(&w);
+#pragma unroll
+              for (int e = 0; e < PER; ++e) q[e] = from_f32<T>(v[u * PER + e] * f);
+              *reinterpret_cast<uint4*>(o + u * PER) = w;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c + e < p.L) o[e * p.ol] = from_f32<T>(v[e] * f);
+          }
+        }
+      }
+      fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncthreads();
+      fence_after();
+    }
+  }
+  if (gave_up) {
+    // MMAs still in flight end within microseconds
+    const uint64_t t0 = now_ns();
+    while (now_ns() - t0 < 20000000ull) {
+    }
+    __syncthreads();
+  }
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+}
+
+bool inject_timeout() {
+  const char* t = getenv("B2C_GEMM_INJECT_TIMEOUT");
+  return t && strcmp(t, "1") == 0;
+}
+
+template <typename T, int PLANES>
+cudaError_t launch_c(const CtaParams& p, size_t smem, unsigned grid, cudaStream_t s) {
+  auto kern = polar_cta_kernel<T, PLANES>;
+  static int cache[64];
+  int occ = 0;
+  const cudaError_t e = kernel_occupancy(kern, kThreadsC, smem, cache, &occ);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, kThreadsC, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+int64_t smem_of(int planes, int64_t xblocks, int64_t sblocks) { return 1024 + planes * (xblocks + sblocks) * kBlockBytes; }
+
+// Planes that fit with one matrix's S: two, or one for bfloat16 results only;
+// 0 if the matrix is too large. Two planes cost three products instead of one,
+// which these sizes hide, and leave a bfloat16 result its own rounding alone.
+int planes_of(const PolarParams& p) {
+  const int64_t side = p.m < p.n ? p.m : p.n, L = p.m < p.n ? p.n : p.m;
+  if (side > 128) return 0;
+  const int64_t x = (L + 63) / 64, sb = side <= 64 ? 1 : 2;
+  if (smem_of(2, x, sb) <= kSmemMaxC) return 2;
+  return p.dtype == B2C_BF16 && smem_of(1, x, sb) <= kSmemMaxC ? 1 : 0;
+}
+
+}  // namespace
+
+bool polar_cta_fits(const PolarParams& p) { return planes_of(p) > 0; }
+
+cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
+  CtaParams p{};
+  const bool wide = in.m <= in.n;
+  const int planes = planes_of(in);
+  p.G = in.G;
+  p.bs = in.bs, p.sr = wide ? in.rs : in.cs, p.sl = wide ? in.cs : in.rs;
+  p.out = in.out;
+  p.obs = in.m * in.n, p.orr = wide ? in.out_rs : in.out_cs, p.ol = wide ? in.out_cs : in.out_rs;
+  p.batch = in.batch;
+  p.side = (int)(wide ? in.m : in.n);
+  p.L = (int)(wide ? in.n : in.m);
+  p.xblocks = (p.L + 63) / 64;
+  // matrices of a CTA: no more than keeps two CTAs on every SM, and than fit with their S
+  int64_t g = (in.batch + 2 * sms - 1) / (2 * sms);
+  if (g > 128 / p.side) g = 128 / p.side;
+  while (g > 1 && smem_of(planes, p.xblocks, (g * p.side + 63) / 64) > kSmemMaxC) --g;
+  p.g = (int)g;
+  p.kk = (p.g * p.side + 15) / 16 * 16;
+  p.sblocks = (p.kk + 63) / 64;
+  p.along_l = p.sl <= p.sr || p.side == 1;
+  p.steps = in.steps;
+  p.eps = in.eps;
+  p.inject = inject_timeout();
+  p.lanes_per_row = 1;
+  while (p.lanes_per_row < 32 && p.lanes_per_row * 8 < p.L) p.lanes_per_row *= 2;
+  const int64_t per = in.dtype == B2C_F32 ? 4 : 8;
+  p.vec_in = p.sl == 1 && (reinterpret_cast<uintptr_t>(in.G) & 15) == 0 && p.sr % per == 0 && p.bs % per == 0;
+  const int64_t elt = in.dtype == B2C_F32 ? 4 : 2;
+  p.vec_out = p.ol == 1 && (reinterpret_cast<uintptr_t>(in.out) & 15) == 0 && p.orr * elt % 16 == 0 && p.obs * elt % 16 == 0;
+  double hi = 1.0;
+  for (int t = 0; t < in.steps; ++t) {
+    const double a = in.coef[3 * t], b = in.coef[3 * t + 1], c = in.coef[3 * t + 2], t2 = hi * hi, sx = kPolarScale;
+    const double ss = polar_scale_for(t2), sp = polar_scale_for(fabs(b) * t2 + fabs(c) * t2 * t2);
+    p.step[t] = CtaStep{(float)(ss / (sx * sx)), (float)(c * sp / (ss * ss)), (float)(b * sp / (sx * sx)), (float)(1 / sp),
+                        (float)(sp / (sx * sx)), (float)a, (float)b, (float)c};
+    hi = polar_poly_bound(a, b, c, hi);
+  }
+  size_t smem = (size_t)smem_of(planes, p.xblocks, p.sblocks);
+  if (smem < 77 * 1024) smem = 77 * 1024;  // two CTAs at most: each holds half of the tensor memory
+  const int64_t ctas = (in.batch + g - 1) / g;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const unsigned grid = (unsigned)ctas;
+  switch (in.dtype) {
+    case B2C_F32: return launch_c<float, 2>(p, smem, grid, s);
+    case B2C_BF16:
+      return planes == 2 ? launch_c<__nv_bfloat16, 2>(p, smem, grid, s) : launch_c<__nv_bfloat16, 1>(p, smem, grid, s);
+    default: return launch_c<__half, 2>(p, smem, grid, s);
+  }
+}
+
+cudaError_t polar_take_fault(unsigned int* fault) {
+  unsigned int f = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&f, g_polar_fault, sizeof(unsigned int));
+  if (e != cudaSuccess) return e;
+  *fault |= f;
+  return cudaMemcpyToSymbol(g_polar_fault, &zero, sizeof(unsigned int));
+}
+
+}  // namespace b2c
