@@ -22,12 +22,17 @@ inline float polar_scale_for(double bound) {
 struct PolarNorm {
   double scale;
   float r;
+  int e;  // scale = 2^e
+  // The scale as two float powers of two, neither beyond float's range.
+  __device__ __forceinline__ float2 half_scale() const {
+    return scale == 0.0 ? make_float2(0.f, 0.f) : make_float2(scalbnf(1.f, e / 2), scalbnf(1.f, e - e / 2));
+  }
 };
 __device__ __forceinline__ PolarNorm polar_norm(double norm) {
-  if (!isfinite(norm) || norm == 0.0) return PolarNorm{0.0, __int_as_float(0x7fffffff)};
+  if (!isfinite(norm) || norm == 0.0) return PolarNorm{0.0, __int_as_float(0x7fffffff), 0};
   int q;
   const double f = frexp(norm, &q);
-  return PolarNorm{scalbn(16384.0, -q), (float)(1.0 / f)};
+  return PolarNorm{scalbn(16384.0, -q), (float)(1.0 / f), 14 - q};
 }
 
 // Both take a problem whose rows lie no closer together than its columns.

@@ -30,9 +30,9 @@ __device__ unsigned int g_polar_fault;
 
 namespace {
 
-constexpr int kThreadsC = 256;
 constexpr int kBlockBytes = 16384;  // 128 rows x 64 columns of f16
 constexpr int kMaxStepsC = 64;
+constexpr int kRowsInFlight = 4;  // rows that a warp loads at a time
 constexpr int kSmemMaxC = 232448 - 4096;
 
 // S is stored times ss, P times sp; the sums of S are 2^28 S, of P ss^2 S S,
@@ -49,7 +49,7 @@ struct CtaParams {
   void* out;
   int64_t obs, orr, ol;
   int64_t batch;
-  int side, L, g, xblocks, sblocks, kk, steps, along_l, lanes_per_row, vec_in, vec_out, inject;
+  int side, L, g, xblocks, sblocks, kk, steps, along_l, lanes_per_row, blockwise, vec_in, vec_out, inject;
   double eps;
   CtaStep step[kMaxStepsC];
 };
@@ -67,11 +67,14 @@ __device__ __forceinline__ uint64_t block_desc(uint32_t addr, int inner) {
 
 template <int PLANES>
 __device__ __forceinline__ void store_unit(unsigned char* buf, int plane_bytes, int off, const float (&v)[8]) {
-  __align__(16) __half h[8], l[8];
+  __align__(16) __half2 h[4], l[4];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    h[k] = __float2half_rn(v[k]);
-    if constexpr (PLANES == 2) l[k] = __float2half_rn(v[k] - __half2float(h[k]));
+  for (int k = 0; k < 4; ++k) {
+    h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+    if constexpr (PLANES == 2) {
+      const float2 f = __half22float2(h[k]);
+      l[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
+    }
   }
   *reinterpret_cast<uint4*>(buf + off) = *reinterpret_cast<const uint4*>(h);
   if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(buf + plane_bytes + off) = *reinterpret_cast<const uint4*>(l);
@@ -95,14 +98,16 @@ __device__ __forceinline__ void load_unit8(const T* row, int64_t stride, int c, 
   }
 }
 
-template <typename T, int PLANES>
-__global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_constant__ CtaParams p) {
+template <typename T, int PLANES, int NT>
+__global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_constant__ CtaParams p) {
   extern __shared__ unsigned char raw[];
-  __shared__ double rowsum[256], factor[128];
+  __shared__ double rowsum[NT];
+  __shared__ float2 factor[128];  // the scale of a matrix as two powers of two, 0 for a broken one
   __shared__ float first_r[128], sdiag[128], pdiag[128];
   __shared__ __align__(8) uint64_t bars[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
+  constexpr int NW = NT / 32, NG = NT / 128;  // warps; threads that share a row of X
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* X = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int x_plane = p.xblocks * kBlockBytes, s_plane = p.sblocks * kBlockBytes;
@@ -126,35 +131,45 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
   const int64_t m0 = (int64_t)blockIdx.x * p.g;
   const int have = (int)(p.batch - m0 < p.g ? p.batch - m0 : p.g), rows = have * p.side;
   const T* G = static_cast<const T*>(p.G) + m0 * p.bs;
-  for (int e = tid * 16; e < PLANES * (x_plane + s_plane); e += kThreadsC * 16)
+  for (int e = tid * 16; e < PLANES * (x_plane + s_plane); e += NT * 16)
     *reinterpret_cast<uint4*>(X + e) = make_uint4(0, 0, 0, 0);
   // rows of X: `lpr` lanes take the 8-element units of a row in turn (its neighbours lie along the lanes), or, where the
-  // small index has the smaller stride, two threads share a row and the lanes run along the rows
+  // small index has the smaller stride, NG threads share a row and the lanes run along the rows
   const int units = (p.L + 7) / 8, lpr = p.lanes_per_row;
   if (p.along_l) {
     const int per = 32 / lpr, sub = lane / lpr, u0 = lane % lpr;
-    for (int r0 = warp * per; r0 < rows; r0 += 8 * per) {
-      const int r = r0 + sub, m = r / p.side;
-      const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
-      double s = 0.0;
-      if (r < rows) {
-#pragma unroll 2
-        for (int u = u0; u < units; u += lpr) {
-          float v[8];
-          load_unit8<T>(row, p.sl, u * 8, p.L, p.vec_in, v);
+    for (int r0 = warp * per; r0 < rows; r0 += NW * per * kRowsInFlight) {
+      double s[kRowsInFlight] = {};
+      for (int u = u0; u < units; u += lpr) {
+        float v[kRowsInFlight][8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
+        for (int k = 0; k < kRowsInFlight; ++k) {
+          const int r = r0 + sub + k * NW * per, m = r / p.side;
+          load_unit8<T>(G + m * p.bs + (r - m * p.side) * p.sr, p.sl, u * 8, r < rows ? p.L : 0, p.vec_in, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsInFlight; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[k] += (double)v[k][e] * (double)v[k][e];
+      }
+      for (int o = lpr / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < kRowsInFlight; ++k) s[k] += __shfl_xor_sync(kFull, s[k], o);
+#pragma unroll
+      for (int k = 0; k < kRowsInFlight; ++k) {
+        const int r = r0 + sub + k * NW * per;
+        if (u0 == 0 && r < rows) {
+#pragma unroll
+          for (int g = 0; g < NG; ++g) rowsum[r + 128 * g] = g ? 0.0 : s[k];
         }
       }
-      for (int o = lpr / 2; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
-      if (u0 == 0 && r < rows) rowsum[r] = s, rowsum[r + 128] = 0.0;
     }
   } else {
     const int r = tid & 127, m = r / p.side;
     const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
     double s = 0.0;
     if (r < rows) {
-      for (int u = tid >> 7; u < units; u += 2) {
+      for (int u = tid >> 7; u < units; u += NG) {
         float v[8];
         load_unit8<T>(row, p.sl, u * 8, p.L, 0, v);
 #pragma unroll
@@ -164,41 +179,52 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
     rowsum[tid] = s;
   }
   __syncthreads();
-  if (tid < have) {
+  for (int m = warp; m < have; m += NW) {
     double s = 0.0;
-    for (int r = 0; r < p.side; ++r) s += rowsum[tid * p.side + r] + rowsum[tid * p.side + r + 128];
-    const PolarNorm n = polar_norm(sqrt(s) + p.eps);
-    factor[tid] = n.scale;
-    first_r[tid] = n.r;
+    for (int r = lane; r < p.side; r += 32)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) s += rowsum[m * p.side + r + 128 * g];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+    if (lane == 0) {
+      const PolarNorm n = polar_norm(sqrt(s) + p.eps);
+      factor[m] = n.half_scale();
+      first_r[m] = n.r;
+    }
   }
   __syncthreads();
   // ---- X = G / (|G| + eps), up to the factor r ----
   if (p.along_l) {
     const int per = 32 / lpr, sub = lane / lpr, u0 = lane % lpr;
-    for (int r = warp * per + sub; r < rows; r += 8 * per) {
-      const int m = r / p.side;
-      const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
-      const double f = factor[m];
-      if (f == 0.0) continue;
-#pragma unroll 2
+    for (int r0 = warp * per + sub; r0 < rows; r0 += NW * per * kRowsInFlight) {
       for (int u = u0; u < units; u += lpr) {
-        float v[8];
-        load_unit8<T>(row, p.sl, u * 8, p.L, p.vec_in, v);
+        float v[kRowsInFlight][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)((double)v[e] * f);
-        store_unit<PLANES>(X, x_plane, unit_off(r, u), v);
+        for (int k = 0; k < kRowsInFlight; ++k) {
+          const int r = r0 + k * NW * per, m = r / p.side;
+          load_unit8<T>(G + m * p.bs + (r - m * p.side) * p.sr, p.sl, u * 8, r < rows ? p.L : 0, p.vec_in, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsInFlight; ++k) {
+          const int r = r0 + k * NW * per;
+          const float2 f = r < rows ? factor[r / p.side] : make_float2(0.f, 0.f);
+          if (f.x == 0.f) continue;  // no such row, or a broken matrix
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * f.x * f.y;
+          store_unit<PLANES>(X, x_plane, unit_off(r, u), v[k]);
+        }
       }
     }
   } else {
     const int r = tid & 127, m = r / p.side;
-    const double f = r < rows ? factor[m] : 0.0;
-    if (f != 0.0) {
+    const float2 f = r < rows ? factor[m] : make_float2(0.f, 0.f);
+    if (f.x != 0.f) {
       const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
-      for (int u = tid >> 7; u < units; u += 2) {
+      for (int u = tid >> 7; u < units; u += NG) {
         float v[8];
         load_unit8<T>(row, p.sl, u * 8, p.L, 0, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)((double)v[e] * f);
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * f.x * f.y;
         store_unit<PLANES>(X, x_plane, unit_off(r, u), v);
       }
     }
@@ -219,17 +245,17 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
   };
 
   // this lane's row, its matrix and where that matrix lies among the columns of S
-  const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+  const int quad = warp & 3, group = warp >> 2, row = quad * 32 + lane;
   const int mine = row / p.side, lo = mine * p.side, hi = mine < p.g ? lo + p.side : lo;
   const int first = quad * 32 / p.side * p.side, last = min((quad * 32 + 31) / p.side * p.side + p.side, p.kk);
   const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
 
-  const float r0 = row < rows && factor[mine] != 0.0 ? first_r[mine] : 1.f;
+  const float r0 = row < rows && factor[mine].x != 0.f ? first_r[mine] : 1.f;
   // with one plane, S and P are held without their diagonals, which stay in float32 (see polar.cu)
   constexpr bool kSplitDiag = PLANES == 1;
   for (int t = 0; t < p.steps; ++t) {
     const CtaStep k = p.step[t];
-    const float f1 = t ? 1.f : r0, f2 = f1 * f1;
+    const float f1 = t ? 1.f : r0, f2 = f1 * f1, k3 = k.k3 * f2, kp = k.kp * f2;
     // ---- S = X X^T ----
     if (tid == 0) {
       for (int s = 0; s < SEGS; ++s)
@@ -240,20 +266,21 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
                    block_desc(xa + seg_q[s] * x_plane + b * kBlockBytes + q * 32, 0), idesc_s, s + b + q > 0);
       commit<1>(done);
     }
+    __syncwarp();  // the issuing lane first: a warp that sleeps on the barrier sleeps as a whole
     wait();
     for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
-      if (((c0 >> 5) & 1) != half) continue;
+      if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
       float v[32];
       tmem_row32(lanes + c0, v);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float w[8];
+        const float f = k.k1 * f2;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int c = c0 + u * 8 + e;
-          const float x = v[u * 8 + e] * f2;
-          if (kSplitDiag && c == row) sdiag[row] = x * kUnitS;
-          w[e] = c >= lo && c < hi && !(kSplitDiag && c == row) ? x * k.k1 : 0.f;
+          if (kSplitDiag && c == row) sdiag[row] = v[u * 8 + e] * f2 * kUnitS;
+          w[e] = (unsigned)(c - lo) < (unsigned)(hi - lo) && !(kSplitDiag && c == row) ? v[u * 8 + e] * f : 0.f;
         }
         if (c0 + u * 8 < p.kk) store_unit<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), w);
       }
@@ -264,18 +291,23 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
     fence_after();
     // ---- P = c S S + b S ----
     if (tid == 0) {
-      for (int s = 0; s < SEGS; ++s)
-        for (int q = 0; q < p.kk / 16; ++q) {
-          const int off = (q >> 2) * kBlockBytes + (q & 3) * 32;
-          mma<1>(tmem + 128, block_desc(sa + seg_p[s] * s_plane + off, 0), block_desc(sa + seg_q[s] * s_plane + off, 0),
-                 idesc_s, s + q > 0);
-        }
+      // a matrix's columns of S S take its own rows of S alone: the rest are zeros
+      const int width = p.blockwise ? p.side : p.kk;
+      const uint32_t idesc_p = mma_idesc(1, 0, 0, 128, width);
+      for (int c0 = 0; c0 < p.kk; c0 += width)
+        for (int s = 0; s < SEGS; ++s)
+          for (int c = c0; c < c0 + width; c += 16) {
+            const int off = (c >> 6) * kBlockBytes + (c & 63) * 2;
+            mma<1>(tmem + 128 + c0, block_desc(sa + seg_p[s] * s_plane + off, 0),
+                   block_desc(sa + seg_q[s] * s_plane + off + c0 * 128, 0), idesc_p, s + (c - c0) > 0);
+          }
       commit<1>(done);
     }
+    __syncwarp();  // the issuing lane first: a warp that sleeps on the barrier sleeps as a whole
     wait();
     const float di = kSplitDiag && row < p.kk ? sdiag[row] : 0.f;
     for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
-      if (((c0 >> 5) & 1) != half) continue;
+      if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
       float v[32], w[32];
       tmem_row32(lanes + c0, v);
       tmem_row32(lanes + 128 + c0, w);
@@ -285,13 +317,14 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int c = c0 + u * 8 + e;
-          const float o = v[u * 8 + e] * f2, oo = w[u * 8 + e] * k.k2;
+          const bool in = (unsigned)(c - lo) < (unsigned)(hi - lo);
+          const float o = v[u * 8 + e], oo = w[u * 8 + e] * k.k2;
           if constexpr (kSplitDiag) {
-            const float b = fmaf(k.c, di + sdiag[c], k.b) * k.kp;
-            x[e] = c >= lo && c < hi && c != row ? fmaf(o, b, oo) : 0.f;
+            const float b = fmaf(k.c, di + sdiag[c], k.b) * kp;
+            x[e] = in && c != row ? fmaf(o, b, oo) : 0.f;
             if (c == row) pdiag[row] = fmaf(oo, k.k4, di * fmaf(k.c, di, k.b));
           } else {
-            x[e] = c >= lo && c < hi ? fmaf(o, k.k3, oo) : 0.f;
+            x[e] = in ? fmaf(o, k3, oo) : 0.f;
           }
         }
         if (c0 + u * 8 < p.kk) store_unit<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), x);
@@ -313,8 +346,9 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
                    block_desc(xa + seg_q[s] * x_plane + b0 * kBlockBytes + q * 2048, 1), idesc_x, s + q > 0);
         commit<1>(done);
       }
+      __syncwarp();
       wait();
-      for (int c0 = half * 32; c0 < nb * 64; c0 += 64) {
+      for (int c0 = group * 32; c0 < nb * 64; c0 += NG * 32) {
         float v[32];
         tmem_row32(lanes + c0, v);
         const int c = b0 * 64 + c0;
@@ -342,7 +376,7 @@ __global__ void __launch_bounds__(kThreadsC, 2) polar_cta_kernel(const __grid_co
         }
         if (t == p.steps - 1 && row < rows) {
           const float nan = __int_as_float(0x7fffffff);
-          const float f = factor[mine] == 0.0 || *gu ? nan : 1.f / kPolarScale;
+          const float f = factor[mine].x == 0.f || *gu ? nan : 1.f / kPolarScale;
           T* o = static_cast<T*>(p.out) + (m0 + mine) * p.obs + (row - lo) * p.orr + c * p.ol;
           constexpr int PER = 16 / sizeof(T);
           if (p.vec_out && c + 32 <= p.L) {
@@ -382,15 +416,23 @@ bool inject_timeout() {
   return t && strcmp(t, "1") == 0;
 }
 
-template <typename T, int PLANES>
-cudaError_t launch_c(const CtaParams& p, size_t smem, unsigned grid, cudaStream_t s) {
-  auto kern = polar_cta_kernel<T, PLANES>;
+template <typename T, int PLANES, int NT>
+cudaError_t launch_n(const CtaParams& p, size_t smem, unsigned grid, cudaStream_t s) {
+  auto kern = polar_cta_kernel<T, PLANES, NT>;
   static int cache[64];
   int occ = 0;
-  const cudaError_t e = kernel_occupancy(kern, kThreadsC, smem, cache, &occ);
+  const cudaError_t e = kernel_occupancy(kern, NT, smem, cache, &occ);
   if (e != cudaSuccess) return e;
-  kern<<<grid, kThreadsC, smem, s>>>(p);
+  kern<<<grid, NT, smem, s>>>(p);
   return cudaGetLastError();
+}
+
+// 16 warps where one CTA has an SM to itself, by its shared memory or because
+// there are no more CTAs than SMs; otherwise two CTAs of 8.
+template <typename T, int PLANES>
+cudaError_t launch_c(const CtaParams& p, size_t smem, unsigned grid, int sms, cudaStream_t s) {
+  if (smem > 113 * 1024 || grid <= (unsigned)sms) return launch_n<T, PLANES, 512>(p, smem, grid, s);
+  return launch_n<T, PLANES, 256>(p, smem, grid, s);
 }
 
 int64_t smem_of(int planes, int64_t xblocks, int64_t sblocks) { return 1024 + planes * (xblocks + sblocks) * kBlockBytes; }
@@ -429,6 +471,7 @@ cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
   p.g = (int)g;
   p.kk = (p.g * p.side + 15) / 16 * 16;
   p.sblocks = (p.kk + 63) / 64;
+  p.blockwise = p.side % 16 == 0;
   p.along_l = p.sl <= p.sr || p.side == 1;
   p.steps = in.steps;
   p.eps = in.eps;
@@ -453,10 +496,11 @@ cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
   if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const unsigned grid = (unsigned)ctas;
   switch (in.dtype) {
-    case B2C_F32: return launch_c<float, 2>(p, smem, grid, s);
+    case B2C_F32: return launch_c<float, 2>(p, smem, grid, sms, s);
     case B2C_BF16:
-      return planes == 2 ? launch_c<__nv_bfloat16, 2>(p, smem, grid, s) : launch_c<__nv_bfloat16, 1>(p, smem, grid, s);
-    default: return launch_c<__half, 2>(p, smem, grid, s);
+      return planes == 2 ? launch_c<__nv_bfloat16, 2>(p, smem, grid, sms, s)
+                         : launch_c<__nv_bfloat16, 1>(p, smem, grid, sms, s);
+    default: return launch_c<__half, 2>(p, smem, grid, sms, s);
   }
 }
 
