@@ -146,6 +146,16 @@ __device__ __forceinline__ void epilogue_store(const GemmEpilogue& e, int64_t b,
 // Launchers. gemm_simt.cu
 cudaError_t launch_gemm_simt(const GemmProblem& g, cudaStream_t s);
 
+// gemm_skinny.cu: g.J columns in passes of up to 8
+cudaError_t launch_gemm_skinny(const GemmProblem& g, int sms, cudaStream_t s);
+
+// SM count of the current device.
+inline cudaError_t device_sms(int* sms) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  return e == cudaSuccess ? cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) : e;
+}
+
 // dP = dY act'(pre) (rounded to the type once), and the column sums of the
 // unrounded dP. gemm_dact.cu
 struct DactParams {

@@ -12,6 +12,7 @@ using namespace b2c;
 
 constexpr int64_t kMaxDim = (int64_t)1 << 30;
 constexpr int64_t kMaxPolarDim = (int64_t)1 << 20;
+constexpr double kSkinny16 = 2097152.0;  // largest 16-bit P of the FP32-unit form
 constexpr int kMaxSteps = 64;
 constexpr double kMaxSigma = 3.5;
 
@@ -46,9 +47,9 @@ GemmProblem problem(int dtype, const b2c_matrix* A, const b2c_matrix* B, int64_t
 // Which kernel takes a product, and what has to be copied for it.
 struct GemmChoice {
   GemmProblem g;
-  bool tc;
+  enum { kSimt, kSkinny, kTc } tier;
   PackPlan pack_p, pack_q;
-  size_t ws() const { return tc ? (size_t)(pack_p.bytes + pack_q.bytes) : 0; }
+  size_t ws() const { return tier == kTc ? (size_t)(pack_p.bytes + pack_q.bytes) : 0; }
 };
 
 GemmChoice choose(const GemmProblem& in) {
@@ -64,8 +65,14 @@ GemmChoice choose(const GemmProblem& in) {
     }
     g.e.bias_on_i = !in.e.bias_on_i;
   }
-  c.tc = in.K >= 32 && (double)in.I * (double)in.J * (double)in.K * (double)in.batch > 1048576.0;
-  if (c.tc) {
+  const bool small = (double)c.g.I * (double)in.K * (double)in.batch <= kSkinny16;
+  if (in.K > 0 && (in.dtype == B2C_F32 ? c.g.J <= 16 : c.g.J <= 8 && small)) {
+    c.tier = GemmChoice::kSkinny;
+    return c;
+  }
+  const bool tc = in.K >= 32 && (double)in.I * (double)in.J * (double)in.K * (double)in.batch > 1048576.0;
+  c.tier = tc ? GemmChoice::kTc : GemmChoice::kSimt;
+  if (tc) {
     c.pack_p = plan_pack(in.dtype, c.g.P, in.batch, c.g.I, in.K);
     c.pack_q = plan_pack(in.dtype, c.g.Q, in.batch, c.g.J, in.K);
   }
@@ -74,9 +81,13 @@ GemmChoice choose(const GemmProblem& in) {
 
 cudaError_t launch_gemm(const GemmChoice& c, void* ws, cudaStream_t s) {
   const GemmProblem& g = c.g;
-  if (!c.tc) return launch_gemm_simt(g, s);
-  TcProblem t{};
   cudaError_t e;
+  if (c.tier == GemmChoice::kSimt) return launch_gemm_simt(g, s);
+  if (c.tier == GemmChoice::kSkinny) {
+    int sms = 0;
+    return (e = device_sms(&sms)) == cudaSuccess ? launch_gemm_skinny(g, sms, s) : e;
+  }
+  TcProblem t{};
   char* w = static_cast<char*>(ws);
   if (!c.pack_p.needed) tc_direct(g.P, g.batch, g.I, g.K, &t.P);
   else if ((e = launch_pack(g.dtype, g.P, c.pack_p, w, &t.P, s)) != cudaSuccess) return e;

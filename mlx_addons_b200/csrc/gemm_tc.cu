@@ -4,14 +4,16 @@
 //
 // A pair of CTAs (two SMs) computes a 256 x 256 tile (cta_group::2): each CTA
 // holds 128 rows of P and 128 of Q's 256 in shared memory and 128 x 256 of D
-// in its tensor memory. Where D has fewer rows or columns than that pays for,
-// single CTAs compute 128 x BN tiles. Both forms are persistent: the grid is
-// one CTA per SM, tiles are dealt in order.
+// in its tensor memory. The pairs are persistent, one CTA an SM, and tensor
+// memory holds two accumulators, so the epilogue of a tile runs under the MMAs
+// of the next. Where D is too small for that, single CTAs compute 128 x BN
+// tiles, several to an SM, and k may be split over a cluster of up to 8 of
+// them, whose partial sums are joined in order through distributed shared
+// memory.
 //
 // Roles in a CTA: one thread issues the TMA loads (a ring of 64-deep slices),
-// one thread of the leading CTA issues the MMAs, eight warps take finished
-// accumulators from tensor memory through the epilogue. Tensor memory holds
-// two accumulators, so the epilogue of a tile runs under the MMAs of the next.
+// one thread (of the leading CTA) issues the MMAs, four or eight warps take
+// finished accumulators from tensor memory through the epilogue.
 //
 // Both axis orders of an operand are read as they lie: with unit stride along
 // k ("K-major") and along the rows ("MN-major"), both with 128-byte swizzle.
@@ -20,8 +22,10 @@
 // known, two f16 planes; the product is then the sum of the plane pairs whose
 // weight is 2^-24 or more (6 of 9, or 3 of 4), smallest first. The tensor
 // cores truncate when they add to an accumulator, so such a product's
-// accumulator is joined in float32 registers every kChunk values of k
-// (JOIN): without that the truncations, all towards zero, add up along k.
+// accumulator is joined in float32 registers after every slice (JOIN):
+// without that the truncations, all towards zero, add up along k. A slice in
+// shared memory holds all planes, each loaded once for all its products.
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <type_traits>
@@ -38,21 +42,19 @@ namespace {
 
 constexpr int BM = 128;          // rows of D per CTA
 constexpr int BK = 64;           // depth of a slice: 128 bytes
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 8;      // of a pair's CTA
 constexpr int kThreads = (kEpiWarps + 4) * 32;  // the last warpgroup: loads, products, two idle warps
 // Registers: 384 x 168 at launch = 128 x 72 + 256 x 216 after the split.
 constexpr int kRegsFew = 72, kRegsMany = 216;
 constexpr int kMaxStages = 8;
-constexpr int kChunk = 2;        // slices of k per joined accumulator
-constexpr int kMaxSeg = 6;
+constexpr int kABytes = BM * BK * 2;  // one plane of P's rows in a slice
 constexpr int kSmemMax = 232448;
 
 struct TcParams {
   int64_t I, J, tiles;
   int tiles_i, tiles_j, band;
-  int kblocks, nseg, chunk;
-  int seg_p[kMaxSeg], seg_q[kMaxSeg];
-  int BN, share, stages, a_bytes, b_bytes;
+  int kblocks;
+  int BN, share, split, stages, b_bytes, stage_bytes, tmem_cols;
   int p_inner, q_inner, p_bcast, q_bcast, sym;
   uint32_t idesc;
   GemmEpilogue e;
@@ -322,24 +324,107 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t t) {
 
 __device__ __forceinline__ int clamp32(int64_t n) { return n > 32 ? 32 : (int)n; }
 
-template <int CG, bool JOIN, typename OUT>
+// After a wait that ran out: copies and MMAs still in flight end within microseconds.
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = now_ns();
+  while (now_ns() - t0 < 20000000ull) {
+  }
+}
+
+// The plane pairs of a product, smallest first.
+template <int PLANES>
+struct Segs;
+template <>
+struct Segs<1> {
+  static constexpr int N = 1;
+  static __host__ __device__ constexpr int p(int) { return 0; }
+  static __host__ __device__ constexpr int q(int) { return 0; }
+};
+template <>
+struct Segs<2> {  // lo hi, hi lo, hi hi
+  static constexpr int N = 3;
+  static __host__ __device__ constexpr int p(int g) { return g == 0; }
+  static __host__ __device__ constexpr int q(int g) { return g == 1; }
+};
+template <>
+struct Segs<3> {  // lo hi, mid mid, hi lo, mid hi, hi mid, hi hi
+  static constexpr int N = 6;
+  static __host__ __device__ constexpr int p(int g) { return g == 0 ? 2 : g == 1 || g == 3 ? 1 : 0; }
+  static __host__ __device__ constexpr int q(int g) { return g == 2 ? 2 : g == 1 || g == 4 ? 1 : 0; }
+};
+
+// One slice: every plane of this CTA's rows of P, then of Q.
+template <int CG, int PLANES>
+__device__ __forceinline__ void load_slice(const TcParams& p, const CUtensorMap* map_p, const CUtensorMap* map_q, uint32_t at,
+                                           int i0, int j0, int kb, int bp, int bq, uint32_t bar) {
+#pragma unroll
+  for (int g = 0; g < PLANES; ++g, at += kABytes) {
+    if (p.p_inner) {
+      tma_load<CG>(at, map_p, i0, kb * BK, bp, g, bar);
+      tma_load<CG>(at + 8192, map_p, i0 + 64, kb * BK, bp, g, bar);
+    } else {
+      tma_load<CG>(at, map_p, kb * BK, i0, bp, g, bar);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < PLANES; ++g, at += p.b_bytes) {
+    if (p.q_inner) {
+      for (int h = 0; h < p.b_bytes / 8192; ++h) tma_load<CG>(at + h * 8192, map_q, j0 + 64 * h, kb * BK, bq, g, bar);
+    } else {
+      tma_load<CG>(at, map_q, kb * BK, j0, bq, g, bar);
+    }
+  }
+}
+
+// What the issuing thread needs of every slice: descriptors of stage 0 and the
+// steps to the next 16 values of k, kept in registers (the thread must not be
+// slower than 4 MMAs of 32 clocks).
+template <int CG, int PLANES>
+struct Multiplier {
+  uint64_t dp, dq;
+  uint32_t step_p, step_q, plane_q, stage, idesc;
+  __device__ __forceinline__ Multiplier(const TcParams& p, uint32_t ring) {
+    dp = tile_desc(ring, p.p_inner);
+    dq = tile_desc(ring + PLANES * kABytes, p.q_inner);
+    step_p = p.p_inner ? 2048 >> 4 : 32 >> 4;
+    step_q = p.q_inner ? 2048 >> 4 : 32 >> 4;
+    plane_q = p.b_bytes >> 4;
+    stage = p.stage_bytes >> 4;
+    idesc = p.idesc;
+  }
+  // The products of stage s into the accumulator at d; fresh: its first ones.
+  __device__ __forceinline__ void slice(uint32_t s, uint32_t d, bool fresh) const {
+    typedef Segs<PLANES> S;
+#pragma unroll
+    for (int g = 0; g < S::N; ++g) {
+      const uint64_t a = dp + s * stage + S::p(g) * (kABytes >> 4), q = dq + s * stage + S::q(g) * plane_q;
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk) mma<CG>(d, a + kk * step_p, q + kk * step_q, idesc, g || kk ? 1u : !fresh);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// pairs of CTAs
+// ---------------------------------------------------------------------------
+
+template <int PLANES, typename OUT>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemm_tc_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
-                   const __grid_constant__ TcParams p) {
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                     const __grid_constant__ TcParams p) {
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   typedef typename OutOf<OUT>::T T;
+  constexpr bool JOIN = PLANES > 1;
   constexpr int kStage = 32 * (32 * sizeof(T) + 16);  // one warp's staging rows
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const uint32_t rank = cluster_rank();
   unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
-  const int stage_bytes = p.a_bytes + p.b_bytes;
-  unsigned char* staging = ring + p.stages * stage_bytes;
+  unsigned char* staging = ring + p.stages * p.stage_bytes;
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, tfull0 = empty0 + 8 * kMaxStages,
-                 tempty0 = tfull0 + 16;
-  const uint32_t never = tempty0 + 16;
+                 tempty0 = tfull0 + 16, never = tempty0 + 16;
   const uint64_t limit = p.inject ? 1000000ull : kWaitNs;
 
   if (tid == 0) {
@@ -351,32 +436,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(never, 1);
     for (int s = 0; s < 2; ++s) {
       bar_init(tfull0 + 8 * s, 1);
-      bar_init(tempty0 + 8 * s, kEpiWarps * CG);
+      bar_init(tempty0 + 8 * s, kEpiWarps * 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kEpiWarps) {
-    if constexpr (CG == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     fence_before();
   }
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  cluster_sync();
   fence_after();
   const uint32_t tmem = tmem_slot;
-  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
   volatile int* gu = &gave_up;
+  const int per = JOIN ? 1 : p.kblocks;  // slices of one accumulator
 
   if (warp < kEpiWarps) {
     if constexpr (JOIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     // ---- epilogue: warps w and w + 4 share the rows 32 (w % 4).., and take every other 32 columns ----
     const int quad = warp & 3, half = warp >> 2;
-    const uint32_t lead_tempty0 = CG == 2 ? map_rank(tempty0, 0) : tempty0;
+    const uint32_t lead_tempty0 = map_rank(tempty0, 0);
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     unsigned char* stage = staging + warp * kStage;
     uint32_t buf = 0, tphase = 0;
@@ -384,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float bad = __int_as_float(0x7fffffff);
     if (p.inject && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, limit, &g_gemm_fault));
     for (int64_t t = first; t < p.tiles; t += step) {
-      const Tile o = tile_at<CG>(p, t);
+      const Tile o = tile_at<2>(p, t);
       const int64_t i = o.i + rank * BM + quad * 32;
       const int rows = clamp32(p.I - i);
       if constexpr (JOIN) {
@@ -393,18 +474,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[q][c] = 0.f;
-        for (int c0 = 0; c0 < p.kblocks; c0 += p.chunk) {
+        for (int kb = 0; kb < p.kblocks; ++kb) {
           ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
           fence_after();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int col = (2 * q + half) * 32;
-            if (col < p.BN) {
-              float v[32];
-              tmem_row32(lanes + buf * 256 + col, v);
+            float v[32];
+            tmem_row32(lanes + buf * 256 + (2 * q + half) * 32, v);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) acc[q][c] += v[c];
-            }
+            for (int c = 0; c < 32; ++c) acc[q][c] += v[c];
           }
           fence_before();
           __syncwarp();
@@ -414,21 +492,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int col = (2 * q + half) * 32;
-          if (col < p.BN) {
-            if (!ok) {
+          if (!ok) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c) acc[q][c] = bad;
-            }
-            epilogue32<OUT>(acc[q], p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
+            for (int c = 0; c < 32; ++c) acc[q][c] = bad;
           }
+          epilogue32<OUT>(acc[q], p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
         }
       } else {
         ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
         fence_after();
-        for (int col = half * 32; col < p.BN; col += 64) {
+        for (int col = half * 32; col < 256; col += 64) {
           float v[32];
           tmem_row32(lanes + buf * 256 + col, v);
-          if (col + 64 >= p.BN) {  // the last of this warp's columns: the accumulator is free
+          if (col + 64 >= 256) {  // the last of this warp's columns: the accumulator is free
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive_cluster(lead_tempty0 + 8 * buf);
@@ -439,7 +515,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           epilogue32<OUT>(v, p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
         }
-        if (half * 32 >= p.BN && lane == 0) bar_arrive_cluster(lead_tempty0 + 8 * buf);
         if (++buf == 2) buf = 0, tphase ^= 1;
       }
     }
@@ -447,78 +522,233 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
     if (warp == kEpiWarps && lane == 0) {
       // ---- loads ----
-      const uint32_t lead_full0 = CG == 2 ? map_rank(full0, 0) : full0;
+      const uint32_t lead_full0 = map_rank(full0, 0);
       uint32_t s = 0, phase = 0;
       for (int64_t t = first; t < p.tiles && !*gu; t += step) {
-        const Tile o = tile_at<CG>(p, t);
+        const Tile o = tile_at<2>(p, t);
         const int i0 = (int)(o.i + rank * BM), j0 = (int)(o.j + rank * p.share);
         const int bp = p.p_bcast ? 0 : (int)o.b, bq = p.q_bcast ? 0 : (int)o.b;
-        for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
-          const int c1 = min(c0 + p.chunk, p.kblocks);
-          for (int g = 0; g < p.nseg; ++g) {
-            for (int kb = c0; kb < c1; ++kb) {
-              if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_gemm_fault)) break;
-              if (rank == 0) bar_expect(full0 + 8 * s, CG * stage_bytes);
-              const uint32_t bar = lead_full0 + 8 * s, a = smem_u32(ring + s * stage_bytes), q = a + p.a_bytes;
-              if (p.p_inner) {
-                tma_load<CG>(a, &map_p, i0, kb * BK, bp, p.seg_p[g], bar);
-                tma_load<CG>(a + 8192, &map_p, i0 + 64, kb * BK, bp, p.seg_p[g], bar);
-              } else {
-                tma_load<CG>(a, &map_p, kb * BK, i0, bp, p.seg_p[g], bar);
-              }
-              if (p.q_inner) {
-                for (int h = 0; h < p.b_bytes / 8192; ++h)
-                  tma_load<CG>(q + h * 8192, &map_q, j0 + 64 * h, kb * BK, bq, p.seg_q[g], bar);
-              } else {
-                tma_load<CG>(q, &map_q, kb * BK, j0, bq, p.seg_q[g], bar);
-              }
-              if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
-            }
-          }
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_gemm_fault)) break;
+          if (rank == 0) bar_expect(full0 + 8 * s, 2 * p.stage_bytes);
+          load_slice<2, PLANES>(p, &map_p, &map_q, smem_u32(ring + s * p.stage_bytes), i0, j0, kb, bp, bq, lead_full0 + 8 * s);
+          if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
         }
       }
     } else if (warp == kEpiWarps + 1 && rank == 0 && lane == 0) {
       // ---- products ----
+      const Multiplier<2, PLANES> mul(p, smem_u32(ring));
       uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
-      const uint32_t step_p = p.p_inner ? 2048 >> 4 : 32 >> 4, step_q = p.q_inner ? 2048 >> 4 : 32 >> 4;
       for (int64_t t = first; t < p.tiles && !*gu; t += step) {
-        for (int c0 = 0; c0 < p.kblocks && !*gu; c0 += p.chunk) {
-          const int n = (min(c0 + p.chunk, p.kblocks) - c0) * p.nseg;
+        for (int k0 = 0; k0 < p.kblocks; k0 += per) {
           if (!bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
           fence_after();
-          const uint32_t d = tmem + buf * 256;
-          for (int it = 0; it < n; ++it) {
+          for (int kb = 0; kb < per; ++kb) {
             if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
             fence_after();
-            const uint32_t a = smem_u32(ring + s * stage_bytes);
-            const uint64_t da = tile_desc(a, p.p_inner), dq = tile_desc(a + p.a_bytes, p.q_inner);
-  #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk)
-              mma<CG>(d, da + kk * step_p, dq + kk * step_q, p.idesc, it > 0 || kk > 0);
-            commit<CG>(empty0 + 8 * s);
+            mul.slice(s, tmem + buf * 256, kb == 0);
+            commit<2>(empty0 + 8 * s);
             if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
           }
           if (*gu) break;
-          commit<CG>(tfull0 + 8 * buf);
+          commit<2>(tfull0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
       }
     }
   }
   __syncthreads();
-  if (gave_up) {
-    // copies and MMAs of this CTA that are still in flight end within microseconds
-    const uint64_t t0 = now_ns();
-    while (now_ns() - t0 < 20000000ull) {
-    }
-  }
+  if (gave_up) settle();
   fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();
+  cluster_sync();
   if (warp == kEpiWarps) {
     fence_after();
-    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// single CTAs, one tile each, k split over a cluster
+// ---------------------------------------------------------------------------
+
+// JOIN: one CTA an SM with eight epilogue warps, so that a slice's planes fit
+// twice; otherwise two CTAs with four.
+template <int PLANES>
+struct Solo {
+  static constexpr bool JOIN = PLANES > 1;
+  static constexpr int EPI = JOIN ? 8 : 4;
+  static constexpr int NT = (EPI + 2) * 32;
+  static constexpr int CTAS = JOIN ? 1 : 2;
+  static constexpr int SMEM = JOIN ? kSmemMax - 1024 : 113 * 1024;
+};
+
+template <int PLANES, typename OUT>
+__global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
+    gemm_solo_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                     const __grid_constant__ TcParams p) {
+  extern __shared__ unsigned char raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up;
+  typedef typename OutOf<OUT>::T T;
+  constexpr bool JOIN = PLANES > 1;
+  constexpr int EPI = Solo<PLANES>::EPI, GROUPS = EPI / 4, SLICES = JOIN ? 4 / GROUPS : 1;
+  constexpr int kStage = 32 * (32 * sizeof(T) + 16);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = p.split, rank = split > 1 ? (int)cluster_rank() : 0;
+  unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, tfull0 = empty0 + 8 * kMaxStages,
+                 tempty0 = tfull0 + 16, never = tempty0 + 16;
+  const uint64_t limit = p.inject ? 1000000ull : kWaitNs;
+  const Tile o = tile_at<1>(p, blockIdx.x / split);
+  // this CTA's slices of k
+  const int kb0 = (int)((int64_t)p.kblocks * rank / split), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / split);
+
+  if (tid == 0) {
+    gave_up = 0;
+    for (int s = 0; s < p.stages; ++s) {
+      bar_init(full0 + 8 * s, 1);
+      bar_init(empty0 + 8 * s, 1);
+    }
+    bar_init(never, 1);
+    for (int s = 0; s < 2; ++s) {
+      bar_init(tfull0 + 8 * s, 1);
+      bar_init(tempty0 + 8 * s, EPI);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == EPI) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(p.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  volatile int* gu = &gave_up;
+  const int quad = warp & 3, group = warp >> 2;
+  const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+  const int64_t i = o.i + quad * 32;
+  const int rows = clamp32(p.I - i), pitch = p.BN + 4;
+  float* partial = reinterpret_cast<float*>(ring);
+  unsigned char* stage = ring + (split > 1 ? BM * pitch * 4 : 0) + warp * kStage;
+
+  if (warp < EPI) {
+    bool ok = true;
+    if (p.inject && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, limit, &g_gemm_fault));
+    float acc[SLICES][32];
+    if constexpr (JOIN) {
+#pragma unroll
+      for (int q = 0; q < SLICES; ++q)
+#pragma unroll
+        for (int c = 0; c < 32; ++c) acc[q][c] = 0.f;
+      uint32_t buf = 0, tphase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
+        fence_after();
+#pragma unroll
+        for (int q = 0; q < SLICES; ++q) {
+          const int col = (GROUPS * q + group) * 32;
+          if (col < p.BN) {
+            float v[32];
+            tmem_row32(lanes + buf * p.BN + col, v);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) acc[q][c] += v[c];
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_cluster(tempty0 + 8 * buf);
+        if (++buf == 2) buf = 0, tphase ^= 1;
+      }
+    } else {
+      ok = __all_sync(kFull, ok && bar_wait(tfull0, 0, gu, limit, &g_gemm_fault));
+      fence_after();
+    }
+    // every product is done: the ring is free for partial sums and staging (after a wait that ran out, once what is
+    // still in flight has landed)
+    if (!ok) settle();
+#pragma unroll
+    for (int q = 0; q < (JOIN ? SLICES : 4); ++q) {
+      const int col = (GROUPS * q + group) * 32;
+      if (col < p.BN) {
+        float(&v)[32] = acc[JOIN ? q : 0];
+        if constexpr (!JOIN) tmem_row32(lanes + col, v);
+        if (!ok) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = __int_as_float(0x7fffffff);
+        }
+        if (split > 1) {
+          float4* at = reinterpret_cast<float4*>(partial + (quad * 32 + lane) * pitch + col);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) at[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        } else {
+          epilogue32<OUT>(v, p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
+        }
+      }
+    }
+  } else if (warp == EPI && lane == 0) {
+    // ---- loads ----
+    uint32_t s = 0, phase = 0;
+    const int bp = p.p_bcast ? 0 : (int)o.b, bq = p.q_bcast ? 0 : (int)o.b;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_gemm_fault)) break;
+      bar_expect(full0 + 8 * s, p.stage_bytes);
+      load_slice<1, PLANES>(p, &map_p, &map_q, smem_u32(ring + s * p.stage_bytes), (int)o.i, (int)o.j, kb, bp, bq, full0 + 8 * s);
+      if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
+    }
+  } else if (warp == EPI + 1 && lane == 0) {
+    // ---- products ----
+    const Multiplier<1, PLANES> mul(p, smem_u32(ring));
+    uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (JOIN && !bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
+      if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
+      fence_after();
+      mul.slice(s, tmem + buf * p.BN, JOIN || kb == kb0);
+      commit<1>(empty0 + 8 * s);
+      if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
+      if (JOIN || kb == kb1 - 1) commit<1>(tfull0 + 8 * buf);
+      if (JOIN && ++buf == 2) buf = 0, tphase ^= 1;
+    }
+  }
+  if (split > 1) {
+    __syncwarp();
+    cluster_sync();
+    // the tile's 32 x 32 pieces are dealt over the cluster's epilogue warps
+    if (warp < EPI) {
+      for (int u = rank * EPI + warp; u < 4 * (p.BN / 32); u += split * EPI) {
+        const int pq = u & 3, col = (u >> 2) * 32;
+        const uint32_t at = smem_u32(partial + (pq * 32 + lane) * pitch + col);
+        float v[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = 0.f;
+        for (int q = 0; q < split; ++q) {
+          const uint32_t peer = map_rank(at, q);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            float x, y, z, w;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x), "=f"(y), "=f"(z), "=f"(w) : "r"(peer + c * 4) : "memory");
+            v[c] += x, v[c + 1] += y, v[c + 2] += z, v[c + 3] += w;
+          }
+        }
+        const int64_t ii = o.i + pq * 32;
+        epilogue32<OUT>(v, p, o.b, ii, o.j + col, clamp32(p.I - ii), clamp32(p.J - o.j - col), o.mirror, stage, lane);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // peers' partial sums stay until they have been read
+  }
+  __syncthreads();
+  if (gave_up) settle();
+  fence_before();
+  __syncthreads();
+  if (warp == EPI) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols));
   }
 }
 
@@ -564,45 +794,117 @@ bool vec16(const void* p, int64_t elt, int64_t bs, int64_t is, int64_t js, int64
          plane * elt % 16 == 0;
 }
 
-template <int CG, bool JOIN, typename OUT>
-cudaError_t launch_t(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
-  typedef typename OutOf<OUT>::T T;
-  const int staging = kEpiWarps * 32 * (32 * (int)sizeof(T) + 16), stage = p.a_bytes + p.b_bytes;
-  int stages = (kSmemMax - 1024 - 512 - staging) / stage;
-  p.stages = stages > kMaxStages ? kMaxStages : stages;
-  const size_t smem = 1024 + (size_t)p.stages * stage + staging;
-  auto kern = gemm_tc_kernel<CG, JOIN, OUT>;
-  static int cache[64];
-  int occ = 0;
-  cudaError_t e = kernel_occupancy(kern, kThreads, smem, cache, &occ);
-  if (e != cudaSuccess) return e;
-  const int64_t want = p.tiles * CG, cap = sms / CG * CG;
+template <typename Kern>
+cudaError_t launch_in_clusters(Kern kern, int64_t ctas, int cluster, int threads, size_t smem, cudaStream_t s,
+                               const CUtensorMap& mp, const CUtensorMap& mq, const TcParams& p) {
+  if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(want < cap ? want : cap));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.x = cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, mp, mq, p);
 }
 
-template <int CG>
-cudaError_t launch_cg(const TcProblem& t, const CUtensorMap& mp, const CUtensorMap& mq, const TcParams& p, int sms,
-                      cudaStream_t s) {
+template <int PLANES, typename OUT>
+cudaError_t launch_pair(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
+  typedef typename OutOf<OUT>::T T;
+  const int staging = kEpiWarps * 32 * (32 * (int)sizeof(T) + 16);
+  const int stages = (kSmemMax - 1024 - 512 - staging) / p.stage_bytes;
+  p.stages = stages > kMaxStages ? kMaxStages : stages;
+  const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + staging;
+  auto kern = gemm_pair_kernel<PLANES, OUT>;
+  static int cache[64];
+  int occ = 0;
+  cudaError_t e = kernel_occupancy(kern, kThreads, smem, cache, &occ);
+  if (e != cudaSuccess) return e;
+  const int64_t want = p.tiles * 2, cap = sms / 2 * 2;
+  return launch_in_clusters(kern, want < cap ? want : cap, 2, kThreads, smem, s, mp, mq, p);
+}
+
+template <int PLANES, typename OUT>
+cudaError_t launch_solo(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int, cudaStream_t s) {
+  typedef typename OutOf<OUT>::T T;
+  constexpr int NT = Solo<PLANES>::NT;
+  const int staging = Solo<PLANES>::EPI * 32 * (32 * (int)sizeof(T) + 16) + (p.split > 1 ? BM * (p.BN + 4) * 4 : 0);
+  const int per = (p.kblocks + p.split - 1) / p.split;
+  int stages = (Solo<PLANES>::SMEM - 1024 - 512) / p.stage_bytes;
+  if (stages > kMaxStages) stages = kMaxStages;
+  p.stages = stages > per ? per : stages;
+  size_t smem = (size_t)p.stages * p.stage_bytes;
+  if (smem < (size_t)staging) smem = staging;
+  smem += 1024;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < (PLANES > 1 ? 2 : 1) * p.BN) p.tmem_cols *= 2;
+  auto kern = gemm_solo_kernel<PLANES, OUT>;
+  static int cache[64];
+  int occ = 0;
+  cudaError_t e = kernel_occupancy(kern, NT, smem, cache, &occ);
+  if (e != cudaSuccess) return e;
+  return launch_in_clusters(kern, p.tiles * p.split, p.split, NT, smem, s, mp, mq, p);
+}
+
+template <bool PAIR, int PLANES, typename OUT>
+cudaError_t launch_form(const CUtensorMap& mp, const CUtensorMap& mq, const TcParams& p, int sms, cudaStream_t s) {
+  if constexpr (PAIR) return launch_pair<PLANES, OUT>(mp, mq, p, sms, s);
+  else return launch_solo<PLANES, OUT>(mp, mq, p, sms, s);
+}
+
+template <bool PAIR>
+cudaError_t launch_out(const TcProblem& t, const CUtensorMap& mp, const CUtensorMap& mq, const TcParams& p, int sms,
+                       cudaStream_t s) {
   if (t.kind == kOne) {
-    if (t.out == B2C_BF16) return launch_t<CG, false, __nv_bfloat16>(mp, mq, p, sms, s);
-    if (t.out == B2C_F16) return launch_t<CG, false, __half>(mp, mq, p, sms, s);
+    if (t.out == B2C_BF16) return launch_form<PAIR, 1, __nv_bfloat16>(mp, mq, p, sms, s);
+    if (t.out == B2C_F16) return launch_form<PAIR, 1, __half>(mp, mq, p, sms, s);
     return cudaErrorInvalidValue;
   }
-  if (t.out == B2C_F32) return launch_t<CG, true, float>(mp, mq, p, sms, s);
-  if (t.out == B2C_F16) return launch_t<CG, true, __half>(mp, mq, p, sms, s);
-  if (t.out == kOutHalves) return launch_t<CG, true, Halves>(mp, mq, p, sms, s);
+  if (t.kind == kThirds && t.out == B2C_F32) return launch_form<PAIR, 3, float>(mp, mq, p, sms, s);
+  if (t.kind == kHalves && t.out == B2C_F32) return launch_form<PAIR, 2, float>(mp, mq, p, sms, s);
+  if (t.kind == kHalves && t.out == B2C_F16) return launch_form<PAIR, 2, __half>(mp, mq, p, sms, s);
+  if (t.kind == kHalves && t.out == kOutHalves) return launch_form<PAIR, 2, Halves>(mp, mq, p, sms, s);
   return cudaErrorInvalidValue;
+}
+
+// The form of a product: pairs, or single CTAs with BN columns and k split
+// over `split` of them.
+struct Form {
+  int pair, BN, split;
+  double clocks;
+};
+
+// Estimated clocks of an SM: its share of tiles times the longer of loading a
+// slice (about 40 bytes a clock and SM from L2) and multiplying it (128 x 16 x
+// 16 values a clock, and 128 bytes of shared memory a clock), plus what a
+// launch, a join over a cluster and an epilogue cost. Only the order of these
+// estimates matters: on 1000 x 777 x 1301 float32 the forms take 26 to 80 us, on
+// 16 x 4096 x 16384 f16 29 to 44 us, and the estimate's choice is the first.
+Form choose_form(const TcProblem& t, int kblocks, int planes, int nseg, int sms) {
+  Form best{0, 0, 0, 1e300};
+  const int64_t ti = (t.I + BM - 1) / BM;
+  for (int BN = t.sym ? 128 : 32; BN <= 128; BN *= 2) {
+    if (!t.sym && BN > 32 && BN / 2 >= t.J) break;
+    const int64_t tj = (t.J + BN - 1) / BN, tiles = t.batch * (t.sym ? ti * (ti + 1) / 2 : ti * tj);
+    for (int split = 1; split <= 8 && split <= kblocks; split *= 2) {
+      const double load = planes * (16384.0 + BN * 128.0) / 40, mul = nseg * 4.0 * fmax(BN / 2.0, (128 + BN) / 4.0);
+      const double slice = fmax(load, mul), ctas = ceil((double)tiles * split / sms);
+      const double c = ctas * ((kblocks + split - 1) / split * slice + BN * 12.0) + 3000 + (split > 1 ? 1500 : 0);
+      if (c < best.clocks) best = Form{0, BN, split, c};
+    }
+  }
+  if (t.I > BM && t.J > 128) {
+    const int64_t ti2 = (t.I + 255) / 256, tj2 = (t.J + 255) / 256;
+    const int64_t tiles = t.batch * (t.sym ? ti2 * (ti2 + 1) / 2 : ti2 * tj2);
+    const double slice = fmax(planes * 32768.0 / 40, nseg * 4.0 * 128);
+    const double c = ceil(2.0 * tiles / sms) * kblocks * slice + 4000 + 3000;
+    if (c < best.clocks) best = Form{1, 256, 1, c};
+  }
+  return best;
 }
 
 bool inject_timeout() {
@@ -636,36 +938,18 @@ bool tc_direct(const GemmOperand& o, int64_t batch, int64_t rows, int64_t K, TcO
 }
 
 cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int sms = 0;
+  const cudaError_t e = device_sms(&sms);
   if (e != cudaSuccess) return e;
   TcParams p{};
   p.I = t.I;
   p.J = t.J;
   p.kblocks = (int)((t.K + BK - 1) / BK);
   const int planes = t.kind == kOne ? 1 : t.kind == kHalves ? 2 : 3;
-  static const int seg2[3][2] = {{1, 0}, {0, 1}, {0, 0}};
-  static const int seg3[6][2] = {{2, 0}, {1, 1}, {0, 2}, {1, 0}, {0, 1}, {0, 0}};
-  p.nseg = t.kind == kOne ? 1 : t.kind == kHalves ? 3 : 6;
-  for (int g = 0; g < p.nseg; ++g) {
-    p.seg_p[g] = t.kind == kOne ? 0 : t.kind == kHalves ? seg2[g][0] : seg3[g][0];
-    p.seg_q[g] = t.kind == kOne ? 0 : t.kind == kHalves ? seg2[g][1] : seg3[g][1];
-  }
-  p.chunk = t.kind == kOne ? p.kblocks : kChunk;
-  // a pair's 256 x 256 tile where there is at least half a wave of them
-  const int64_t big = ((t.I + 255) / 256) * ((t.J + 255) / 256) * t.batch;
-  const bool pair = t.I > 128 && t.J > 128 && big * 4 >= sms;
-  const int CG = pair ? 2 : 1;
-  if (pair) {
-    p.BN = 256;
-  } else if (t.sym) {
-    p.BN = 128;
-  } else {
-    const int64_t ti = (t.I + 127) / 128;
-    p.BN = 256;
-    while (p.BN > 32 && (p.BN / 2 >= t.J || ti * ((t.J + p.BN - 1) / p.BN) * t.batch < sms)) p.BN /= 2;
-  }
+  const Form f = choose_form(t, p.kblocks, planes, planes == 1 ? 1 : planes == 2 ? 3 : 6, sms);
+  const int CG = f.pair ? 2 : 1;
+  p.BN = f.BN;
+  p.split = f.split;
   p.share = p.BN / CG;
   p.tiles_i = (int)((t.I + BM * CG - 1) / (BM * CG));
   p.tiles_j = (int)((t.J + p.BN - 1) / p.BN);
@@ -676,8 +960,8 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   p.p_bcast = t.P.bcast;
   p.q_bcast = t.Q.bcast;
   p.sym = t.sym;
-  p.a_bytes = BM * BK * 2;
   p.b_bytes = (p.q_inner ? (p.share + 63) / 64 * 64 : p.share) * BK * 2;
+  p.stage_bytes = planes * (kABytes + p.b_bytes);
   p.idesc = mma_idesc(t.f16, p.p_inner, p.q_inner, BM * CG, p.BN);
   p.e = t.e;
   p.polar = t.polar;
@@ -693,7 +977,7 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   if (!encode(&mp, t.P, t.f16, planes, t.batch, t.I, t.K, BM) ||
       !encode(&mq, t.Q, t.f16, planes, t.batch, t.J, t.K, p.share))
     return cudaErrorInvalidValue;
-  return pair ? launch_cg<2>(t, mp, mq, p, sms, s) : launch_cg<1>(t, mp, mq, p, sms, s);
+  return f.pair ? launch_out<true>(t, mp, mq, p, sms, s) : launch_out<false>(t, mp, mq, p, sms, s);
 }
 
 cudaError_t gemm_take_fault(unsigned int* fault) {

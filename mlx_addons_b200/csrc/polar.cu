@@ -293,9 +293,8 @@ size_t polar_ws_bytes(const PolarParams& in) {
 cudaError_t launch_polar(const PolarParams& in, cudaStream_t s) {
   const PolarParams p = along_rows(in);
   if (polar_cta_fits(p)) {
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int sms = 0;
+    const cudaError_t e = device_sms(&sms);
     return e == cudaSuccess ? launch_polar_cta(p, sms, s) : e;
   }
   switch (p.dtype) {
