@@ -59,13 +59,13 @@ struct TcParams {
   uint32_t idesc;
   GemmEpilogue e;
   TcPolar polar;
-  int res_kind, y_vec, pre_vec, res_vec;
+  int res_kind, y_vec, pre_vec, res_vec, bias_vec;
   int64_t y_plane, res_plane;
   int inject;
 };
 
 // ---------------------------------------------------------------------------
-// epilogue of one lane's 32 columns
+// epilogue
 // ---------------------------------------------------------------------------
 
 struct Halves {};  // output tag: two f16 planes
@@ -74,6 +74,44 @@ template <typename OUT>
 struct OutOf { typedef OUT T; };
 template <>
 struct OutOf<Halves> { typedef __half T; };
+
+// Eight neighbours along i or j: v = alpha D, r = the addends; see TcPolarMode.
+template <bool ALONG_I>
+__device__ __forceinline__ void polar8(float (&v)[8], const float (&r)[8], const TcPolar& q, float beta, int64_t b, int64_t i,
+                                       int64_t j, int n) {
+  const float f = q.r ? q.r[b] : 1.f;
+  const float* d = q.d_in + b * q.side;
+  float* out = q.d_out + b * q.side;
+  const int64_t along = ALONG_I ? i : j, across = ALONG_I ? j : i, diag = across - along;  // which of them is diagonal
+  if (q.mode == kPolarS) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] *= f * f;
+      if (k == diag && k < n) out[across] = v[k] * q.k, v[k] = 0.f;
+    }
+    return;
+  }
+  // the diagonal enters by the row, the column or both
+  const bool by_along = q.mode == kPolarP || q.mode == (ALONG_I ? kPolarXi : kPolarXj);
+  const bool by_across = q.mode == kPolarP || q.mode == (ALONG_I ? kPolarXj : kPolarXi);
+  const float da = by_across ? d[across] : 0.f;
+  float w[8] = {};
+  if (by_along) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) w[k] = d[along + k];
+  }
+  if (q.mode == kPolarP) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k == diag && k < n) out[across] = fmaf(q.k2, v[k], da * fmaf(q.k3, da, q.k4)), v[k] = 0.f;
+      else v[k] = fmaf(fmaf(q.k, da + w[k], beta), r[k], v[k]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = f * fmaf(beta * (q.k + da + w[k]), r[k], v[k]);
+}
 
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
   const __nv_bfloat162 v = __halves2bfloat162(a, b);
@@ -183,7 +221,7 @@ __device__ __forceinline__ void apply_act(float (&v)[32], int act) {
 }
 
 // v = alpha D, r = the addend; see TcPolarMode.
-__device__ __forceinline__ void polar_epilogue(float (&v)[32], const float (&r)[32], const TcPolar& q, const GemmEpilogue& e,
+__device__ __forceinline__ void polar_row32(float (&v)[32], const float (&r)[32], const TcPolar& q, const GemmEpilogue& e,
                                                int64_t b, int64_t i, int64_t j, int rows, int cols, int lane) {
   const float f = q.r ? q.r[b] : 1.f;
   const float* d = q.d_in + b * q.side;
@@ -225,67 +263,50 @@ __device__ __forceinline__ void polar_epilogue(float (&v)[32], const float (&r)[
   }
 }
 
-// v: 32 columns j.. of row i + lane. rows / cols: how many of the 32 x 32
-// exist (either may be <= 0).
-template <typename OUT>
-__device__ __forceinline__ void epilogue32(float (&v)[32], const TcParams& p, int64_t b, int64_t i, int64_t j, int rows,
-                                           int cols, bool mirror, unsigned char* stage, int lane) {
-  typedef typename OutOf<OUT>::T T;
+// The epilogue of a pair's 16-bit outputs, 32 columns (v) of row i + lane in
+// every lane. The main loop of a pair takes all of its shared memory's
+// bandwidth (64 bytes a clock arriving, 64 read by the tensor cores), so what
+// passes through shared memory here is the rounded outputs alone; with the
+// sums staged in float32 (finish32) four 4096 x 4096 orthogonalisation steps take 1.28
+// times as long.
+// rows / cols: how many of the 32 x 32 exist (either may be <= 0).
+template <typename T>
+__device__ __forceinline__ void finish_row32(float (&v)[32], const TcParams& p, int64_t b, int64_t i, int64_t j, int rows,
+                                             int cols, bool mirror, unsigned char* stage, int lane) {
+  static_assert(sizeof(T) == 2, "16-bit outputs");
   const GemmEpilogue& e = p.e;
   if (rows <= 0 || cols <= 0) return;
 #pragma unroll
   for (int c = 0; c < 32; ++c) v[c] *= e.alpha;
-  if constexpr (!std::is_same<OUT, Halves>::value) {
-    if (e.bias) {
-      const T* bias = static_cast<const T*>(e.bias);
-      if (e.bias_on_i) {
-        const float x = lane < rows ? to_f32(bias[i + lane]) : 0.f;
+  if (e.bias) {
+    const T* bias = static_cast<const T*>(e.bias);
+    if (e.bias_on_i) {
+      const float x = lane < rows ? to_f32(bias[i + lane]) : 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] += x;
-      } else {
-        const float x = lane < cols ? to_f32(bias[j + lane]) : 0.f;
+      for (int c = 0; c < 32; ++c) v[c] += x;
+    } else {
+      const float x = lane < cols ? to_f32(bias[j + lane]) : 0.f;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] += __shfl_sync(kFull, x, c);
-      }
+      for (int c = 0; c < 32; ++c) v[c] += __shfl_sync(kFull, x, c);
     }
-    if (e.pre.p) store_tile<T>(v, e.pre, b, i, j, rows, cols, p.pre_vec, stage, lane);
-    apply_act<sizeof(T) == 2>(v, e.act);
   }
+  if (e.pre.p) store_tile<T>(v, e.pre, b, i, j, rows, cols, p.pre_vec, stage, lane);
+  apply_act<true>(v, e.act);
   float r[32] = {};
   if (e.res.p && lane < rows) {
     const int64_t off = b * e.res.bs + (i + lane) * e.res.is + j * e.res.js;
-    switch (p.res_kind) {
-      case B2C_F32: load_res(r, static_cast<const float*>(e.res.p) + off, e.res.js, cols, p.res_vec); break;
-      case B2C_BF16: load_res(r, static_cast<const __nv_bfloat16*>(e.res.p) + off, e.res.js, cols, p.res_vec); break;
-      default:
-        if (p.res_kind == kOutHalves)
-          load_res(r, static_cast<const __half*>(e.res.p) + p.res_plane + off, e.res.js, cols, p.res_vec);
-        load_res(r, static_cast<const __half*>(e.res.p) + off, e.res.js, cols, p.res_vec);
-    }
+    const int vec = p.res_vec && e.res.js == 1;
+    if (p.res_kind == B2C_BF16) load_res(r, static_cast<const __nv_bfloat16*>(e.res.p) + off, e.res.js, cols, vec);
+    else load_res(r, static_cast<const __half*>(e.res.p) + off, e.res.js, cols, vec);
   }
-  if (p.polar.mode == kPolarNone) {
-    if (e.res.p) {
+  if (p.polar.mode != kPolarNone) {
+    polar_row32(v, r, p.polar, e, b, i, j, rows, cols, lane);
+  } else if (e.res.p) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = fmaf(e.beta, r[c], v[c]);
-    }
-  } else {
-    polar_epilogue(v, r, p.polar, e, b, i, j, rows, cols, lane);
+    for (int c = 0; c < 32; ++c) v[c] = fmaf(e.beta, r[c], v[c]);
   }
-  const GemmView flip{e.y.p, e.y.bs, e.y.js, e.y.is};
-  if constexpr (std::is_same<OUT, Halves>::value) {
-    float lo[32];
-#pragma unroll
-    for (int c = 0; c < 32; ++c) lo[c] = v[c] - __half2float(__float2half_rn(v[c]));
-    store_tile<__half>(v, e.y, b, i, j, rows, cols, p.y_vec, stage, lane);
-    if (mirror) store_tile<__half>(v, flip, b, i, j, rows, cols, p.y_vec, stage, lane);
-    const GemmView y2{static_cast<__half*>(e.y.p) + p.y_plane, e.y.bs, e.y.is, e.y.js};
-    const GemmView f2{y2.p, e.y.bs, e.y.js, e.y.is};
-    store_tile<__half>(lo, y2, b, i, j, rows, cols, p.y_vec, stage, lane);
-    if (mirror) store_tile<__half>(lo, f2, b, i, j, rows, cols, p.y_vec, stage, lane);
-  } else {
-    store_tile<T>(v, e.y, b, i, j, rows, cols, p.y_vec, stage, lane);
-    if (mirror) store_tile<T>(v, flip, b, i, j, rows, cols, p.y_vec, stage, lane);
-  }
+  store_tile<T>(v, e.y, b, i, j, rows, cols, p.y_vec, stage, lane);
+  if (mirror) store_tile<T>(v, GemmView{e.y.p, e.y.bs, e.y.js, e.y.is}, b, i, j, rows, cols, 0, stage, lane);
 }
 
 struct Tile {
@@ -320,6 +341,217 @@ __device__ __forceinline__ Tile tile_at(const TcParams& p, int64_t t) {
   o.j = v / w * p.BN;
   o.mirror = false;
   return o;
+}
+
+
+// The epilogue of a block of D whose sums lie in shared memory, row by row:
+// the sums leave tensor memory with a row in every lane, but addends and outputs are
+// read and written along their rows. Kept small on purpose, since a kernel
+// that runs once over a tile fetches every instruction from memory (with 32 columns a
+// lane, unrolled, 32 x 32 values took 2,600 clocks, 8,400 with an addend).
+
+template <typename T>
+__device__ __forceinline__ void load8(float (&v)[8], const T* at, int64_t js, int n, bool vec) {
+  if (vec) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 8 / PER; ++u) {
+      const uint4 w = *reinterpret_cast<const uint4*>(at + u * PER);
+      const T* q = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int c = 0; c < PER; ++c) v[u * PER + c] += to_f32(q[c]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < n) v[c] += to_f32(at[c * js]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* at, const float (&v)[8], int n, bool vec) {
+  if (vec) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < 8 / PER; ++u) {
+      uint4 w;
+      T* q = reinterpret_cast<T*>(&w);
+#pragma unroll
+      for (int c = 0; c < PER; ++c) q[c] = from_f32<T>(v[u * PER + c]);
+      *reinterpret_cast<uint4*>(at + u * PER) = w;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < n) at[c] = from_f32<T>(v[c]);
+  }
+}
+
+// n (up to 8) addends at stride js.
+__device__ __forceinline__ void load_res8(float (&r)[8], const TcParams& p, int64_t at, int64_t js, int n, bool vec) {
+  const void* base = p.e.res.p;
+  if (p.res_kind == B2C_F32) load8(r, static_cast<const float*>(base) + at, js, n, vec);
+  else if (p.res_kind == B2C_BF16) load8(r, static_cast<const __nv_bfloat16*>(base) + at, js, n, vec);
+  else load8(r, static_cast<const __half*>(base) + at, js, n, vec);
+  if (p.res_kind == kOutHalves) load8(r, static_cast<const __half*>(base) + p.res_plane + at, js, n, vec);
+}
+
+template <bool FAST>
+__device__ __forceinline__ void act8(float (&v)[8], int act) {
+  switch (act) {
+    case B2C_ACT_RELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = act_f32<FAST>(v[k], B2C_ACT_RELU);
+      break;
+    case B2C_ACT_GELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = act_f32<FAST>(v[k], B2C_ACT_GELU);
+      break;
+    case B2C_ACT_GELU_TANH:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = act_f32<FAST>(v[k], B2C_ACT_GELU_TANH);
+      break;
+    case B2C_ACT_SILU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = act_f32<FAST>(v[k], B2C_ACT_SILU);
+      break;
+    default: break;
+  }
+}
+
+// The sums v of n (up to 8) neighbours from (i, j) along the axis that has
+// unit stride in y and pre: i (ALONG_I) or j.
+template <typename OUT, bool ALONG_I>
+__device__ __forceinline__ void finish8(const TcParams& p, int64_t b, int64_t i, int64_t j, int n, float (&v)[8]) {
+  typedef typename OutOf<OUT>::T T;
+  const GemmEpilogue& e = p.e;
+  const bool whole = n == 8;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] *= e.alpha;
+  if constexpr (!std::is_same<OUT, Halves>::value) {
+    if (e.bias) {
+      const bool along = ALONG_I == (bool)e.bias_on_i;
+      load8(v, static_cast<const T*>(e.bias) + (e.bias_on_i ? i : j), along ? 1 : 0, n, along && whole && p.bias_vec);
+    }
+    if (e.pre.p)
+      store8(static_cast<T*>(e.pre.p) + b * e.pre.bs + i * e.pre.is + j * e.pre.js, v, n, whole && p.pre_vec);
+    act8<sizeof(T) == 2>(v, e.act);
+  }
+  if (p.polar.mode != kPolarNone) {
+    float x[8] = {};
+    if (e.res.p)
+      load_res8(x, p, b * e.res.bs + i * e.res.is + j * e.res.js, ALONG_I ? e.res.is : e.res.js, n, whole && p.res_vec);
+    polar8<ALONG_I>(v, x, p.polar, e.beta, b, i, j, n);
+  } else if (e.res.p) {
+    float x[8] = {};
+    load_res8(x, p, b * e.res.bs + i * e.res.is + j * e.res.js, ALONG_I ? e.res.is : e.res.js, n, whole && p.res_vec);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = fmaf(e.beta, x[k], v[k]);
+  }
+  T* y = static_cast<T*>(e.y.p) + b * e.y.bs + i * e.y.is + j * e.y.js;
+  store8(y, v, n, whole && p.y_vec);
+  if constexpr (std::is_same<OUT, Halves>::value) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] -= __half2float(__float2half_rn(v[k]));
+    store8(y + p.y_plane, v, n, whole && p.y_vec);
+  }
+}
+
+// The sum over the cluster, in order, of 8 values at distance `step` from `at`.
+template <bool CLUSTER>
+__device__ __forceinline__ void joined8(const float* at, int step, int split, float (&v)[8]) {
+  if (!CLUSTER || split == 1) {
+    if (CLUSTER && step == 1) {  // rows of the single CTAs' sums start on 16 bytes
+      const float4 x = *reinterpret_cast<const float4*>(at), y = *reinterpret_cast<const float4*>(at + 4);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = at[k * step];
+    }
+    return;
+  }
+  const uint32_t a = smem_u32(at);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 0.f;
+  for (int q = 0; q < split; ++q) {
+    const uint32_t peer = map_rank(a, q);
+    if (step == 1) {
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        float x, y, z, w;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(x), "=f"(y), "=f"(z), "=f"(w)
+                     : "r"(peer + k * 4)
+                     : "memory");
+        v[k] += x, v[k + 1] += y, v[k + 2] += z, v[k + 3] += w;
+      }
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float x;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(peer + k * step * 4) : "memory");
+      v[k] += x;
+    }
+  }
+}
+
+// A block of sums: 2^lg_rows x 2^lg_cols of them, from row i and column j of D.
+struct Block {
+  int64_t b, i, j;
+  const float* sums;
+  int pitch, lg_rows, lg_cols;
+};
+
+// Thread t0 of nt finishes its share of the block. With mirror the block is
+// also written as its transpose (the other half of a symmetric product).
+template <typename OUT, bool CLUSTER>
+__device__ __forceinline__ void finish(const TcParams& p, const Block& o, bool mirror, int t0, int nt) {
+  const int total = 1 << (o.lg_rows + o.lg_cols - 3);
+  float v[8];
+  if (p.e.y.js == 1) {
+#pragma unroll 1
+    for (int u = t0; u < total; u += nt) {
+      const int r = u >> (o.lg_cols - 3), c = (u & ((1 << (o.lg_cols - 3)) - 1)) * 8;
+      const int64_t i = o.i + r, j = o.j + c;
+      if (i >= p.I || j >= p.J) continue;
+      joined8<CLUSTER>(o.sums + r * o.pitch + c, 1, p.split, v);
+      finish8<OUT, false>(p, o.b, i, j, p.J - j < 8 ? (int)(p.J - j) : 8, v);
+    }
+  } else {
+#pragma unroll 1
+    for (int u = t0; u < total; u += nt) {
+      const int c = u >> (o.lg_rows - 3), r = (u & ((1 << (o.lg_rows - 3)) - 1)) * 8;
+      const int64_t i = o.i + r, j = o.j + c;
+      if (i >= p.I || j >= p.J) continue;
+      joined8<CLUSTER>(o.sums + r * o.pitch + c, o.pitch, p.split, v);
+      finish8<OUT, true>(p, o.b, i, j, p.I - i < 8 ? (int)(p.I - i) : 8, v);
+    }
+  }
+  if (mirror) {
+#pragma unroll 1
+    for (int u = t0; u < total; u += nt) {
+      const int c = u >> (o.lg_rows - 3), r = (u & ((1 << (o.lg_rows - 3)) - 1)) * 8;
+      const int64_t i = o.j + c, j = o.i + r;
+      if (i >= p.I || j >= p.J) continue;
+      joined8<CLUSTER>(o.sums + r * o.pitch + c, o.pitch, p.split, v);
+      finish8<OUT, false>(p, o.b, i, j, p.J - j < 8 ? (int)(p.J - j) : 8, v);
+    }
+  }
+}
+
+// A warp's 32 x 32 values, one row a lane, through its own staging rows.
+// With 33 floats a row both ways of reading it touch every bank once.
+constexpr int kStagePitch = 33;
+constexpr int kStageFloats = 32 * kStagePitch;  // a multiple of 4, for 16-byte units in other layouts
+template <typename OUT>
+__device__ __forceinline__ void finish32(const TcParams& p, const float (&v)[32], int64_t b, int64_t i, int64_t j, bool mirror,
+                                         float* stage, int lane) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) stage[lane * kStagePitch + c] = v[c];
+  __syncwarp();
+  finish<OUT, false>(p, Block{b, i, j, stage, kStagePitch, 5, 5}, mirror, lane, 32);
+  __syncwarp();
 }
 
 __device__ __forceinline__ int clamp32(int64_t n) { return n > 32 ? 32 : (int)n; }
@@ -416,13 +648,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
-  typedef typename OutOf<OUT>::T T;
   constexpr bool JOIN = PLANES > 1;
-  constexpr int kStage = 32 * (32 * sizeof(T) + 16);  // one warp's staging rows
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
-  unsigned char* staging = ring + p.stages * p.stage_bytes;
+  float* staging = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, tfull0 = empty0 + 8 * kMaxStages,
                  tempty0 = tfull0 + 16, never = tempty0 + 16;
   const uint64_t limit = p.inject ? 1000000ull : kWaitNs;
@@ -459,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3, half = warp >> 2;
     const uint32_t lead_tempty0 = map_rank(tempty0, 0);
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    unsigned char* stage = staging + warp * kStage;
+    float* stage = staging + warp * kStageFloats;
     uint32_t buf = 0, tphase = 0;
     bool ok = true;
     const float bad = __int_as_float(0x7fffffff);
@@ -467,7 +697,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int64_t t = first; t < p.tiles; t += step) {
       const Tile o = tile_at<2>(p, t);
       const int64_t i = o.i + rank * BM + quad * 32;
-      const int rows = clamp32(p.I - i);
       if constexpr (JOIN) {
         float acc[4][32];
 #pragma unroll
@@ -496,7 +725,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 32; ++c) acc[q][c] = bad;
           }
-          epilogue32<OUT>(acc[q], p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
+          finish32<OUT>(p, acc[q], o.b, i, o.j + col, o.mirror, stage, lane);
         }
       } else {
         ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
@@ -513,7 +742,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] = bad;
           }
-          epilogue32<OUT>(v, p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
+          finish_row32<OUT>(v, p, o.b, i, o.j + col, clamp32(p.I - i), clamp32(p.J - o.j - col), o.mirror,
+                            reinterpret_cast<unsigned char*>(stage), lane);
         }
         if (++buf == 2) buf = 0, tphase ^= 1;
       }
@@ -591,10 +821,8 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
-  typedef typename OutOf<OUT>::T T;
   constexpr bool JOIN = PLANES > 1;
   constexpr int EPI = Solo<PLANES>::EPI, GROUPS = EPI / 4, SLICES = JOIN ? 4 / GROUPS : 1;
-  constexpr int kStage = 32 * (32 * sizeof(T) + 16);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = p.split, rank = split > 1 ? (int)cluster_rank() : 0;
   unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
@@ -631,10 +859,8 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   volatile int* gu = &gave_up;
   const int quad = warp & 3, group = warp >> 2;
   const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-  const int64_t i = o.i + quad * 32;
-  const int rows = clamp32(p.I - i), pitch = p.BN + 4;
-  float* partial = reinterpret_cast<float*>(ring);
-  unsigned char* stage = ring + (split > 1 ? BM * pitch * 4 : 0) + warp * kStage;
+  const int pitch = p.BN + 4;
+  float* partial = reinterpret_cast<float*>(ring);  // this CTA's sums of the tile, once the ring is free
 
   if (warp < EPI) {
     bool ok = true;
@@ -668,7 +894,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
       ok = __all_sync(kFull, ok && bar_wait(tfull0, 0, gu, limit, &g_gemm_fault));
       fence_after();
     }
-    // every product is done: the ring is free for partial sums and staging (after a wait that ran out, once what is
+    // every product is done, so the ring is free (after a wait that ran out, once what is
     // still in flight has landed)
     if (!ok) settle();
 #pragma unroll
@@ -681,13 +907,9 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
 #pragma unroll
           for (int c = 0; c < 32; ++c) v[c] = __int_as_float(0x7fffffff);
         }
-        if (split > 1) {
-          float4* at = reinterpret_cast<float4*>(partial + (quad * 32 + lane) * pitch + col);
+        float4* at = reinterpret_cast<float4*>(partial + (quad * 32 + lane) * pitch + col);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) at[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-        } else {
-          epilogue32<OUT>(v, p, o.b, i, o.j + col, rows, clamp32(p.J - o.j - col), o.mirror, stage, lane);
-        }
+        for (int c = 0; c < 8; ++c) at[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
       }
     }
   } else if (warp == EPI && lane == 0) {
@@ -715,33 +937,15 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
       if (JOIN && ++buf == 2) buf = 0, tphase ^= 1;
     }
   }
-  if (split > 1) {
-    __syncwarp();
-    cluster_sync();
-    // the tile's 32 x 32 pieces are dealt over the cluster's epilogue warps
-    if (warp < EPI) {
-      for (int u = rank * EPI + warp; u < 4 * (p.BN / 32); u += split * EPI) {
-        const int pq = u & 3, col = (u >> 2) * 32;
-        const uint32_t at = smem_u32(partial + (pq * 32 + lane) * pitch + col);
-        float v[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = 0.f;
-        for (int q = 0; q < split; ++q) {
-          const uint32_t peer = map_rank(at, q);
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            float x, y, z, w;
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x), "=f"(y), "=f"(z), "=f"(w) : "r"(peer + c * 4) : "memory");
-            v[c] += x, v[c + 1] += y, v[c + 2] += z, v[c + 3] += w;
-          }
-        }
-        const int64_t ii = o.i + pq * 32;
-        epilogue32<OUT>(v, p, o.b, ii, o.j + col, clamp32(p.I - ii), clamp32(p.J - o.j - col), o.mirror, stage, lane);
-      }
-    }
-    __syncwarp();
-    cluster_sync();  // peers' partial sums stay until they have been read
-  }
+  __syncwarp();
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+  // each CTA of the cluster finishes its share of the rows
+  const int nrows = BM / split, r0 = rank * nrows;
+  const Block mine{o.b, o.i + r0, o.j, partial + r0 * pitch, pitch, 31 - __clz(nrows), 31 - __clz(p.BN)};
+  finish<OUT, true>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
+  __syncwarp();
+  if (split > 1) cluster_sync();  // peers' sums stay until they have been read
   __syncthreads();
   if (gave_up) settle();
   fence_before();
@@ -789,8 +993,10 @@ bool encode(CUtensorMap* m, const TcOperand& o, int f16, int planes, int64_t bat
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool vec16(const void* p, int64_t elt, int64_t bs, int64_t is, int64_t js, int64_t plane) {
-  return js == 1 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && bs * elt % 16 == 0 && is * elt % 16 == 0 &&
+// Whether 8 neighbours along j (or i) can be read and written as 16-byte units.
+bool vec16(const GemmView& v, bool along_i, int64_t elt, int64_t plane) {
+  const int64_t unit = along_i ? v.is : v.js, other = along_i ? v.js : v.is;
+  return v.p && unit == 1 && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.bs * elt % 16 == 0 && other * elt % 16 == 0 &&
          plane * elt % 16 == 0;
 }
 
@@ -814,8 +1020,7 @@ cudaError_t launch_in_clusters(Kern kern, int64_t ctas, int cluster, int threads
 
 template <int PLANES, typename OUT>
 cudaError_t launch_pair(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
-  typedef typename OutOf<OUT>::T T;
-  const int staging = kEpiWarps * 32 * (32 * (int)sizeof(T) + 16);
+  const int staging = kEpiWarps * kStageFloats * 4;
   const int stages = (kSmemMax - 1024 - 512 - staging) / p.stage_bytes;
   p.stages = stages > kMaxStages ? kMaxStages : stages;
   const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + staging;
@@ -829,16 +1034,17 @@ cudaError_t launch_pair(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p
 }
 
 template <int PLANES, typename OUT>
-cudaError_t launch_solo(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int, cudaStream_t s) {
-  typedef typename OutOf<OUT>::T T;
+cudaError_t launch_solo(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
   constexpr int NT = Solo<PLANES>::NT;
-  const int staging = Solo<PLANES>::EPI * 32 * (32 * (int)sizeof(T) + 16) + (p.split > 1 ? BM * (p.BN + 4) * 4 : 0);
+  const int sums = BM * (p.BN + 4) * 4;
   const int per = (p.kblocks + p.split - 1) / p.split;
-  int stages = (Solo<PLANES>::SMEM - 1024 - 512) / p.stage_bytes;
+  // all of an SM's shared memory where it gets one CTA anyway: a slice takes about 2,000 clocks to arrive
+  const int room = p.tiles * p.split <= sms ? kSmemMax - 1024 : Solo<PLANES>::SMEM;
+  int stages = (room - 1024 - 512) / p.stage_bytes;
   if (stages > kMaxStages) stages = kMaxStages;
   p.stages = stages > per ? per : stages;
   size_t smem = (size_t)p.stages * p.stage_bytes;
-  if (smem < (size_t)staging) smem = staging;
+  if (smem < (size_t)sums) smem = sums;
   smem += 1024;
   p.tmem_cols = 32;
   while (p.tmem_cols < (PLANES > 1 ? 2 : 1) * p.BN) p.tmem_cols *= 2;
@@ -878,30 +1084,38 @@ struct Form {
   double clocks;
 };
 
-// Estimated clocks of an SM: its share of tiles times the longer of loading a
-// slice (about 40 bytes a clock and SM from L2) and multiplying it (128 x 16 x
-// 16 values a clock, and 128 bytes of shared memory a clock), plus what a
-// launch, a join over a cluster and an epilogue cost. Only the order of these
-// estimates matters: on 1000 x 777 x 1301 float32 the forms take 26 to 80 us, on
-// 16 x 4096 x 16384 f16 29 to 44 us, and the estimate's choice is the first.
+// Estimated clocks: waves of CTAs times their slices of k, each the longest of
+// its arrival (500 clocks with a full ring), its load (L2 gives an SM up to
+// 100 bytes a clock and all of them 6,000) and its products (4096 a clock, and
+// 128 bytes of shared memory a clock), plus what a CTA costs beside them. Fitted to
+// sweeps of these forms; measured, us, the first of each the choice:
+//   16 x 4096 x 16384 f16       32 columns 37, split 2 38, 4 48, 64 columns 39
+//   16 x 8192 x 8192 bf16       32 columns split 2 36, 1 51, 4 39, 8 48
+//   512 x 2048 x 512 bf16       64 columns split 4 11, 2 13, 1 17, pairs 20
+//   1000 x 777 x 1301 float32   128 columns 28, split 2 38, 64 columns 46, pairs 69
+//   2048 x 2048 x 2048 bf16     pairs 22, 128 columns 25, 64 columns 37
 Form choose_form(const TcProblem& t, int kblocks, int planes, int nseg, int sms) {
   Form best{0, 0, 0, 1e300};
   const int64_t ti = (t.I + BM - 1) / BM;
+  auto rate = [&](double ctas) { return fmin(100.0, 6000.0 / fmin(ctas, (double)sms)); };
   for (int BN = t.sym ? 128 : 32; BN <= 128; BN *= 2) {
     if (!t.sym && BN > 32 && BN / 2 >= t.J) break;
     const int64_t tj = (t.J + BN - 1) / BN, tiles = t.batch * (t.sym ? ti * (ti + 1) / 2 : ti * tj);
-    for (int split = 1; split <= 8 && split <= kblocks; split *= 2) {
-      const double load = planes * (16384.0 + BN * 128.0) / 40, mul = nseg * 4.0 * fmax(BN / 2.0, (128 + BN) / 4.0);
-      const double slice = fmax(load, mul), ctas = ceil((double)tiles * split / sms);
-      const double c = ctas * ((kblocks + split - 1) / split * slice + BN * 12.0) + 3000 + (split > 1 ? 1500 : 0);
+    for (int split = 1; split <= 4 && split <= kblocks; split *= 2) {
+      const double ctas = (double)tiles * split, on_sm = ceil(ctas / sms), at_once = fmin(on_sm, planes > 1 ? 1.0 : 2.0);
+      const double load = planes * (16384.0 + BN * 128.0) / rate(ctas), mul = nseg * 4.0 * fmax(BN / 2.0, (128 + BN) / 4.0);
+      const double slice = fmax(500.0, at_once * fmax(load, mul));
+      const double c = ceil(on_sm / at_once) * ((kblocks + split - 1) / split * slice + 8000 + BN * 20) +
+                       (split > 2 ? 4000 : split > 1 ? 1500 : 0);
       if (c < best.clocks) best = Form{0, BN, split, c};
     }
   }
   if (t.I > BM && t.J > 128) {
     const int64_t ti2 = (t.I + 255) / 256, tj2 = (t.J + 255) / 256;
     const int64_t tiles = t.batch * (t.sym ? ti2 * (ti2 + 1) / 2 : ti2 * tj2);
-    const double slice = fmax(planes * 32768.0 / 40, nseg * 4.0 * 128);
-    const double c = ceil(2.0 * tiles / sms) * kblocks * slice + 4000 + 3000;
+    // with several planes the ring holds two or three slices, and their arrival is not hidden
+    const double slice = planes > 1 ? planes * 2000.0 : fmax(32768.0 / rate(2.0 * tiles), 4.0 * 128);
+    const double c = ceil(2.0 * tiles / sms) * kblocks * slice + 11000;
     if (c < best.clocks) best = Form{1, 256, 1, c};
   }
   return best;
@@ -969,9 +1183,11 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   p.y_plane = t.y_plane;
   p.res_plane = t.res_plane;
   const int64_t osize = t.out == B2C_F32 ? 4 : 2, rsize = t.res == B2C_F32 ? 4 : 2;
-  p.y_vec = vec16(t.e.y.p, osize, t.e.y.bs, t.e.y.is, t.e.y.js, t.y_plane);
-  p.pre_vec = vec16(t.e.pre.p, osize, t.e.pre.bs, t.e.pre.is, t.e.pre.js, 0);
-  p.res_vec = t.e.res.p && vec16(t.e.res.p, rsize, t.e.res.bs, t.e.res.is, t.e.res.js, t.res_plane);
+  const bool along_i = t.e.y.js != 1;
+  p.y_vec = vec16(t.e.y, along_i, osize, t.y_plane);
+  p.pre_vec = vec16(t.e.pre, along_i, osize, 0);
+  p.res_vec = vec16(t.e.res, along_i, rsize, t.res_plane);
+  p.bias_vec = (reinterpret_cast<uintptr_t>(t.e.bias) & 15) == 0;
   p.inject = inject_timeout();
   CUtensorMap mp, mq;
   if (!encode(&mp, t.P, t.f16, planes, t.batch, t.I, t.K, BM) ||
