@@ -42,10 +42,17 @@ namespace {
 
 constexpr int BM = 128;          // rows of D per CTA
 constexpr int BK = 64;           // depth of a slice: 128 bytes
-constexpr int kEpiWarps = 8;      // of a pair's CTA
-constexpr int kThreads = (kEpiWarps + 4) * 32;  // the last warpgroup: loads, products, two idle warps
-// Registers: 384 x 168 at launch = 128 x 72 + 256 x 216 after the split.
-constexpr int kRegsFew = 72, kRegsMany = 216;
+// Warps of a pair's CTA: its epilogue warps, then a warpgroup of loads,
+// products and two idle warps. Joined sums stay in registers, 64 a thread with
+// sixteen epilogue warps (eight, with 128, took 1.3 times as long over a tile).
+template <int PLANES>
+struct Pair {
+  static constexpr bool JOIN = PLANES > 1;
+  static constexpr int EPI = JOIN ? 16 : 8;
+  static constexpr int NT = (EPI + 4) * 32;
+  // registers where JOIN: 640 x 96 at launch = 128 x 64 + 512 x 104 after the split
+  static constexpr int FEW = 64, MANY = 104;
+};
 constexpr int kMaxStages = 8;
 constexpr int kABytes = BM * BK * 2;  // one plane of P's rows in a slice
 constexpr int kSmemMax = 232448;
@@ -419,10 +426,21 @@ __device__ __forceinline__ void act8(float (&v)[8], int act) {
   }
 }
 
-// The sums v of n (up to 8) neighbours from (i, j) along the axis that has
-// unit stride in y and pre: i (ALONG_I) or j.
+// The addends of 8 neighbours, zeros where there are none.
+template <bool ALONG_I>
+__device__ __forceinline__ void addends8(float (&x)[8], const TcParams& p, int64_t b, int64_t i, int64_t j, int n) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = 0.f;
+  const GemmEpilogue& e = p.e;
+  if (e.res.p)
+    load_res8(x, p, b * e.res.bs + i * e.res.is + j * e.res.js, ALONG_I ? e.res.is : e.res.js, n, n == 8 && p.res_vec);
+}
+
+// The sums v and addends x of n (up to 8) neighbours from (i, j) along the
+// axis that has unit stride in y and pre: i (ALONG_I) or j.
 template <typename OUT, bool ALONG_I>
-__device__ __forceinline__ void finish8(const TcParams& p, int64_t b, int64_t i, int64_t j, int n, float (&v)[8]) {
+__device__ __forceinline__ void finish8(const TcParams& p, int64_t b, int64_t i, int64_t j, int n, float (&v)[8],
+                                        const float (&x)[8]) {
   typedef typename OutOf<OUT>::T T;
   const GemmEpilogue& e = p.e;
   const bool whole = n == 8;
@@ -438,13 +456,8 @@ __device__ __forceinline__ void finish8(const TcParams& p, int64_t b, int64_t i,
     act8<sizeof(T) == 2>(v, e.act);
   }
   if (p.polar.mode != kPolarNone) {
-    float x[8] = {};
-    if (e.res.p)
-      load_res8(x, p, b * e.res.bs + i * e.res.is + j * e.res.js, ALONG_I ? e.res.is : e.res.js, n, whole && p.res_vec);
     polar8<ALONG_I>(v, x, p.polar, e.beta, b, i, j, n);
   } else if (e.res.p) {
-    float x[8] = {};
-    load_res8(x, p, b * e.res.bs + i * e.res.is + j * e.res.js, ALONG_I ? e.res.is : e.res.js, n, whole && p.res_vec);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = fmaf(e.beta, x[k], v[k]);
   }
@@ -503,41 +516,62 @@ struct Block {
   int pitch, lg_rows, lg_cols;
 };
 
+// Units of 8 of a block: along the rows of the sums, along their columns, or
+// along their columns as rows of the transpose.
+enum FinishMode { kRowUnits, kColUnits, kMirrorUnits };
+
+// Threads t0, t0 + nt, ... take a block's units, BATCH at a time: their addends
+// are asked for together, since each is a trip to memory.
+template <typename OUT, bool CLUSTER, int BATCH, int MODE>
+__device__ __forceinline__ void finish_units(const TcParams& p, const Block& o, int t0, int nt) {
+  constexpr bool ALONG_I = MODE == kColUnits;
+  const int total = 1 << (o.lg_rows + o.lg_cols - 3), lg = (MODE == kRowUnits ? o.lg_cols : o.lg_rows) - 3;
+  const int64_t end_i = p.I, end_j = p.J;
+#pragma unroll 1
+  for (int u0 = t0; u0 < total; u0 += nt * BATCH) {
+    float x[BATCH][8];
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int u = u0 + q * nt, across = u >> lg, along = (u & ((1 << lg) - 1)) * 8;
+      const int64_t i = MODE == kRowUnits ? o.i + across : MODE == kColUnits ? o.i + along : o.j + across;
+      const int64_t j = MODE == kRowUnits ? o.j + along : MODE == kColUnits ? o.j + across : o.i + along;
+      const int64_t left = ALONG_I ? end_i - i : end_j - j;
+      if (u < total && i < end_i && j < end_j) addends8<ALONG_I>(x[q], p, o.b, i, j, left < 8 ? (int)left : 8);
+    }
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int u = u0 + q * nt, across = u >> lg, along = (u & ((1 << lg) - 1)) * 8;
+      const int64_t i = MODE == kRowUnits ? o.i + across : MODE == kColUnits ? o.i + along : o.j + across;
+      const int64_t j = MODE == kRowUnits ? o.j + along : MODE == kColUnits ? o.j + across : o.i + along;
+      const int64_t left = ALONG_I ? end_i - i : end_j - j;
+      if (u >= total || i >= end_i || j >= end_j) continue;
+      const int r = MODE == kRowUnits ? across : along, c = MODE == kRowUnits ? along : across;
+      float v[8];
+      joined8<CLUSTER>(o.sums + r * o.pitch + c, MODE == kRowUnits ? 1 : o.pitch, p.split, v);
+      finish8<OUT, ALONG_I>(p, o.b, i, j, left < 8 ? (int)left : 8, v, x[q]);
+    }
+  }
+}
+
 // Thread t0 of nt finishes its share of the block. With mirror the block is
 // also written as its transpose (the other half of a symmetric product).
-template <typename OUT, bool CLUSTER>
+template <typename OUT, bool CLUSTER, int BATCH>
 __device__ __forceinline__ void finish(const TcParams& p, const Block& o, bool mirror, int t0, int nt) {
-  const int total = 1 << (o.lg_rows + o.lg_cols - 3);
-  float v[8];
-  if (p.e.y.js == 1) {
-#pragma unroll 1
-    for (int u = t0; u < total; u += nt) {
-      const int r = u >> (o.lg_cols - 3), c = (u & ((1 << (o.lg_cols - 3)) - 1)) * 8;
-      const int64_t i = o.i + r, j = o.j + c;
-      if (i >= p.I || j >= p.J) continue;
-      joined8<CLUSTER>(o.sums + r * o.pitch + c, 1, p.split, v);
-      finish8<OUT, false>(p, o.b, i, j, p.J - j < 8 ? (int)(p.J - j) : 8, v);
-    }
-  } else {
-#pragma unroll 1
-    for (int u = t0; u < total; u += nt) {
-      const int c = u >> (o.lg_rows - 3), r = (u & ((1 << (o.lg_rows - 3)) - 1)) * 8;
-      const int64_t i = o.i + r, j = o.j + c;
-      if (i >= p.I || j >= p.J) continue;
-      joined8<CLUSTER>(o.sums + r * o.pitch + c, o.pitch, p.split, v);
-      finish8<OUT, true>(p, o.b, i, j, p.I - i < 8 ? (int)(p.I - i) : 8, v);
-    }
-  }
-  if (mirror) {
-#pragma unroll 1
-    for (int u = t0; u < total; u += nt) {
-      const int c = u >> (o.lg_rows - 3), r = (u & ((1 << (o.lg_rows - 3)) - 1)) * 8;
-      const int64_t i = o.j + c, j = o.i + r;
-      if (i >= p.I || j >= p.J) continue;
-      joined8<CLUSTER>(o.sums + r * o.pitch + c, o.pitch, p.split, v);
-      finish8<OUT, false>(p, o.b, i, j, p.J - j < 8 ? (int)(p.J - j) : 8, v);
-    }
-  }
+  if (p.e.y.js == 1) finish_units<OUT, CLUSTER, BATCH, kRowUnits>(p, o, t0, nt);
+  else finish_units<OUT, CLUSTER, BATCH, kColUnits>(p, o, t0, nt);
+  if (mirror) finish_units<OUT, CLUSTER, BATCH, kMirrorUnits>(p, o, t0, nt);
+}
+
+// Asks for 32 addends of a row, to be in L2 when the epilogue reads them: a
+// trip to HBM there is not hidden by anything (1000 products of 256 x 256 x 256, float32, with
+// an addend: 421 us without this).
+__device__ __forceinline__ void prefetch_res(const TcParams& p, int64_t b, int64_t i, int64_t j) {
+  const GemmView& r = p.e.res;
+  if (!r.p || r.js != 1 || i >= p.I || j >= p.J) return;
+  const int64_t at = b * r.bs + i * r.is + j, size = p.res_kind == B2C_F32 ? 4 : 2;
+  const char* q = static_cast<const char*>(r.p) + at * size;
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+  if (p.res_kind == kOutHalves) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + p.res_plane * 2));
 }
 
 // A warp's 32 x 32 values, one row a lane, through its own staging rows.
@@ -550,7 +584,7 @@ __device__ __forceinline__ void finish32(const TcParams& p, const float (&v)[32]
 #pragma unroll
   for (int c = 0; c < 32; ++c) stage[lane * kStagePitch + c] = v[c];
   __syncwarp();
-  finish<OUT, false>(p, Block{b, i, j, stage, kStagePitch, 5, 5}, mirror, lane, 32);
+  finish<OUT, false, 1>(p, Block{b, i, j, stage, kStagePitch, 5, 5}, mirror, lane, 32);
   __syncwarp();
 }
 
@@ -641,7 +675,7 @@ struct Multiplier {
 // ---------------------------------------------------------------------------
 
 template <int PLANES, typename OUT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ TcParams p) {
   extern __shared__ unsigned char raw[];
@@ -649,6 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   constexpr bool JOIN = PLANES > 1;
+  constexpr int EPI = Pair<PLANES>::EPI, GROUPS = EPI / 4, SLICES = 8 / GROUPS;  // slices: 32 columns of a warp's rows
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
@@ -666,11 +701,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     bar_init(never, 1);
     for (int s = 0; s < 2; ++s) {
       bar_init(tfull0 + 8 * s, 1);
-      bar_init(tempty0 + 8 * s, kEpiWarps * 2);
+      bar_init(tempty0 + 8 * s, EPI * 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kEpiWarps) {
+  if (warp == EPI) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     fence_before();
@@ -683,10 +718,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* gu = &gave_up;
   const int per = JOIN ? 1 : p.kblocks;  // slices of one accumulator
 
-  if (warp < kEpiWarps) {
-    if constexpr (JOIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
-    // ---- epilogue: warps w and w + 4 share the rows 32 (w % 4).., and take every other 32 columns ----
-    const int quad = warp & 3, half = warp >> 2;
+  if (warp < EPI) {
+    if constexpr (JOIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Pair<PLANES>::MANY));
+    // ---- epilogue: warps w, w + 4, ... share the rows 32 (w % 4).. and deal out the columns ----
+    const int quad = warp & 3, group = warp >> 2;
     const uint32_t lead_tempty0 = map_rank(tempty0, 0);
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     float* stage = staging + warp * kStageFloats;
@@ -697,19 +732,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int64_t t = first; t < p.tiles; t += step) {
       const Tile o = tile_at<2>(p, t);
       const int64_t i = o.i + rank * BM + quad * 32;
-      if constexpr (JOIN) {
-        float acc[4][32];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < SLICES; ++q) prefetch_res(p, o.b, i + lane, o.j + (GROUPS * q + group) * 32);
+      if constexpr (JOIN) {
+        float acc[SLICES][32];
+#pragma unroll
+        for (int q = 0; q < SLICES; ++q)
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[q][c] = 0.f;
         for (int kb = 0; kb < p.kblocks; ++kb) {
           ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
           fence_after();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < SLICES; ++q) {
             float v[32];
-            tmem_row32(lanes + buf * 256 + (2 * q + half) * 32, v);
+            tmem_row32(lanes + buf * 256 + (GROUPS * q + group) * 32, v);
 #pragma unroll
             for (int c = 0; c < 32; ++c) acc[q][c] += v[c];
           }
@@ -718,22 +755,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) bar_arrive_cluster(lead_tempty0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int col = (2 * q + half) * 32;
+        // one copy of the epilogue's code: the sums move up instead of the index
+#pragma unroll 1
+        for (int q = 0; q < SLICES; ++q) {
           if (!ok) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) acc[q][c] = bad;
+            for (int c = 0; c < 32; ++c) acc[0][c] = bad;
           }
-          finish32<OUT>(p, acc[q], o.b, i, o.j + col, o.mirror, stage, lane);
+          finish32<OUT>(p, acc[0], o.b, i, o.j + (GROUPS * q + group) * 32, o.mirror, stage, lane);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+#pragma unroll
+            for (int m = 1; m < SLICES; ++m) acc[m - 1][c] = acc[m][c];
         }
       } else {
         ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
         fence_after();
-        for (int col = half * 32; col < 256; col += 64) {
+        for (int col = group * 32; col < 256; col += GROUPS * 32) {
           float v[32];
           tmem_row32(lanes + buf * 256 + col, v);
-          if (col + 64 >= 256) {  // the last of this warp's columns: the accumulator is free
+          if (col + GROUPS * 32 >= 256) {  // the last of this warp's columns: the accumulator is free
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive_cluster(lead_tempty0 + 8 * buf);
@@ -749,8 +790,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
-    if (warp == kEpiWarps && lane == 0) {
+    if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Pair<PLANES>::FEW));
+    if (warp == EPI && lane == 0) {
       // ---- loads ----
       const uint32_t lead_full0 = map_rank(full0, 0);
       uint32_t s = 0, phase = 0;
@@ -765,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
         }
       }
-    } else if (warp == kEpiWarps + 1 && rank == 0 && lane == 0) {
+    } else if (warp == EPI + 1 && rank == 0 && lane == 0) {
       // ---- products ----
       const Multiplier<2, PLANES> mul(p, smem_u32(ring));
       uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
@@ -792,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   cluster_sync();
-  if (warp == kEpiWarps) {
+  if (warp == EPI) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
@@ -863,6 +904,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   float* partial = reinterpret_cast<float*>(ring);  // this CTA's sums of the tile, once the ring is free
 
   if (warp < EPI) {
+    for (int col = group * 32; col < p.BN; col += GROUPS * 32) prefetch_res(p, o.b, o.i + quad * 32 + lane, o.j + col);
     bool ok = true;
     if (p.inject && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, limit, &g_gemm_fault));
     float acc[SLICES][32];
@@ -943,7 +985,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   // each CTA of the cluster finishes its share of the rows
   const int nrows = BM / split, r0 = rank * nrows;
   const Block mine{o.b, o.i + r0, o.j, partial + r0 * pitch, pitch, 31 - __clz(nrows), 31 - __clz(p.BN)};
-  finish<OUT, true>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
+  finish<OUT, true, 2>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
   __syncwarp();
   if (split > 1) cluster_sync();  // peers' sums stay until they have been read
   __syncthreads();
@@ -1020,17 +1062,18 @@ cudaError_t launch_in_clusters(Kern kern, int64_t ctas, int cluster, int threads
 
 template <int PLANES, typename OUT>
 cudaError_t launch_pair(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
-  const int staging = kEpiWarps * kStageFloats * 4;
+  constexpr int NT = Pair<PLANES>::NT;
+  const int staging = Pair<PLANES>::EPI * kStageFloats * 4;
   const int stages = (kSmemMax - 1024 - 512 - staging) / p.stage_bytes;
   p.stages = stages > kMaxStages ? kMaxStages : stages;
   const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + staging;
   auto kern = gemm_pair_kernel<PLANES, OUT>;
   static int cache[64];
   int occ = 0;
-  cudaError_t e = kernel_occupancy(kern, kThreads, smem, cache, &occ);
+  cudaError_t e = kernel_occupancy(kern, NT, smem, cache, &occ);
   if (e != cudaSuccess) return e;
   const int64_t want = p.tiles * 2, cap = sms / 2 * 2;
-  return launch_in_clusters(kern, want < cap ? want : cap, 2, kThreads, smem, s, mp, mq, p);
+  return launch_in_clusters(kern, want < cap ? want : cap, 2, NT, smem, s, mp, mq, p);
 }
 
 template <int PLANES, typename OUT>
