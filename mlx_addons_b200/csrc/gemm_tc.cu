@@ -68,7 +68,7 @@ struct TcParams {
   TcPolar polar;
   int res_kind, y_vec, pre_vec, res_vec, bias_vec;
   int64_t y_plane, res_plane;
-  int inject;
+  int inject, chained;
 };
 
 // ---------------------------------------------------------------------------
@@ -436,8 +436,8 @@ __device__ __forceinline__ void addends8(float (&x)[8], const TcParams& p, int64
     load_res8(x, p, b * e.res.bs + i * e.res.is + j * e.res.js, ALONG_I ? e.res.is : e.res.js, n, n == 8 && p.res_vec);
 }
 
-// The sums v and addends x of n (up to 8) neighbours from (i, j) along the
-// axis that has unit stride in y and pre: i (ALONG_I) or j.
+// The sums v (results on return) and addends x of n (up to 8) neighbours from
+// (i, j) along the axis that has unit stride in y and pre: i (ALONG_I) or j.
 template <typename OUT, bool ALONG_I>
 __device__ __forceinline__ void finish8(const TcParams& p, int64_t b, int64_t i, int64_t j, int n, float (&v)[8],
                                         const float (&x)[8]) {
@@ -464,9 +464,10 @@ __device__ __forceinline__ void finish8(const TcParams& p, int64_t b, int64_t i,
   T* y = static_cast<T*>(e.y.p) + b * e.y.bs + i * e.y.is + j * e.y.js;
   store8(y, v, n, whole && p.y_vec);
   if constexpr (std::is_same<OUT, Halves>::value) {
+    float lo[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] -= __half2float(__float2half_rn(v[k]));
-    store8(y + p.y_plane, v, n, whole && p.y_vec);
+    for (int k = 0; k < 8; ++k) lo[k] = v[k] - __half2float(__float2half_rn(v[k]));
+    store8(y + p.y_plane, lo, n, whole && p.y_vec);
   }
 }
 
@@ -512,20 +513,16 @@ __device__ __forceinline__ void joined8(const float* at, int step, int split, fl
 // A block of sums: 2^lg_rows x 2^lg_cols of them, from row i and column j of D.
 struct Block {
   int64_t b, i, j;
-  const float* sums;
+  float* sums;
   int pitch, lg_rows, lg_cols;
 };
 
-// Units of 8 of a block: along the rows of the sums, along their columns, or
-// along their columns as rows of the transpose.
-enum FinishMode { kRowUnits, kColUnits, kMirrorUnits };
-
-// Threads t0, t0 + nt, ... take a block's units, BATCH at a time: their addends
-// are asked for together, since each is a trip to memory.
-template <typename OUT, bool CLUSTER, int BATCH, int MODE>
-__device__ __forceinline__ void finish_units(const TcParams& p, const Block& o, int t0, int nt) {
-  constexpr bool ALONG_I = MODE == kColUnits;
-  const int total = 1 << (o.lg_rows + o.lg_cols - 3), lg = (MODE == kRowUnits ? o.lg_cols : o.lg_rows) - 3;
+// Threads t0, t0 + nt, ... take a block's units of 8 neighbours along the axis
+// of unit stride in y (i with ALONG_I), BATCH at a time: their addends are asked
+// for together, since each is a trip to memory. With KEEP the results replace the sums.
+template <typename OUT, bool CLUSTER, int BATCH, bool ALONG_I>
+__device__ __forceinline__ void finish_units(const TcParams& p, const Block& o, bool keep, int t0, int nt) {
+  const int total = 1 << (o.lg_rows + o.lg_cols - 3), lg = (ALONG_I ? o.lg_rows : o.lg_cols) - 3;
   const int64_t end_i = p.I, end_j = p.J;
 #pragma unroll 1
   for (int u0 = t0; u0 < total; u0 += nt * BATCH) {
@@ -533,33 +530,61 @@ __device__ __forceinline__ void finish_units(const TcParams& p, const Block& o, 
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
       const int u = u0 + q * nt, across = u >> lg, along = (u & ((1 << lg) - 1)) * 8;
-      const int64_t i = MODE == kRowUnits ? o.i + across : MODE == kColUnits ? o.i + along : o.j + across;
-      const int64_t j = MODE == kRowUnits ? o.j + along : MODE == kColUnits ? o.j + across : o.i + along;
+      const int64_t i = o.i + (ALONG_I ? along : across), j = o.j + (ALONG_I ? across : along);
       const int64_t left = ALONG_I ? end_i - i : end_j - j;
       if (u < total && i < end_i && j < end_j) addends8<ALONG_I>(x[q], p, o.b, i, j, left < 8 ? (int)left : 8);
     }
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
       const int u = u0 + q * nt, across = u >> lg, along = (u & ((1 << lg) - 1)) * 8;
-      const int64_t i = MODE == kRowUnits ? o.i + across : MODE == kColUnits ? o.i + along : o.j + across;
-      const int64_t j = MODE == kRowUnits ? o.j + along : MODE == kColUnits ? o.j + across : o.i + along;
+      const int64_t i = o.i + (ALONG_I ? along : across), j = o.j + (ALONG_I ? across : along);
       const int64_t left = ALONG_I ? end_i - i : end_j - j;
       if (u >= total || i >= end_i || j >= end_j) continue;
-      const int r = MODE == kRowUnits ? across : along, c = MODE == kRowUnits ? along : across;
+      float* at = o.sums + (ALONG_I ? along : across) * o.pitch + (ALONG_I ? across : along);
       float v[8];
-      joined8<CLUSTER>(o.sums + r * o.pitch + c, MODE == kRowUnits ? 1 : o.pitch, p.split, v);
+      joined8<CLUSTER>(at, ALONG_I ? o.pitch : 1, p.split, v);
       finish8<OUT, ALONG_I>(p, o.b, i, j, left < 8 ? (int)left : 8, v, x[q]);
+      if (keep) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) at[k * (ALONG_I ? o.pitch : 1)] = v[k];
+      }
     }
   }
 }
 
-// Thread t0 of nt finishes its share of the block. With mirror the block is
-// also written as its transpose (the other half of a symmetric product).
+// Writes a finished block's results once more, as its transpose: the other
+// half of a symmetric product. Lanes run along 16 columns and two units of rows, so
+// that shared memory is read without conflicts and stores fill 32-byte sectors.
+template <typename OUT>
+__device__ __forceinline__ void mirror_units(const TcParams& p, const Block& o, int t0, int nt) {
+  typedef typename OutOf<OUT>::T T;
+  const int total = 1 << (o.lg_rows + o.lg_cols - 3);
+#pragma unroll 1
+  for (int u = t0; u < total; u += nt) {
+    const int c = (u & 15) | (u >> 5 << 4 & ((1 << o.lg_cols) - 1));
+    const int r = ((u >> 4 & 1) | (u >> (o.lg_cols + 1) << 1)) * 8;
+    const int64_t i = o.j + c, j = o.i + r;
+    if (i >= p.I || j >= p.J) continue;
+    const int n = p.J - j < 8 ? (int)(p.J - j) : 8;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = o.sums[(r + k) * o.pitch + c];
+    T* y = static_cast<T*>(p.e.y.p) + o.b * p.e.y.bs + i * p.e.y.is + j;
+    store8(y, v, n, n == 8 && p.y_vec);
+    if constexpr (std::is_same<OUT, Halves>::value) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] -= __half2float(__float2half_rn(v[k]));
+      store8(y + p.y_plane, v, n, n == 8 && p.y_vec);
+    }
+  }
+}
+
+// Thread t0 of nt finishes its share of the block; with keep, for
+// mirror_units, which needs a barrier in between.
 template <typename OUT, bool CLUSTER, int BATCH>
-__device__ __forceinline__ void finish(const TcParams& p, const Block& o, bool mirror, int t0, int nt) {
-  if (p.e.y.js == 1) finish_units<OUT, CLUSTER, BATCH, kRowUnits>(p, o, t0, nt);
-  else finish_units<OUT, CLUSTER, BATCH, kColUnits>(p, o, t0, nt);
-  if (mirror) finish_units<OUT, CLUSTER, BATCH, kMirrorUnits>(p, o, t0, nt);
+__device__ __forceinline__ void finish(const TcParams& p, const Block& o, bool keep, int t0, int nt) {
+  if (p.e.y.js == 1) finish_units<OUT, CLUSTER, BATCH, false>(p, o, keep, t0, nt);
+  else finish_units<OUT, CLUSTER, BATCH, true>(p, o, keep, t0, nt);
 }
 
 // Asks for 32 addends of a row, to be in L2 when the epilogue reads them: a
@@ -584,8 +609,13 @@ __device__ __forceinline__ void finish32(const TcParams& p, const float (&v)[32]
 #pragma unroll
   for (int c = 0; c < 32; ++c) stage[lane * kStagePitch + c] = v[c];
   __syncwarp();
-  finish<OUT, false, 1>(p, Block{b, i, j, stage, kStagePitch, 5, 5}, mirror, lane, 32);
+  const Block o{b, i, j, stage, kStagePitch, 5, 5};
+  finish<OUT, false, 1>(p, o, mirror, lane, 32);
   __syncwarp();
+  if (mirror) {
+    mirror_units<OUT>(p, o, lane, 32);
+    __syncwarp();
+  }
 }
 
 __device__ __forceinline__ int clamp32(int64_t n) { return n > 32 ? 32 : (int)n; }
@@ -679,6 +709,7 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ TcParams p) {
   extern __shared__ unsigned char raw[];
+  next_may_launch();
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
@@ -714,6 +745,7 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
   cluster_sync();
   fence_after();
   const uint32_t tmem = tmem_slot;
+  previous_done();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
   volatile int* gu = &gave_up;
   const int per = JOIN ? 1 : p.kblocks;  // slices of one accumulator
@@ -859,6 +891,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
     gemm_solo_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ TcParams p) {
   extern __shared__ unsigned char raw[];
+  next_may_launch();
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
@@ -897,6 +930,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
+  previous_done();
   volatile int* gu = &gave_up;
   const int quad = warp & 3, group = warp >> 2;
   const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -986,6 +1020,10 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   const int nrows = BM / split, r0 = rank * nrows;
   const Block mine{o.b, o.i + r0, o.j, partial + r0 * pitch, pitch, 31 - __clz(nrows), 31 - __clz(p.BN)};
   finish<OUT, true, 2>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
+  if (o.mirror) {
+    __syncthreads();
+    mirror_units<OUT>(p, mine, tid, Solo<PLANES>::NT);
+  }
   __syncwarp();
   if (split > 1) cluster_sync();  // peers' sums stay until they have been read
   __syncthreads();
@@ -1051,12 +1089,21 @@ cudaError_t launch_in_clusters(Kern kern, int64_t ctas, int cluster, int threads
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (p.chained) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, mp, mq, p);
 }
 
@@ -1232,6 +1279,7 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   p.res_vec = vec16(t.e.res, along_i, rsize, t.res_plane);
   p.bias_vec = (reinterpret_cast<uintptr_t>(t.e.bias) & 15) == 0;
   p.inject = inject_timeout();
+  p.chained = t.chained;
   CUtensorMap mp, mq;
   if (!encode(&mp, t.P, t.f16, planes, t.batch, t.I, t.K, BM) ||
       !encode(&mq, t.Q, t.f16, planes, t.batch, t.J, t.K, p.share))

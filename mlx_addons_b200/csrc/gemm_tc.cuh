@@ -51,6 +51,7 @@ struct TcProblem {
   int res;               // the type of e.res, or kOutHalves
   int64_t y_plane, res_plane;  // plane strides, elements, where kOutHalves
   TcPolar polar;
+  int chained;           // follows a kernel of the same chain: may be set up while that one ends
   int sym;               // D is symmetric (P and Q the same, or commuting symmetric): compute the lower tiles, mirror them
 };
 constexpr int kOutHalves = 3;

@@ -191,6 +191,7 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   TcProblem t{};
   t.kind = kTwo ? kHalves : kOne;
   t.f16 = 1;
+  t.chained = 1;
   t.batch = p.batch;
   const int bcast = p.batch == 1;
   const int64_t sx = side * l.pitch_s, xx = p.m * l.pitch_x;
