@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   // each CTA of the cluster finishes its share of the rows
   const int nrows = BM / split, r0 = rank * nrows;
   const Block mine{o.b, o.i + r0, o.j, partial + r0 * pitch, pitch, 31 - __clz(nrows), 31 - __clz(p.BN)};
-  finish<OUT, true, 2>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
+  finish<OUT, true, 1>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
   if (o.mirror) {
     __syncthreads();
     mirror_units<OUT>(p, mine, tid, Solo<PLANES>::NT);
