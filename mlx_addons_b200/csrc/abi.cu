@@ -112,6 +112,7 @@ int b2c_take_device_fault(unsigned int* fault) {
   if (e == cudaSuccess) e = b2c::dag_take_fault(fault);
   if (e == cudaSuccess) e = b2c::gemm_take_fault(fault);
   if (e == cudaSuccess) e = b2c::polar_take_fault(fault);
+  if (e == cudaSuccess) e = b2c::polar_grid_take_fault(fault);
   if (e != cudaSuccess) return cuda_fail(e, "b2c_take_device_fault");
   return ok();
 }

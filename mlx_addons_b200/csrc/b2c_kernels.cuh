@@ -50,6 +50,8 @@ cudaError_t blocked_take_fault(unsigned int* fault);
 cudaError_t gemm_take_fault(unsigned int* fault);
 // Reads and clears the small orthogonalisation's fault flag. polar_cta.cu
 cudaError_t polar_take_fault(unsigned int* fault);
+// The same of the grid-wide orthogonalisation. polar_grid.cu
+cudaError_t polar_grid_take_fault(unsigned int* fault);
 cudaError_t launch_posv_blocked2(const PosvParams& p, int grid, cudaStream_t s);
 
 // Triangular solves, any k. posv_blocked.cu

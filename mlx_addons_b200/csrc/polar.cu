@@ -74,7 +74,8 @@ __device__ __forceinline__ void load_unit(const PolarIn& in, const T* row, int64
 // float32 neither overflow nor vanish there. Bound by HBM (2 or 4 bytes an
 // element; the 64-bit additions take about as long).
 template <typename T>
-__global__ void __launch_bounds__(kNormThreads) polar_norm_kernel(const PolarIn in, double* part) {
+__global__ void __launch_bounds__(kNormThreads) polar_norm_kernel(const PolarIn in, double* part, unsigned int* counter) {
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *counter = 0;
   __shared__ double red[kNormThreads / 32];
   for (int64_t b = blockIdx.y; b < in.batch; b += gridDim.y) {
     const T* base = static_cast<const T*>(in.G) + b * in.bs;
@@ -158,7 +159,7 @@ PolarLayout polar_layout(const PolarParams& p) {
 }
 
 template <typename T>
-cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
+cudaError_t launch_t(const PolarParams& p, int sms, cudaStream_t s) {
   const PolarLayout l = polar_layout(p);
   const int64_t mn = p.m * p.n, side = l.side;
   char* w = static_cast<char*>(p.ws);
@@ -173,6 +174,7 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   float* ds = reinterpret_cast<float*>(w);  // diagonals of S and P
   float* dp = reinterpret_cast<float*>(w + l.vec_bytes);
   float* r = reinterpret_cast<float*>(w + 2 * l.vec_bytes);
+  unsigned int* counter = reinterpret_cast<unsigned int*>(w + 3 * l.vec_bytes);
   const PolarIn in{p.G, p.bs, p.rs, p.cs, p.batch, p.m, p.n,
                    (reinterpret_cast<uintptr_t>(p.G) & 15) == 0 && p.cs == 1 && p.rs % PER == 0 && p.bs % PER == 0};
   const int64_t units = p.m * ((p.n + 7) / 8);
@@ -180,12 +182,15 @@ cudaError_t launch_t(const PolarParams& p, cudaStream_t s) {
   if (blocks > kNormParts) blocks = kNormParts;
   const int parts = (int)blocks;
   const dim3 grid((unsigned)blocks, (unsigned)(p.batch < 65535 ? p.batch : 65535));
-  polar_norm_kernel<T><<<grid, kNormThreads, 0, s>>>(in, part);
+  polar_norm_kernel<T><<<grid, kNormThreads, 0, s>>>(in, part, counter);
   constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;
   polar_scale_kernel<T, kTwo><<<grid, kNormThreads, 0, s>>>(in, part, parts, p.eps, X0, l.pitch_x, l.x_plane, r);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
 
+  if (polar_grid_fits(p, sms))
+    return launch_polar_grid(p, PolarScratch{side, l.pitch_x, l.pitch_s, l.x_plane, l.s_plane, X0, X1, S, P, ds, dp, r, counter},
+                             sms, s);
   const bool wide = p.m <= p.n;
   const int inner = kTwo ? kOutHalves : B2C_F16;
   TcProblem t{};
@@ -288,20 +293,19 @@ size_t polar_ws_bytes(const PolarParams& in) {
   const PolarParams p = along_rows(in);
   if (polar_cta_fits(p)) return 0;
   const PolarLayout l = polar_layout(p);
-  return (size_t)(l.part_bytes + 2 * l.x_bytes + 2 * l.s_bytes + 3 * l.vec_bytes);
+  return (size_t)(l.part_bytes + 2 * l.x_bytes + 2 * l.s_bytes + 3 * l.vec_bytes + 256);
 }
 
 cudaError_t launch_polar(const PolarParams& in, cudaStream_t s) {
   const PolarParams p = along_rows(in);
-  if (polar_cta_fits(p)) {
-    int sms = 0;
-    const cudaError_t e = device_sms(&sms);
-    return e == cudaSuccess ? launch_polar_cta(p, sms, s) : e;
-  }
+  int sms = 0;
+  const cudaError_t e = device_sms(&sms);
+  if (e != cudaSuccess) return e;
+  if (polar_cta_fits(p)) return launch_polar_cta(p, sms, s);
   switch (p.dtype) {
-    case B2C_F32: return launch_t<float>(p, s);
-    case B2C_BF16: return launch_t<__nv_bfloat16>(p, s);
-    default: return launch_t<__half>(p, s);
+    case B2C_F32: return launch_t<float>(p, sms, s);
+    case B2C_BF16: return launch_t<__nv_bfloat16>(p, sms, s);
+    default: return launch_t<__half>(p, sms, s);
   }
 }
 

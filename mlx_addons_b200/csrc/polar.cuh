@@ -35,6 +35,16 @@ __device__ __forceinline__ PolarNorm polar_norm(double norm) {
   return PolarNorm{scalbn(16384.0, -q), (float)(1.0 / f), 14 - q};
 }
 
+// Scratch of the forms that keep X, S and P in memory (polar.cu).
+struct PolarScratch {
+  int64_t side, pitch_x, pitch_s, x_plane, s_plane;
+  __half *X0, *X1, *S, *P;  // X0 holds G, scaled
+  float *ds, *dp, *r;       // diagonals of S and P, (batch, side); the first step's factors, (batch,)
+  unsigned int* counter;    // zero
+};
+bool polar_grid_fits(const PolarParams& p, int sms);
+cudaError_t launch_polar_grid(const PolarParams& p, const PolarScratch& w, int sms, cudaStream_t s);
+
 // Both take a problem whose rows lie no closer together than its columns.
 bool polar_cta_fits(const PolarParams& p);
 cudaError_t launch_polar_cta(const PolarParams& p, int sms, cudaStream_t s);

@@ -183,6 +183,38 @@ def test_batches_that_share_a_tile(batch, m, n, dtype):
     assert torch.equal(out2[keep], out[keep]) and bool(torch.isnan(out2[~keep]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 129, 129), (1, 256, 256), (1, 1000, 517), (3, 517, 1000), (2, 130, 1500), (1, 700, 2000),
+                                   (5, 384, 384), (1, 2048, 640), (40, 200, 260), (300, 140, 136), (2, 2100, 2300)])
+def test_middle_sizes(shape, dtype):
+    """The sizes between one CTA's shared memory and the largest, on both sides of each border."""
+    G = _grad_like(shape, dtype, seed=sum(shape))
+    out = la.orthogonalize(G)
+    if dtype == F32:  # 64-bit values of the large ones once
+        _check(out, G)
+    else:
+        ref, its = orth64(G)
+        err, bound = torch.linalg.matrix_norm(out.double() - ref), orth_bound(its, 5, MUON, UNIT[dtype], dtype)
+        assert bool((err <= bound).all()), float((err / bound).max())
+    again = la.orthogonalize(G)
+    assert torch.equal(out, again)
+
+
+def test_two_streams_at_once():
+    """Calls that need every SM together, side by side on two streams."""
+    G = [_grad_like((3, 300 + 50 * i, 500), F32, seed=i) for i in range(2)]
+    want = [la.orthogonalize(g) for g in G]
+    streams = [torch.cuda.Stream() for _ in G]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(la.orthogonalize(G[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
 def test_host_inputs_and_empty():
     G = _grad_like((3, 20, 30), F32, seed=12)
     want = la.orthogonalize(G).cpu()
