@@ -154,7 +154,7 @@ PolarLayout polar_layout(const PolarParams& p) {
   l.x_bytes = (l.x_plane * l.planes * 2 + 255) / 256 * 256;
   l.s_bytes = (l.s_plane * l.planes * 2 + 255) / 256 * 256;
   l.part_bytes = (p.batch * kNormParts * (int64_t)sizeof(double) + 255) / 256 * 256;
-  l.vec_bytes = (p.batch * l.side * (int64_t)sizeof(float) + 255) / 256 * 256;
+  l.vec_bytes = (p.batch * l.pitch_s * (int64_t)sizeof(float) + 255) / 256 * 256;
   return l;
 }
 
@@ -218,7 +218,7 @@ cudaError_t launch_t(const PolarParams& p, int sms, cudaStream_t s) {
     t.polar.mode = kPolarS;
     t.polar.r = step ? nullptr : r;
     t.polar.d_in = t.polar.d_out = ds;
-    t.polar.side = side;
+    t.polar.side = l.pitch_s;
     t.polar.k = 1.f / ss;
     t.out = t.res = inner;
     t.y_plane = t.res_plane = l.s_plane;

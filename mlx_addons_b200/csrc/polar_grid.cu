@@ -61,51 +61,27 @@ struct GridMaps {
   CUtensorMap x_p[2], x_q[2];  // X' = P X or X P
 };
 
-// What the epilogue of a product needs, in shared memory.
+// What the general epilogue needs for the last product, whose outputs have the
+// caller's type and layout.
 template <int PLANES>
-__device__ __forceinline__ void set_phase(TcParams& c, const GridParams& p, int step, int ph) {
-  const GridStep& k = p.step[step];
-  const GridPhase& g = p.phase[ph];
-  const int inner = PLANES == 2 ? kOutHalves : B2C_F16, cur = step & 1;
-  const bool last = ph == 2 && step == p.steps - 1;
+__device__ __forceinline__ void set_last(TcParams& c, const GridParams& p) {
+  const GridStep& k = p.step[p.steps - 1];
+  const int inner = PLANES == 2 ? kOutHalves : B2C_F16, cur = (p.steps - 1) & 1;
   c = TcParams{};
-  c.I = g.I, c.J = g.J;
-  c.tiles = g.tiles, c.tiles_i = g.tiles_i, c.tiles_j = g.tiles_j;
-  c.BN = g.BN, c.sym = g.sym, c.band = 8;
+  c.I = p.phase[2].I, c.J = p.phase[2].J;
   c.split = 1;
   c.res_kind = inner;
-  c.y_vec = c.res_vec = 1;
-  c.polar.side = p.side;
-  c.polar.r = step ? nullptr : p.r;
-  if (ph == 0) {
-    c.e.y = GemmView{p.S, p.ss, p.pitch_s, 1};
-    c.e.alpha = k.s_alpha;
-    c.polar.mode = kPolarS;
-    c.polar.d_in = c.polar.d_out = p.ds;
-    c.polar.k = k.s_k;
-    c.y_plane = p.s_plane;
-  } else if (ph == 1) {
-    c.e.y = GemmView{p.P, p.ss, p.pitch_s, 1};
-    c.e.res = GemmView{p.S, p.ss, p.pitch_s, 1};
-    c.e.alpha = k.p_alpha, c.e.beta = k.p_beta;
-    c.polar.mode = kPolarP;
-    c.polar.r = nullptr;
-    c.polar.d_in = p.ds, c.polar.d_out = p.dp;
-    c.polar.k = k.p_k, c.polar.k2 = k.p_k2, c.polar.k3 = k.p_k3, c.polar.k4 = k.p_k4;
-    c.y_plane = c.res_plane = p.s_plane;
-  } else {
-    c.e.y = last ? GemmView{p.out, p.mn, p.out_rs, p.out_cs} : GemmView{p.X[cur ^ 1], p.xx, p.pitch_x, 1};
-    c.e.res = GemmView{p.X[cur], p.xx, p.pitch_x, 1};
-    c.e.alpha = k.x_alpha, c.e.beta = k.x_beta;
-    c.polar.mode = p.wide ? kPolarXi : kPolarXj;
-    c.polar.d_in = p.dp, c.polar.d_out = p.dp;
-    c.polar.k = k.x_k;
-    c.y_plane = c.res_plane = p.x_plane;
-    if (last) {
-      c.y_vec = p.last_vec;
-      c.res_vec = p.out_cs == 1;
-    }
-  }
+  c.y_vec = p.last_vec;
+  c.res_vec = p.out_cs == 1;
+  c.e.y = GemmView{p.out, p.mn, p.out_rs, p.out_cs};
+  c.e.res = GemmView{p.X[cur], p.xx, p.pitch_x, 1};
+  c.res_plane = p.x_plane;
+  c.e.alpha = k.x_alpha, c.e.beta = k.x_beta;
+  c.polar.mode = p.wide ? kPolarXi : kPolarXj;
+  c.polar.r = p.steps > 1 ? nullptr : p.r;
+  c.polar.d_in = c.polar.d_out = p.dp;
+  c.polar.side = p.pitch_s;
+  c.polar.k = k.x_k;
 }
 
 // The tile order of a phase alone.
@@ -129,10 +105,117 @@ __device__ __forceinline__ bool epi_any(bool x) {
   return r != 0;
 }
 
+template <int PLANES>
+__device__ __forceinline__ void load_x(float (&x)[8], const __half* at, int64_t plane) {
+  const uint4 h = *reinterpret_cast<const uint4*>(at);
+  const __half2* q = reinterpret_cast<const __half2*>(&h);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = __half22float2(q[k]);
+    x[2 * k] = f.x, x[2 * k + 1] = f.y;
+  }
+  if constexpr (PLANES == 2) {
+    const uint4 l = *reinterpret_cast<const uint4*>(at + plane);
+    const __half2* m = reinterpret_cast<const __half2*>(&l);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __half22float2(m[k]);
+      x[2 * k] += f.x, x[2 * k + 1] += f.y;
+    }
+  }
+}
+
+template <int PLANES>
+__device__ __forceinline__ void store_x(const float (&v)[8], __half* at, int64_t plane) {
+  __align__(16) __half2 h[4], l[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+    if constexpr (PLANES == 2) {
+      const float2 f = __half22float2(h[k]);
+      l[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
+    }
+  }
+  *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(h);
+  if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(at + plane) = *reinterpret_cast<const uint4*>(l);
+}
+
+// The epilogue of a 32 x 32 block of S, P or an X that is not the last: the
+// formulas of TcPolarMode. Everything that it reads from memory is asked for at
+// once, before anything else, and rows are padded to units of 8, which needs no
+// edges inside a unit (the general epilogue took 5,000 clocks a block, this one 1,500).
+template <int PLANES>
+__device__ __forceinline__ void polar_block(const GridParams& p, const GridStep& k, int ph, int x, float f, const float (&acc)[32],
+                                            int64_t b, int64_t i, int64_t j, bool mirror, float* stage, int lane) {
+  const int64_t I = p.phase[ph].I, J = p.phase[ph].J;
+  const int c8 = (lane & 3) * 8, r0 = lane >> 2;
+  const int64_t pitch = ph == 2 ? p.pitch_x : p.pitch_s, plane = ph == 2 ? p.x_plane : p.s_plane;
+  __half* y = ph == 0 ? p.S + b * p.ss : ph == 1 ? p.P + b * p.ss : p.X[x ^ 1] + b * p.xx;
+  const __half* res = ph == 1 ? p.S + b * p.ss : p.X[x] + b * p.xx;
+  const float* d = (ph == 1 ? p.ds : p.dp) + b * p.pitch_s;
+  const bool cols = j + c8 < J, by_row = ph == 1 || p.wide, by_col = ph == 1 || !p.wide;
+  float xr[4][8], di[4] = {}, dj[8] = {};
+  if (ph) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (cols && i + r0 + 8 * t < I) {
+        load_x<PLANES>(xr[t], res + (i + r0 + 8 * t) * pitch + j + c8, plane);
+        if (by_row) di[t] = d[i + r0 + 8 * t];
+      }
+    if (by_col && cols) {
+      const float4 a = *reinterpret_cast<const float4*>(d + j + c8), c = *reinterpret_cast<const float4*>(d + j + c8 + 4);
+      dj[0] = a.x, dj[1] = a.y, dj[2] = a.z, dj[3] = a.w, dj[4] = c.x, dj[5] = c.y, dj[6] = c.z, dj[7] = c.w;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 32; ++c) stage[lane * kStagePitch + c] = acc[c];
+  __syncwarp();
+  float* d_out = (ph == 0 ? p.ds : p.dp) + b * p.pitch_s;
+  const float alpha = ph == 0 ? k.s_alpha * f * f : ph == 1 ? k.p_alpha : f * k.x_alpha;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int r = r0 + 8 * t;
+    float* at = stage + r * kStagePitch + c8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = at[e] * alpha;
+    if (ph < 2) {
+      float w = 0.f;  // this row's diagonal element, where it is among the eight
+      const int here = i == j ? r - c8 : -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        w = e == here ? v[e] : w;
+        if (ph == 1) v[e] = fmaf(fmaf(k.p_k, di[t] + dj[e], k.p_beta), xr[t][e], v[e]);
+        v[e] = e == here ? 0.f : v[e];
+      }
+      if (here >= 0 && here < 8 && i + r < I)
+        d_out[i + r] = ph == 0 ? w * k.s_k : fmaf(k.p_k2, w, di[t] * fmaf(k.p_k3, di[t], k.p_k4));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(f * k.x_beta * (k.x_k + di[t] + dj[e]), xr[t][e], v[e]);
+    }
+    if (cols && i + r < I) store_x<PLANES>(v, y + (i + r) * pitch + j + c8, plane);
+    if (mirror) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) at[e] = v[e];
+    }
+  }
+  __syncwarp();
+  if (!mirror) return;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int c = r0 + 8 * t;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = stage[(c8 + e) * kStagePitch + c];
+    if (j + c < I && i + c8 < J) store_x<PLANES>(v, y + (j + c) * pitch + i + c8, plane);
+  }
+  __syncwarp();
+}
+
 template <int PLANES, typename T>
 __global__ void __launch_bounds__(kThreadsG, 1)
     polar_grid_kernel(const __grid_constant__ GridMaps maps, const __grid_constant__ GridParams p) {
-  typedef typename std::conditional<PLANES == 2, Halves, __half>::type Inner;
   constexpr bool JOIN = PLANES > 1;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 6];
@@ -180,13 +263,12 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     if (p.inject && blockIdx.x == 0) bar_wait(never, 0, gu, limit, &g_grid_fault);
     for (int f = 0; f < phases; ++f) {
       const int st = f / 3, ph = f - 3 * st;
-      epi_sync();  // the phase before is done with cur
-      if (tid == 0) set_phase<PLANES>(cur, p, st, ph);
+      if (f == phases - 1 && tid == 0) set_last<PLANES>(cur, p);
       if (epi_any(*gu != 0)) break;
       const int kblocks = p.phase[ph].kblocks, BN = p.phase[ph].BN;
       const bool last = f == phases - 1;
-      for (int64_t t = blockIdx.x; t < cur.tiles; t += gridDim.x) {
-        const Tile o = tile_at<1>(cur, t);
+      for (int64_t t = blockIdx.x; t < p.phase[ph].tiles; t += gridDim.x) {
+        const Tile o = phase_tile(p.phase[ph], t);
         float acc[2][32];
         bool ok = true;
         for (int kb = 0; kb < (JOIN ? kblocks : 1); ++kb) {
@@ -213,7 +295,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         for (int q = 0; q < BN / 64; ++q) {
           const int64_t i = o.i + quad * 32, j = o.j + (2 * q + group) * 32;
           if (last) finish32<T>(cur, acc[0], o.b, i, j, o.mirror, stage, lane);
-          else finish32<Inner>(cur, acc[0], o.b, i, j, o.mirror, stage, lane);
+          else polar_block<PLANES>(p, p.step[st], ph, st & 1, st ? 1.f : p.r[o.b], acc[0], o.b, i, j, o.mirror, stage, lane);
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[0][c] = acc[1][c];
         }
