@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
     }
   } else {
     if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Pair<PLANES>::FEW));
-    if (warp == EPI && lane == 0) {
+    if (warp == EPI) {
       // ---- loads ----
+      const bool lead = elect_one();
       const uint32_t lead_full0 = map_rank(full0, 0);
       uint32_t s = 0, phase = 0;
       for (int64_t t = first; t < p.tiles && !*gu; t += step) {
@@ -182,13 +183,16 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
         const int bp = p.p_bcast ? 0 : (int)o.b, bq = p.q_bcast ? 0 : (int)o.b;
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_gemm_fault)) break;
-          if (rank == 0) bar_expect(full0 + 8 * s, 2 * p.stage_bytes);
-          load_slice<2, PLANES>(p, &map_p, &map_q, smem_u32(ring + s * p.stage_bytes), i0, j0, kb, bp, bq, lead_full0 + 8 * s);
+          if (lead) {
+            if (rank == 0) bar_expect(full0 + 8 * s, 2 * p.stage_bytes);
+            load_slice<2, PLANES>(p, &map_p, &map_q, smem_u32(ring + s * p.stage_bytes), i0, j0, kb, bp, bq, lead_full0 + 8 * s);
+          }
           if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
         }
       }
-    } else if (warp == EPI + 1 && rank == 0 && lane == 0) {
+    } else if (warp == EPI + 1 && rank == 0) {
       // ---- products ----
+      const bool lead = elect_one();
       const Multiplier<2, PLANES> mul(p, smem_u32(ring));
       uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
       for (int64_t t = first; t < p.tiles && !*gu; t += step) {
@@ -198,12 +202,14 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
           for (int kb = 0; kb < per; ++kb) {
             if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
             fence_after();
-            mul.slice(s, tmem + buf * 256, kb == 0);
-            commit<2>(empty0 + 8 * s);
+            if (lead) {
+              mul.slice(s, tmem + buf * 256, kb == 0);
+              commit<2>(empty0 + 8 * s);
+            }
             if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
           }
           if (*gu) break;
-          commit<2>(tfull0 + 8 * buf);
+          if (lead) commit<2>(tfull0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
       }
@@ -337,28 +343,35 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
         for (int c = 0; c < 8; ++c) at[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
       }
     }
-  } else if (warp == EPI && lane == 0) {
+  } else if (warp == EPI) {
     // ---- loads ----
+    const bool lead = elect_one();
     uint32_t s = 0, phase = 0;
     const int bp = p.p_bcast ? 0 : (int)o.b, bq = p.q_bcast ? 0 : (int)o.b;
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_gemm_fault)) break;
-      bar_expect(full0 + 8 * s, p.stage_bytes);
-      load_slice<1, PLANES>(p, &map_p, &map_q, smem_u32(ring + s * p.stage_bytes), (int)o.i, (int)o.j, kb, bp, bq, full0 + 8 * s);
+      if (lead) {
+        bar_expect(full0 + 8 * s, p.stage_bytes);
+        load_slice<1, PLANES>(p, &map_p, &map_q, smem_u32(ring + s * p.stage_bytes), (int)o.i, (int)o.j, kb, bp, bq,
+                              full0 + 8 * s);
+      }
       if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
     }
-  } else if (warp == EPI + 1 && lane == 0) {
+  } else if (warp == EPI + 1) {
     // ---- products ----
+    const bool lead = elect_one();
     const Multiplier<1, PLANES> mul(p, smem_u32(ring));
     uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       if (JOIN && !bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
       if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
       fence_after();
-      mul.slice(s, tmem + buf * p.BN, JOIN || kb == kb0);
-      commit<1>(empty0 + 8 * s);
+      if (lead) {
+        mul.slice(s, tmem + buf * p.BN, JOIN || kb == kb0);
+        commit<1>(empty0 + 8 * s);
+        if (JOIN || kb == kb1 - 1) commit<1>(tfull0 + 8 * buf);
+      }
       if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
-      if (JOIN || kb == kb1 - 1) commit<1>(tfull0 + 8 * buf);
       if (JOIN && ++buf == 2) buf = 0, tphase ^= 1;
     }
   }

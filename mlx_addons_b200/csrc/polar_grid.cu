@@ -326,8 +326,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         bar_arrive_cluster(go);
       }
     }
-  } else if (warp == kEpi && lane == 0) {
+  } else if (warp == kEpi) {
     // ---- loads ----
+    const bool lead = elect_one();
     uint32_t s = 0, phase = 0;
     for (int f = 0; f < phases && !*gu; ++f) {
       const int st = f / 3, ph = f - 3 * st, x = st & 1;
@@ -335,21 +336,25 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       const CUtensorMap* mp = ph == 0 ? &maps.s_p[x] : ph == 1 ? &maps.p_p : &maps.x_p[x];
       const CUtensorMap* mq = ph == 0 ? &maps.s_q[x] : ph == 1 ? &maps.p_q : &maps.x_q[x];
       if (f && !bar_wait(go, (f - 1) & 1, gu, 2 * kBarrierNs, &g_grid_fault)) break;
-      heard = f;
+      __syncwarp();
+      if (lead) heard = f;
       asm volatile("fence.proxy.async;" ::: "memory");
       for (int64_t t = blockIdx.x; t < g.tiles && !*gu; t += gridDim.x) {
         const Tile o = phase_tile(g, t);
         const int b = p.bcast ? 0 : (int)o.b;
         for (int kb = 0; kb < g.kblocks; ++kb) {
           if (!bar_wait(empty0 + 8 * s, phase ^ 1, gu, limit, &g_grid_fault)) break;
-          bar_expect(full0 + 8 * s, g.stage_bytes);
-          load_slice<1, PLANES>(g, mp, mq, smem_u32(ring + s * p.stage_bytes), (int)o.i, (int)o.j, kb, b, b, full0 + 8 * s);
+          if (lead) {
+            bar_expect(full0 + 8 * s, g.stage_bytes);
+            load_slice<1, PLANES>(g, mp, mq, smem_u32(ring + s * p.stage_bytes), (int)o.i, (int)o.j, kb, b, b, full0 + 8 * s);
+          }
           if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
         }
       }
     }
-  } else if (warp == kEpi + 1 && lane == 0) {
+  } else if (warp == kEpi + 1) {
     // ---- products ----
+    const bool lead = elect_one();
     uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
     for (int f = 0; f < phases && !*gu; ++f) {
       const GridPhase& g = p.phase[f % 3];
@@ -364,12 +369,14 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           for (int kb = 0; kb < per; ++kb) {
             if (!bar_wait(full0 + 8 * s, phase, gu, 2 * kBarrierNs, &g_grid_fault)) break;
             fence_after();
-            mul.slice(s, tmem + buf * 128, kb == 0);
-            commit<1>(empty0 + 8 * s);
+            if (lead) {
+              mul.slice(s, tmem + buf * 128, kb == 0);
+              commit<1>(empty0 + 8 * s);
+            }
             if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
           }
           if (*gu) break;
-          commit<1>(tfull0 + 8 * buf);
+          if (lead) commit<1>(tfull0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
       }
