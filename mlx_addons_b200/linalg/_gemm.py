@@ -41,8 +41,8 @@ def _native(x, what, name):
     return t, kind
 
 
-def _same_type(name, first, **others):
-    for what, t in others.items():
+def _same_type(name, first, *others):
+    for what, t in others:
         if t is not None and t.dtype != first.dtype:
             raise ValueError(f"{name}: {what} is {t.dtype}, expected {first.dtype}")
 
@@ -75,7 +75,7 @@ def _addr(t):
 def _call(what, fn, args, ws_fn, ws_args, dev):
     """fn(*args, workspace, bytes, stream); a call that needs scratch says so
     before it launches anything."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     rc = fn(*args, None, 0, stream)
     if rc == _lib.B2C_ERR_WORKSPACE:
         n = ws_fn(*ws_args)
@@ -157,7 +157,7 @@ def gemm(A, B, bias=None, activation: Optional[str] = None, residual=None, *, al
     bt = None if bias is None else _native(bias, "bias", name)[0]
     Rt = None if residual is None else _native(residual, "residual", name)[0]
     _check_product(At, Bt, name)
-    _same_type(name, At, B=Bt, bias=bt, residual=Rt)
+    _same_type(name, At, ("B", Bt), ("bias", bt), ("residual", Rt))
     M, N, lead, shared = At.shape[-2], Bt.shape[-1], tuple(At.shape[:-2]), Bt.dim() == 2
     if bt is not None and tuple(bt.shape) != (N,):
         raise ValueError(f"{name}: bias must have shape ({N},), got {tuple(bt.shape)}")
@@ -168,8 +168,10 @@ def gemm(A, B, bias=None, activation: Optional[str] = None, residual=None, *, al
     Y, pre = _gemm_dev(_flat(At, lead, shared), Bt if shared else _flat(Bt, lead, False),
                        None if bt is None else bt.contiguous(), act, None if Rt is None else _flat(Rt, lead, shared),
                        float(alpha), float(beta), bool(return_pre))
-    shape = lead + (M, N)
-    out = _back((Y.reshape(shape), None if pre is None else pre.reshape(shape)), kind, host)
+    if len(lead) > 1 or (lead and shared):
+        Y = Y.reshape(lead + (M, N))
+        pre = None if pre is None else pre.reshape(Y.shape)
+    out = _back((Y, pre), kind, host)
     return out if return_pre else out[0]
 
 
@@ -194,7 +196,7 @@ def gemm_grad(dY, A, B, pre=None, activation: Optional[str] = None, *, alpha: fl
     Bt, _ = _native(B, "B", name)
     pt = None if pre is None else _native(pre, "pre", name)[0]
     _check_product(At, Bt, name)
-    _same_type(name, At, B=Bt, dY=dYt, pre=pt)
+    _same_type(name, At, ("B", Bt), ("dY", dYt), ("pre", pt))
     M, K, N, lead, shared = At.shape[-2], At.shape[-1], Bt.shape[-1], tuple(At.shape[:-2]), Bt.dim() == 2
     for what, t in (("dY", dYt), ("pre", pt)):
         if t is not None and tuple(t.shape) != lead + (M, N):
@@ -225,6 +227,8 @@ def gemm_grad(dY, A, B, pre=None, activation: Optional[str] = None, *, alpha: fl
                    rows, N), lib.b2c_gemm_dact_workspace_size, (batch, rows, N), dev)
     dA, _ = _gemm_dev(dP, B3.mT, None, 0, None, float(alpha), 1.0, False)
     dB, _ = _gemm_dev(A3.mT, dP, None, 0, None, float(alpha), 1.0, False)
-    out = (dA.reshape(lead + (M, K)), dB.reshape((K, N) if shared else lead + (K, N)), dbias,
-           None if dR is None else dR.reshape(lead + (M, N)))
-    return _back(out, kind, host)
+    if len(lead) > 1 or (lead and shared):
+        dA = dA.reshape(lead + (M, K))
+        dB = dB if shared else dB.reshape(lead + (K, N))
+        dR = None if dR is None else dR.reshape(lead + (M, N))
+    return _back((dA, dB, dbias, dR), kind, host)

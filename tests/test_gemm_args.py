@@ -137,5 +137,5 @@ def test_c_orthogonalize_refuses(lib):
     assert call(coef=three(4.0, 0.0, 0.0)) == bad  # singular values up to 4
     assert b"3.5" in lib.b2c_last_error()
     assert call(coef=three(9.0, -6.0, 0.0)) == bad  # 4.24 inside [0, 1], 3 at its end
-    assert call(coef=three(1.5, -0.5, 0.0)) == _lib.B2C_ERR_WORKSPACE  # fine; and no scratch was given
+    assert call(coef=three(1.5, -0.5, 0.0), m=256, n=256) == _lib.B2C_ERR_WORKSPACE  # fine; and no scratch was given
     assert call(m=0) == _lib.B2C_OK and call(batch=0) == _lib.B2C_OK
