@@ -234,8 +234,9 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
   fence_after();
   const uint32_t tmem = tmem_slot, xa = smem_u32(X), sa = smem_u32(S);
   const uint32_t idesc_s = mma_idesc(1, 0, 0, 128, p.kk);
-  constexpr int SEGS = PLANES == 2 ? 3 : 1;
-  const int seg_p[3] = {PLANES - 1, 0, 0}, seg_q[3] = {0, PLANES - 1, 0};  // small products first
+  constexpr int SEGS = PLANES == 2 ? 3 : 1;  // lo hi, hi lo, hi hi
+  auto seg_p = [](int s) { return PLANES == 2 && s == 0 ? 1 : 0; };
+  auto seg_q = [](int s) { return s == 1 ? 1 : 0; };
   uint32_t phase = 0;
   if (p.inject && blockIdx.x == 0) bar_wait(never, 0, gu, limit, &g_polar_fault);
   auto wait = [&] {
@@ -257,16 +258,20 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     const CtaStep k = p.step[t];
     const float f1 = t ? 1.f : r0, f2 = f1 * f1, k3 = k.k3 * f2, kp = k.kp * f2;
     // ---- S = X X^T ----
-    if (tid == 0) {
-      for (int s = 0; s < SEGS; ++s)
-        for (int b = 0; b < p.xblocks; ++b)
+    if (warp == 0) {
+      if (elect_one()) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mma<1>(tmem, block_desc(xa + seg_p[s] * x_plane + b * kBlockBytes + q * 32, 0),
-                   block_desc(xa + seg_q[s] * x_plane + b * kBlockBytes + q * 32, 0), idesc_s, s + b + q > 0);
-      commit<1>(done);
+        for (int s = 0; s < SEGS; ++s) {
+          const uint64_t dp = block_desc(xa + seg_p(s) * x_plane, 0), dq = block_desc(xa + seg_q(s) * x_plane, 0);
+          for (int b = 0; b < p.xblocks; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mma<1>(tmem, dp + b * (kBlockBytes >> 4) + q * 2, dq + b * (kBlockBytes >> 4) + q * 2, idesc_s, s + b + q > 0);
+        }
+        commit<1>(done);
+      }
+      __syncwarp();  // a warp that sleeps on the barrier sleeps as a whole
     }
-    __syncwarp();  // the issuing lane first: a warp that sleeps on the barrier sleeps as a whole
     wait();
     for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
       if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
@@ -290,20 +295,24 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     __syncthreads();
     fence_after();
     // ---- P = c S S + b S ----
-    if (tid == 0) {
+    if (warp == 0) {
       // a matrix's columns of S S take its own rows of S alone: the rest are zeros
       const int width = p.blockwise ? p.side : p.kk;
       const uint32_t idesc_p = mma_idesc(1, 0, 0, 128, width);
-      for (int c0 = 0; c0 < p.kk; c0 += width)
-        for (int s = 0; s < SEGS; ++s)
-          for (int c = c0; c < c0 + width; c += 16) {
-            const int off = (c >> 6) * kBlockBytes + (c & 63) * 2;
-            mma<1>(tmem + 128 + c0, block_desc(sa + seg_p[s] * s_plane + off, 0),
-                   block_desc(sa + seg_q[s] * s_plane + off + c0 * 128, 0), idesc_p, s + (c - c0) > 0);
+      if (elect_one()) {
+        for (int c0 = 0; c0 < p.kk; c0 += width)
+#pragma unroll
+          for (int s = 0; s < SEGS; ++s) {
+            const uint64_t dp = block_desc(sa + seg_p(s) * s_plane, 0), dq = block_desc(sa + seg_q(s) * s_plane + c0 * 128, 0);
+            for (int c = c0; c < c0 + width; c += 16) {
+              const int off = (c >> 6) * (kBlockBytes >> 4) + (c & 63) / 8;
+              mma<1>(tmem + 128 + c0, dp + off, dq + off, idesc_p, s + (c - c0) > 0);
+            }
           }
-      commit<1>(done);
+        commit<1>(done);
+      }
+      __syncwarp();
     }
-    __syncwarp();  // the issuing lane first: a warp that sleeps on the barrier sleeps as a whole
     wait();
     const float di = kSplitDiag && row < p.kk ? sdiag[row] : 0.f;
     for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
@@ -338,15 +347,20 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     // ---- X <- P X + a X, up to 256 columns at a time ----
     for (int b0 = 0; b0 < p.xblocks; b0 += 4) {
       const int nb = min(4, p.xblocks - b0);
-      if (tid == 0) {
+      if (warp == 0) {
         const uint32_t idesc_x = mma_idesc(1, 0, 1, 128, nb * 64);
-        for (int s = 0; s < SEGS; ++s)
-          for (int q = 0; q < p.kk / 16; ++q)
-            mma<1>(tmem, block_desc(sa + seg_p[s] * s_plane + (q >> 2) * kBlockBytes + (q & 3) * 32, 0),
-                   block_desc(xa + seg_q[s] * x_plane + b0 * kBlockBytes + q * 2048, 1), idesc_x, s + q > 0);
-        commit<1>(done);
+        if (elect_one()) {
+#pragma unroll
+          for (int s = 0; s < SEGS; ++s) {
+            const uint64_t dp = block_desc(sa + seg_p(s) * s_plane, 0),
+                           dq = block_desc(xa + seg_q(s) * x_plane + b0 * kBlockBytes, 1);
+            for (int q = 0; q < p.kk / 16; ++q)
+              mma<1>(tmem, dp + (q >> 2) * (kBlockBytes >> 4) + (q & 3) * 2, dq + q * (2048 >> 4), idesc_x, s + q > 0);
+          }
+          commit<1>(done);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       wait();
       for (int c0 = group * 32; c0 < nb * 64; c0 += NG * 32) {
         float v[32];
