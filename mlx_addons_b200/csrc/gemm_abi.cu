@@ -55,7 +55,18 @@ struct GemmChoice {
 GemmChoice choose(const GemmProblem& in) {
   GemmChoice c{};
   c.g = in;
-  if (in.I <= 64 && in.J > in.I) {  // the longer side takes the 128 rows of a tile
+  const double macs = (double)in.I * (double)in.J * (double)in.K * (double)in.batch;
+  const int64_t shorter = in.I < in.J ? in.I : in.J, longer = in.I < in.J ? in.J : in.I;
+  const bool f32 = in.dtype == B2C_F32;
+  // one to eight (float32: sixteen) columns: one pass over the other operand
+  const bool thin = in.K > 0 && (f32 ? shorter <= 16 : shorter <= 8 && (double)longer * in.K * in.batch <= kSkinny16);
+  // the tensor cores' set-up, and for float32 the pass that splits the operands, cost as much as this
+  // (float32, us on the FP32 units and on the tensor cores: 128 x 512 x 128 28 and 14, 256 x 256 x 256 16 and 14, 1024 x 64 x 1024 9
+  // and 12, 4096 x 64 x 4096 88 and 45)
+  const bool shallow = f32 ? in.K < 40 || (in.K < 96 && macs <= 1e8) || (in.K <= 256 && macs <= 8e6) || macs <= 1e6
+                           : in.K < 32 || macs <= 1048576.0;
+  c.tier = thin ? GemmChoice::kSkinny : shallow ? GemmChoice::kSimt : GemmChoice::kTc;
+  if (c.tier != GemmChoice::kSimt && in.I <= 64 && in.J > in.I) {  // the longer side takes the 128 rows of a tile
     GemmProblem& g = c.g;
     g.P = in.Q, g.Q = in.P;
     g.I = in.J, g.J = in.I;
@@ -65,14 +76,7 @@ GemmChoice choose(const GemmProblem& in) {
     }
     g.e.bias_on_i = !in.e.bias_on_i;
   }
-  const bool small = (double)c.g.I * (double)in.K * (double)in.batch <= kSkinny16;
-  if (in.K > 0 && (in.dtype == B2C_F32 ? c.g.J <= 16 : c.g.J <= 8 && small)) {
-    c.tier = GemmChoice::kSkinny;
-    return c;
-  }
-  const bool tc = in.K >= 32 && (double)in.I * (double)in.J * (double)in.K * (double)in.batch > 1048576.0;
-  c.tier = tc ? GemmChoice::kTc : GemmChoice::kSimt;
-  if (tc) {
+  if (c.tier == GemmChoice::kTc) {
     c.pack_p = plan_pack(in.dtype, c.g.P, in.batch, c.g.I, in.K);
     c.pack_q = plan_pack(in.dtype, c.g.Q, in.batch, c.g.J, in.K);
   }
