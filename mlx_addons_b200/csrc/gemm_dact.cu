@@ -20,9 +20,14 @@ constexpr int kDactWarps = 8;
 constexpr int kCols = 256;      // columns of a CTA: 8 per lane
 constexpr int kMaxBands = 256;
 
-int64_t dact_band_rows(int64_t rows) {
-  int64_t band = 64;
-  while ((rows + band - 1) / band > kMaxBands) band *= 2;
+// Rows of a band: one a warp, and more once that makes a thousand CTAs.
+int64_t dact_band_rows(int64_t rows, int64_t N) {
+  const int64_t blocks = (N + kCols - 1) / kCols;
+  int64_t band = kDactWarps;
+  while ((rows + band - 1) / band > kMaxBands || (rows + band - 1) / band * blocks > 1024) {
+    if (band >= rows) break;
+    band *= 2;
+  }
   return band;
 }
 
@@ -129,7 +134,7 @@ bool rows_on_16(const void* p, int64_t bs, int64_t rs, int64_t cs) {
 
 template <typename T>
 cudaError_t launch_t(const DactParams& p, cudaStream_t s) {
-  const int64_t rows = p.batch * p.M, band = dact_band_rows(rows);
+  const int64_t rows = p.batch * p.M, band = dact_band_rows(rows, p.N);
   const int bands = (int)((rows + band - 1) / band);
   if (bands > 0) {
     const dim3 grid((unsigned)((p.N + kCols - 1) / kCols), (unsigned)bands);
@@ -148,7 +153,7 @@ cudaError_t launch_t(const DactParams& p, cudaStream_t s) {
 }  // namespace
 
 size_t dact_ws_floats(int64_t batch, int64_t M, int64_t N) {
-  const int64_t rows = batch * M, band = dact_band_rows(rows);
+  const int64_t rows = batch * M, band = dact_band_rows(rows, N);
   return (size_t)((rows + band - 1) / band) * (size_t)N;
 }
 
