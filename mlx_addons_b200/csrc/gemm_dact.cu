@@ -71,6 +71,28 @@ __device__ __forceinline__ void store8(void* p, int64_t off, int64_t c, int64_t 
   }
 }
 
+// d[k] = dy[k] act'(x[k]); one choice of act for the eight.
+template <bool FAST>
+__device__ __forceinline__ void slope8(float (&d)[8], const float (&dy)[8], const float (&x)[8], int act) {
+  switch (act) {
+    case B2C_ACT_RELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = x[k] > 0.f ? dy[k] : 0.f;
+      break;
+    case B2C_ACT_GELU:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = dy[k] * act_slope_f32<FAST>(x[k], B2C_ACT_GELU);
+      break;
+    case B2C_ACT_GELU_TANH:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = dy[k] * act_slope_f32<FAST>(x[k], B2C_ACT_GELU_TANH);
+      break;
+    default:
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = dy[k] * act_slope_f32<FAST>(x[k], B2C_ACT_SILU);
+  }
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kDactWarps * 32) gemm_dact_kernel(const DactParams p, int64_t band) {
   __shared__ float part[kDactWarps][kCols];
@@ -86,9 +108,7 @@ __global__ void __launch_bounds__(kDactWarps * 32) gemm_dact_kernel(const DactPa
       if (p.pre) {
         float x[8];
         load8<T, VEC>(p.pre, b * p.pre_bs + i * p.pre_rs, p.pre_cs, c, p.N, x);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          d[k] = p.act == B2C_ACT_RELU ? (x[k] > 0.f ? dy[k] : 0.f) : dy[k] * act_slope_f32<sizeof(T) == 2>(x[k], p.act);
+        slope8<sizeof(T) == 2>(d, dy, x, p.act);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) d[k] = dy[k];
