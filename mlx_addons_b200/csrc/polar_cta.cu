@@ -14,6 +14,10 @@
 // of 64 columns with 128-byte swizzled rows, is K-major for S = X X^T and, read
 // the other way, MN-major for P X.
 //
+// A matrix whose longer side does not fit is shared by a cluster of 2 to 8
+// CTAs, each with some of the columns of X: S is then the sum of their parts,
+// taken through distributed shared memory, and P X stays local.
+//
 // Bound by the phases of a step in turn (product, conversion of the sums to
 // the next operand, barrier): two CTAs share an SM and fill each other's gaps.
 #include <cstdlib>
@@ -49,6 +53,7 @@ struct CtaParams {
   void* out;
   int64_t obs, orr, ol;
   int64_t batch;
+  int cl, chunk, ppitch;  // CTAs of a cluster, columns of X each, pitch of a part of S
   int side, L, g, xblocks, sblocks, kk, steps, along_l, lanes_per_row, blockwise, vec_in, vec_out, inject;
   double eps;
   CtaStep step[kMaxStepsC];
@@ -80,6 +85,63 @@ __device__ __forceinline__ void store_unit(unsigned char* buf, int plane_bytes, 
   if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(buf + plane_bytes + off) = *reinterpret_cast<const uint4*>(l);
 }
 
+// hi + lo of 8 columns.
+template <int PLANES>
+__device__ __forceinline__ void load_halves(const unsigned char* buf, int plane_bytes, int off, float (&v)[8]) {
+  const uint4 h = *reinterpret_cast<const uint4*>(buf + off);
+  const __half2* a = reinterpret_cast<const __half2*>(&h);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = __half22float2(a[k]);
+    v[2 * k] = f.x, v[2 * k + 1] = f.y;
+  }
+  if constexpr (PLANES == 2) {
+    const uint4 l = *reinterpret_cast<const uint4*>(buf + plane_bytes + off);
+    const __half2* c = reinterpret_cast<const __half2*>(&l);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __half22float2(c[k]);
+      v[2 * k] += f.x, v[2 * k + 1] += f.y;
+    }
+  }
+}
+
+// Shared memory of the q-th CTA of the cluster, at the place of a pointer of this one.
+__device__ __forceinline__ double peer_double(const double* p, int q) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(map_rank(smem_u32(p), q)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_load8(const float* p, int q, float (&v)[8]) {
+  const uint32_t a = map_rank(smem_u32(p), q);
+#pragma unroll
+  for (int k = 0; k < 8; k += 4)
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v[k]), "=f"(v[k + 1]), "=f"(v[k + 2]), "=f"(v[k + 3])
+                 : "r"(a + k * 4)
+                 : "memory");
+}
+__device__ __forceinline__ void peer_store_float(float* p, int q, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_rank(smem_u32(p), q)), "f"(v) : "memory");
+}
+template <int PLANES>
+__device__ __forceinline__ void peer_store_unit(unsigned char* buf, int plane_bytes, int off, int q, const float (&v)[8]) {
+  __align__(16) __half2 h[4], l[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+    const float2 f = __half22float2(h[k]);
+    l[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
+  }
+#pragma unroll
+  for (int pl = 0; pl < PLANES; ++pl) {
+    const uint4 w = *reinterpret_cast<const uint4*>(pl ? l : h);
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(map_rank(smem_u32(buf + pl * plane_bytes + off), q)),
+                 "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                 : "memory");
+  }
+}
+
 // 8 elements of a row, zeros past its end.
 template <typename T>
 __device__ __forceinline__ void load_unit8(const T* row, int64_t stride, int c, int n, int vec, float (&v)[8]) {
@@ -98,7 +160,8 @@ __device__ __forceinline__ void load_unit8(const T* row, int64_t stride, int c, 
   }
 }
 
-template <typename T, int PLANES, int NT>
+// CL: a cluster of p.cl CTAs shares a stack, `chunk` columns of X each.
+template <typename T, int PLANES, int NT, bool CL>
 __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_constant__ CtaParams p) {
   extern __shared__ unsigned char raw[];
   __shared__ double rowsum[NT];
@@ -112,6 +175,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
   unsigned char* X = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int x_plane = p.xblocks * kBlockBytes, s_plane = p.sblocks * kBlockBytes;
   unsigned char* S = X + PLANES * x_plane;
+  const int rank = CL ? (int)cluster_rank() : 0, base = rank * p.chunk, L = CL ? max(0, min(p.chunk, p.L - base)) : p.L;
+  float* partial = reinterpret_cast<float*>(S + PLANES * s_plane);  // CL: this CTA's part of S, rows of ppitch floats
   const uint32_t done = smem_u32(bars), never = done + 8;
   const uint64_t limit = p.inject ? 1000000ull : kWaitNs;
   volatile int* gu = &gave_up;
@@ -128,14 +193,14 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     fence_before();
   }
   // ---- norms ----
-  const int64_t m0 = (int64_t)blockIdx.x * p.g;
+  const int64_t m0 = (int64_t)(blockIdx.x / (CL ? p.cl : 1)) * p.g;
   const int have = (int)(p.batch - m0 < p.g ? p.batch - m0 : p.g), rows = have * p.side;
-  const T* G = static_cast<const T*>(p.G) + m0 * p.bs;
+  const T* G = static_cast<const T*>(p.G) + m0 * p.bs + base * p.sl;
   for (int e = tid * 16; e < PLANES * (x_plane + s_plane); e += NT * 16)
     *reinterpret_cast<uint4*>(X + e) = make_uint4(0, 0, 0, 0);
   // rows of X: `lpr` lanes take the 8-element units of a row in turn (its neighbours lie along the lanes), or, where the
   // small index has the smaller stride, NG threads share a row and the lanes run along the rows
-  const int units = (p.L + 7) / 8, lpr = p.lanes_per_row;
+  const int units = (L + 7) / 8, lpr = p.lanes_per_row;
   if (p.along_l) {
     const int per = 32 / lpr, sub = lane / lpr, u0 = lane % lpr;
     for (int r0 = warp * per; r0 < rows; r0 += NW * per * kRowsInFlight) {
@@ -145,7 +210,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
 #pragma unroll
         for (int k = 0; k < kRowsInFlight; ++k) {
           const int r = r0 + sub + k * NW * per, m = r / p.side;
-          load_unit8<T>(G + m * p.bs + (r - m * p.side) * p.sr, p.sl, u * 8, r < rows ? p.L : 0, p.vec_in, v[k]);
+          load_unit8<T>(G + m * p.bs + (r - m * p.side) * p.sr, p.sl, u * 8, r < rows ? L : 0, p.vec_in, v[k]);
         }
 #pragma unroll
         for (int k = 0; k < kRowsInFlight; ++k)
@@ -171,7 +236,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     if (r < rows) {
       for (int u = tid >> 7; u < units; u += NG) {
         float v[8];
-        load_unit8<T>(row, p.sl, u * 8, p.L, 0, v);
+        load_unit8<T>(row, p.sl, u * 8, L, 0, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
       }
@@ -186,10 +251,23 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
       for (int g = 0; g < NG; ++g) s += rowsum[m * p.side + r + 128 * g];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
-    if (lane == 0) {
+    if (CL) {
+      if (lane == 0) rowsum[m * p.side] = s;  // this matrix's own entries have been read
+    } else if (lane == 0) {
       const PolarNorm n = polar_norm(sqrt(s) + p.eps);
       factor[m] = n.half_scale();
       first_r[m] = n.r;
+    }
+  }
+  if constexpr (CL) {
+    __syncwarp();
+    cluster_sync();
+    if (tid < have) {
+      double s = 0.0;
+      for (int q = 0; q < p.cl; ++q) s += peer_double(&rowsum[tid * p.side], q);
+      const PolarNorm n = polar_norm(sqrt(s) + p.eps);
+      factor[tid] = n.half_scale();
+      first_r[tid] = n.r;
     }
   }
   __syncthreads();
@@ -202,7 +280,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
 #pragma unroll
         for (int k = 0; k < kRowsInFlight; ++k) {
           const int r = r0 + k * NW * per, m = r / p.side;
-          load_unit8<T>(G + m * p.bs + (r - m * p.side) * p.sr, p.sl, u * 8, r < rows ? p.L : 0, p.vec_in, v[k]);
+          load_unit8<T>(G + m * p.bs + (r - m * p.side) * p.sr, p.sl, u * 8, r < rows ? L : 0, p.vec_in, v[k]);
         }
 #pragma unroll
         for (int k = 0; k < kRowsInFlight; ++k) {
@@ -222,7 +300,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
       const T* row = G + m * p.bs + (r - m * p.side) * p.sr;
       for (int u = tid >> 7; u < units; u += NG) {
         float v[8];
-        load_unit8<T>(row, p.sl, u * 8, p.L, 0, v);
+        load_unit8<T>(row, p.sl, u * 8, L, 0, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] * f.x * f.y;
         store_unit<PLANES>(X, x_plane, unit_off(r, u), v);
@@ -256,7 +334,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
   constexpr bool kSplitDiag = PLANES == 1;
   for (int t = 0; t < p.steps; ++t) {
     const CtaStep k = p.step[t];
-    const float f1 = t ? 1.f : r0, f2 = f1 * f1, k3 = k.k3 * f2, kp = k.kp * f2;
+    const float f1 = t ? 1.f : r0, f2 = f1 * f1, k3 = CL ? k.k3 / k.k1 : k.k3 * f2, kp = CL ? k.kp / k.k1 : k.kp * f2;
     // ---- S = X X^T ----
     if (warp == 0) {
       if (elect_one()) {
@@ -273,21 +351,71 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
       __syncwarp();  // a warp that sleeps on the barrier sleeps as a whole
     }
     wait();
-    for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
-      if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
-      float v[32];
-      tmem_row32(lanes + c0, v);
+    if constexpr (CL) {
+      // the sum over the cluster: every CTA puts its part into its own shared memory, takes a share of the rows of all
+      // parts, in order, and gives the result to all. One that has given up spreads NaN.
+      const float f = *gu ? __int_as_float(0x7fffffff) : k.k1 * f2;
+      for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
+        if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
+        float v[32];
+        tmem_row32(lanes + c0, v);
+        float4* at = reinterpret_cast<float4*>(partial + row * p.ppitch + c0);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float w[8];
-        const float f = k.k1 * f2;
+        for (int q = 0; q < 8; ++q) {
+          float w[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int c = c0 + u * 8 + e;
-          if (kSplitDiag && c == row) sdiag[row] = v[u * 8 + e] * f2 * kUnitS;
-          w[e] = (unsigned)(c - lo) < (unsigned)(hi - lo) && !(kSplitDiag && c == row) ? v[u * 8 + e] * f : 0.f;
+          for (int e = 0; e < 4; ++e)
+            w[e] = (unsigned)(c0 + 4 * q + e - lo) < (unsigned)(hi - lo) ? v[4 * q + e] * f : 0.f;
+          if (c0 + 4 * q < p.kk) at[q] = make_float4(w[0], w[1], w[2], w[3]);
         }
-        if (c0 + u * 8 < p.kk) store_unit<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), w);
+      }
+      __syncwarp();
+      cluster_sync();
+      const int share = 128 / p.cl, per_row = p.kk / 8;
+      for (int u = tid; u < share * per_row; u += NT) {
+        const int r = rank * share + u / per_row, c8 = u % per_row, m = r / p.side;
+        // blocks off the diagonal stay zero
+        if (r >= p.kk || c8 * 8 + 8 <= m * p.side || c8 * 8 >= m * p.side + p.side) continue;
+        float v[8] = {};
+        const float* at = partial + r * p.ppitch + c8 * 8;
+        for (int q = 0; q < p.cl; ++q) {
+          float w[8];
+          peer_load8(at, q, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += w[e];
+        }
+        float d = 0.f;
+        if constexpr (kSplitDiag) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c8 * 8 + e == r) d = v[e] * (kUnitS / k.k1), v[e] = 0.f;
+        }
+        const bool diag = kSplitDiag && r - c8 * 8 >= 0 && r - c8 * 8 < 8;
+        for (int q = 0; q < p.cl; ++q) {
+          peer_store_unit<PLANES>(S, s_plane, unit_off(r, c8), q, v);
+          if (diag) peer_store_float(&sdiag[r], q, d);
+        }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __syncwarp();
+      cluster_sync();
+    } else {
+      for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
+        if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
+        float v[32];
+        tmem_row32(lanes + c0, v);
+  #pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float w[8];
+          const float f = k.k1 * f2;
+  #pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = c0 + u * 8 + e;
+            if (kSplitDiag && c == row) sdiag[row] = v[u * 8 + e] * f2 * kUnitS;
+            w[e] = (unsigned)(c - lo) < (unsigned)(hi - lo) && !(kSplitDiag && c == row) ? v[u * 8 + e] * f : 0.f;
+          }
+          if (c0 + u * 8 < p.kk) store_unit<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), w);
+        }
       }
     }
     fence_before();
@@ -318,7 +446,17 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     for (int c0 = first / 32 * 32; c0 < last; c0 += 32) {
       if (((c0 - first / 32 * 32) >> 5) % NG != group) continue;
       float v[32], w[32];
-      tmem_row32(lanes + c0, v);
+      if constexpr (CL) {  // the whole S is in shared memory alone
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float x[8] = {};
+          if (c0 + u * 8 < p.kk) load_halves<PLANES>(S, s_plane, unit_off(row, (c0 >> 3) + u), x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u * 8 + e] = x[e];
+        }
+      } else {
+        tmem_row32(lanes + c0, v);
+      }
       tmem_row32(lanes + 128 + c0, w);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -391,9 +529,9 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
         if (t == p.steps - 1 && row < rows) {
           const float nan = __int_as_float(0x7fffffff);
           const float f = factor[mine].x == 0.f || *gu ? nan : 1.f / kPolarScale;
-          T* o = static_cast<T*>(p.out) + (m0 + mine) * p.obs + (row - lo) * p.orr + c * p.ol;
+          T* o = static_cast<T*>(p.out) + (m0 + mine) * p.obs + (row - lo) * p.orr + (base + c) * p.ol;
           constexpr int PER = 16 / sizeof(T);
-          if (p.vec_out && c + 32 <= p.L) {
+          if (p.vec_out && c + 32 <= L) {
 #pragma unroll
             for (int u = 0; u < 32 / PER; ++u) {
               uint4 w;
@@ -405,7 +543,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (c + e < p.L) o[e * p.ol] = from_f32<T>(v[e] * f);
+              if (c + e < L) o[e * p.ol] = from_f32<T>(v[e] * f);
           }
         }
       }
@@ -422,6 +560,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
     }
     __syncthreads();
   }
+  if constexpr (CL) cluster_sync();  // no CTA ends while another may write to it
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
 }
 
@@ -430,46 +569,84 @@ bool inject_timeout() {
   return t && strcmp(t, "1") == 0;
 }
 
-template <typename T, int PLANES, int NT>
+template <typename T, int PLANES, int NT, bool CL>
 cudaError_t launch_n(const CtaParams& p, size_t smem, unsigned grid, cudaStream_t s) {
-  auto kern = polar_cta_kernel<T, PLANES, NT>;
+  auto kern = polar_cta_kernel<T, PLANES, NT, CL>;
   static int cache[64];
   int occ = 0;
   const cudaError_t e = kernel_occupancy(kern, NT, smem, cache, &occ);
   if (e != cudaSuccess) return e;
-  kern<<<grid, NT, smem, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.cl;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CL ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 // 16 warps where one CTA has an SM to itself, by its shared memory or because
 // there are no more CTAs than SMs; otherwise two CTAs of 8.
 template <typename T, int PLANES>
 cudaError_t launch_c(const CtaParams& p, size_t smem, unsigned grid, int sms, cudaStream_t s) {
-  if (smem > 113 * 1024 || grid <= (unsigned)sms) return launch_n<T, PLANES, 512>(p, smem, grid, s);
-  return launch_n<T, PLANES, 256>(p, smem, grid, s);
+  if (p.cl > 1) return launch_n<T, PLANES, 512, true>(p, smem, grid, s);
+  if (smem > 113 * 1024 || grid <= (unsigned)sms) return launch_n<T, PLANES, 512, false>(p, smem, grid, s);
+  return launch_n<T, PLANES, 256, false>(p, smem, grid, s);
 }
 
-int64_t smem_of(int planes, int64_t xblocks, int64_t sblocks) { return 1024 + planes * (xblocks + sblocks) * kBlockBytes; }
+// How a problem is laid out over CTAs.
+struct CtaPlan {
+  int planes, cl, g, xblocks, kk;  // planes 0: does not fit
+  size_t smem;
+};
 
-// Planes that fit with one matrix's S: two, or one for bfloat16 results only;
-// 0 if the matrix is too large. Two planes cost three products instead of one,
-// which these sizes hide, and leave a bfloat16 result its own rounding alone.
-int planes_of(const PolarParams& p) {
+int rounded(int64_t rows) { return (int)((rows + 15) / 16 * 16); }
+
+size_t plan_smem(int planes, int cl, int xblocks, int kk) {
+  return 1024 + (size_t)planes * (xblocks + (kk + 63) / 64) * kBlockBytes + (cl > 1 ? (size_t)128 * (kk + 4) * 4 : 0);
+}
+
+// Two planes, or one for bfloat16 results where two do not fit: they cost three
+// products instead of one, which these sizes hide, and leave a bfloat16
+// result its own rounding alone. As few CTAs a matrix as hold it, and more, up to
+// 8 of at least 128 columns, where that leaves SMs idle; as many matrices a CTA
+// as keep two CTAs on every SM.
+CtaPlan plan_cta(const PolarParams& p, int sms) {
   const int64_t side = p.m < p.n ? p.m : p.n, L = p.m < p.n ? p.n : p.m;
-  if (side > 128) return 0;
-  const int64_t x = (L + 63) / 64, sb = side <= 64 ? 1 : 2;
-  if (smem_of(2, x, sb) <= kSmemMaxC) return 2;
-  return p.dtype == B2C_BF16 && smem_of(1, x, sb) <= kSmemMaxC ? 1 : 0;
+  CtaPlan r{};
+  if (side > 128 || L > 64 * 8 * 16) return r;
+  const int blocks = (int)((L + 63) / 64);
+  for (int planes = 2; planes >= (p.dtype == B2C_BF16 ? 1 : 2) && !r.planes; --planes)
+    for (int cl = 1; cl <= 8 && !r.planes; cl *= 2)
+      if (plan_smem(planes, cl, (blocks + cl - 1) / cl, rounded(side)) <= (size_t)kSmemMaxC) r.planes = planes, r.cl = cl;
+  if (!r.planes) return r;
+  while (r.cl < 8 && (int64_t)p.batch * r.cl * 2 <= sms && (blocks + 2 * r.cl - 1) / (2 * r.cl) >= 2 &&
+         plan_smem(r.planes, r.cl * 2, (blocks + 2 * r.cl - 1) / (2 * r.cl), rounded(side)) <= (size_t)kSmemMaxC)
+    r.cl *= 2;
+  r.xblocks = (blocks + r.cl - 1) / r.cl;
+  const int64_t slots = (r.cl > 1 ? 1 : 2) * (int64_t)sms;
+  int64_t g = (p.batch * r.cl + slots - 1) / slots;
+  if (g > 128 / side) g = 128 / side;
+  while (g > 1 && plan_smem(r.planes, r.cl, r.xblocks, rounded(g * side)) > (size_t)kSmemMaxC) --g;
+  r.g = (int)g;
+  r.kk = rounded(g * side);
+  r.smem = plan_smem(r.planes, r.cl, r.xblocks, r.kk);
+  return r;
 }
 
 }  // namespace
 
-bool polar_cta_fits(const PolarParams& p) { return planes_of(p) > 0; }
+bool polar_cta_fits(const PolarParams& p) { return plan_cta(p, 148).planes > 0; }
 
 cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
   CtaParams p{};
   const bool wide = in.m <= in.n;
-  const int planes = planes_of(in);
+  const CtaPlan plan = plan_cta(in, sms);
   p.G = in.G;
   p.bs = in.bs, p.sr = wide ? in.rs : in.cs, p.sl = wide ? in.cs : in.rs;
   p.out = in.out;
@@ -477,13 +654,12 @@ cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
   p.batch = in.batch;
   p.side = (int)(wide ? in.m : in.n);
   p.L = (int)(wide ? in.n : in.m);
-  p.xblocks = (p.L + 63) / 64;
-  // matrices of a CTA: no more than keeps two CTAs on every SM, and than fit with their S
-  int64_t g = (in.batch + 2 * sms - 1) / (2 * sms);
-  if (g > 128 / p.side) g = 128 / p.side;
-  while (g > 1 && smem_of(planes, p.xblocks, (g * p.side + 63) / 64) > kSmemMaxC) --g;
-  p.g = (int)g;
-  p.kk = (p.g * p.side + 15) / 16 * 16;
+  p.cl = plan.cl;
+  p.xblocks = plan.xblocks;
+  p.chunk = plan.xblocks * 64;
+  p.g = plan.g;
+  p.kk = plan.kk;
+  p.ppitch = p.kk + 4;
   p.sblocks = (p.kk + 63) / 64;
   p.blockwise = p.side % 16 == 0;
   p.along_l = p.sl <= p.sr || p.side == 1;
@@ -491,7 +667,7 @@ cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
   p.eps = in.eps;
   p.inject = inject_timeout();
   p.lanes_per_row = 1;
-  while (p.lanes_per_row < 32 && p.lanes_per_row * 8 < p.L) p.lanes_per_row *= 2;
+  while (p.lanes_per_row < 32 && p.lanes_per_row * 8 < (p.L < p.chunk ? p.L : p.chunk)) p.lanes_per_row *= 2;
   const int64_t per = in.dtype == B2C_F32 ? 4 : 8;
   p.vec_in = p.sl == 1 && (reinterpret_cast<uintptr_t>(in.G) & 15) == 0 && p.sr % per == 0 && p.bs % per == 0;
   const int64_t elt = in.dtype == B2C_F32 ? 4 : 2;
@@ -504,16 +680,16 @@ cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
                         (float)(sp / (sx * sx)), (float)a, (float)b, (float)c};
     hi = polar_poly_bound(a, b, c, hi);
   }
-  size_t smem = (size_t)smem_of(planes, p.xblocks, p.sblocks);
+  size_t smem = plan.smem;
   if (smem < 77 * 1024) smem = 77 * 1024;  // two CTAs at most: each holds half of the tensor memory
-  const int64_t ctas = (in.batch + g - 1) / g;
+  const int64_t ctas = (in.batch + p.g - 1) / p.g * p.cl;
   if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const unsigned grid = (unsigned)ctas;
   switch (in.dtype) {
     case B2C_F32: return launch_c<float, 2>(p, smem, grid, sms, s);
     case B2C_BF16:
-      return planes == 2 ? launch_c<__nv_bfloat16, 2>(p, smem, grid, sms, s)
-                         : launch_c<__nv_bfloat16, 1>(p, smem, grid, sms, s);
+      return plan.planes == 2 ? launch_c<__nv_bfloat16, 2>(p, smem, grid, sms, s)
+                              : launch_c<__nv_bfloat16, 1>(p, smem, grid, sms, s);
     default: return launch_c<__half, 2>(p, smem, grid, sms, s);
   }
 }

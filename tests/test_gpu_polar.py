@@ -200,6 +200,26 @@ def test_middle_sizes(shape, dtype):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,m,n", [(1, 128, 513), (1, 64, 300), (2, 20, 1500), (5, 1469, 38), (1, 1, 2000), (3, 100, 1536),
+                                       (1, 128, 1537), (400, 20, 700), (300, 33, 600), (160, 600, 64), (20, 16, 2560)])
+def test_a_long_side(batch, m, n, dtype):
+    """Matrices shared by a cluster of CTAs, alone and stacked, transposed and with a broken one among them."""
+    G = _grad_like((batch, m, n), dtype, seed=m + 1)
+    G = G * torch.logspace(-2, 2, batch, device=DEV).reshape(-1, 1, 1).to(dtype)
+    out = la.orthogonalize(G)
+    _check(out, G)
+    _check(la.orthogonalize(G.mT.contiguous().mT), G)
+    assert all(torch.equal(la.orthogonalize(G), out) for _ in range(3))
+    if batch > 2:
+        G2 = G.clone()
+        G2[1, m - 1, n - 1], G2[batch - 1, 0, 0] = float("nan"), float("inf")
+        out2 = la.orthogonalize(G2)
+        keep = torch.ones(batch, dtype=torch.bool, device=DEV)
+        keep[1] = keep[batch - 1] = False
+        assert torch.equal(out2[keep], out[keep]) and bool(torch.isnan(out2[~keep]).all())
+
+
 def test_two_streams_at_once():
     """Calls that need every SM together, side by side on two streams."""
     G = [_grad_like((3, 300 + 50 * i, 500), F32, seed=i) for i in range(2)]
