@@ -145,6 +145,7 @@ __device__ __forceinline__ void epilogue_store(const GemmEpilogue& e, int64_t b,
 
 // Launchers. gemm_simt.cu
 cudaError_t launch_gemm_simt(const GemmProblem& g, cudaStream_t s);
+int simt_split(const GemmProblem& g, int sms);
 
 // gemm_skinny.cu: g.J columns in passes of up to 8
 cudaError_t launch_gemm_skinny(const GemmProblem& g, int sms, cudaStream_t s);

@@ -52,7 +52,16 @@ struct GemmChoice {
   size_t ws() const { return tier == kTc ? (size_t)(pack_p.bytes + pack_q.bytes) : 0; }
 };
 
+// Time of a product on the FP32 units, us: a launch, and 0.05 a k of a CTA that has an SM
+// to itself, 0.03 more for each that it shares it with.
+double simt_us(const GemmProblem& g, int sms) {
+  const int split = simt_split(g, sms);
+  const double ctas = (double)g.batch * (double)((g.I + 63) / 64) * (double)((g.J + 63) / 64) * split;
+  return 6.0 + (double)((g.K + split - 1) / split) * (0.02 + 0.03 * ceil(ctas / sms));
+}
+
 GemmChoice choose(const GemmProblem& in) {
+  constexpr int sms = 148;  // of a B200: the choice, and with it the workspace, depends on the sizes alone
   GemmChoice c{};
   c.g = in;
   const double macs = (double)in.I * (double)in.J * (double)in.K * (double)in.batch;
@@ -60,10 +69,10 @@ GemmChoice choose(const GemmProblem& in) {
   const bool f32 = in.dtype == B2C_F32;
   // one to eight (float32: sixteen) columns: one pass over the other operand
   const bool thin = in.K > 0 && (f32 ? shorter <= 16 : shorter <= 8 && (double)longer * in.K * in.batch <= kSkinny16);
-  // the tensor cores' set-up, and for float32 the pass that splits the operands, cost as much as this
-  // (float32, us on the FP32 units and on the tensor cores: 128 x 512 x 128 28 and 14, 256 x 256 x 256 16 and 14, 1024 x 64 x 1024 9
-  // and 12, 4096 x 64 x 4096 88 and 45)
-  const bool shallow = f32 ? in.K < 40 || (in.K < 96 && macs <= 1e8) || (in.K <= 256 && macs <= 8e6) || macs <= 1e6
+  // The tensor cores' set-up, and for float32 the pass that splits the operands, cost as much as this: float32 17 us at
+  // the least, which the FP32 units need for about 200 k of a CTA (us on the FP32 units and on the tensor cores: 145 x 449 x 148
+  // 13 and 19, 256 x 256 x 256 11 and 17, 512 x 512 x 512 19 and 19, 64 x 4096 x 64 32 and 25); 16-bit types 8 us.
+  const bool shallow = f32 ? in.K < 40 || (in.K < 96 && macs <= 1e8) || macs <= 1e6 || simt_us(in, sms) <= 17
                            : in.K < 32 || macs <= 1048576.0;
   c.tier = thin ? GemmChoice::kSkinny : shallow ? GemmChoice::kSimt : GemmChoice::kTc;
   if (c.tier != GemmChoice::kSimt && in.I <= 64 && in.J > in.I) {  // the longer side takes the 128 rows of a tile

@@ -11,8 +11,13 @@
 // shallow product is bound by writing D: the 4 columns of a thread are
 // neighbours and stored as one unit where alignment allows, and 16 apart
 // otherwise, so that a half warp's stores lie together.
+//
+// Too few tiles for the GPU: k is split over a cluster of up to 8 CTAs, which
+// leave their sums in shared memory; each then joins, in order, and finishes its
+// share of the tile's rows.
 #include "b2c_kernels.cuh"
 #include "gemm.cuh"
+#include "tcgen05.cuh"
 
 namespace b2c {
 
@@ -31,17 +36,17 @@ struct SliceLoader {
   const T* at;       // element 0
   int64_t step, kstep, left_r, left_k, dr, dk;
   int r, k;
-  __device__ __forceinline__ SliceLoader(const GemmOperand& o, int64_t b, int64_t r0, int64_t rows, int64_t K) {
+  __device__ __forceinline__ SliceLoader(const GemmOperand& o, int64_t b, int64_t r0, int64_t rows, int64_t k0, int64_t K) {
     const bool along_k = o.ks <= o.rs;
     r = along_k ? threadIdx.x / TK : threadIdx.x % TS;
     k = along_k ? threadIdx.x % TK : threadIdx.x / TS;
     dr = along_k ? kSimtThreads / TK : 0;
     dk = along_k ? 0 : kSimtThreads / TS;
-    at = static_cast<const T*>(o.p) + b * o.bs + (r0 + r) * o.rs + k * o.ks;
+    at = static_cast<const T*>(o.p) + b * o.bs + (r0 + r) * o.rs + (k0 + k) * o.ks;
     step = dr * o.rs + dk * o.ks;
     kstep = TK * o.ks;
     left_r = rows - r0 - r;
-    left_k = K - k;
+    left_k = K - k0 - k;
   }
   __device__ __forceinline__ void load(float (&v)[kLoads]) {
 #pragma unroll
@@ -61,26 +66,42 @@ struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
 
-// VEC: every row of y, pre and the addend starts on a unit of four.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kSimtThreads) gemm_simt_kernel(const GemmProblem g, int64_t tiles_i, int64_t tiles_j) {
+struct SimtParams {
+  GemmProblem g;
+  int64_t tiles_i, tiles_j;
+  int64_t k_per;  // k of one CTA of a cluster
+  int split;      // CTAs of a cluster
+};
+
+// What a thread finishes: single elements, units of four (every row of y, pre
+// and the addend starts on one), or its share of a sum over a cluster.
+enum SimtForm { kElements, kUnits, kSplit };
+
+template <typename T, int FORM>
+__global__ void __launch_bounds__(kSimtThreads) gemm_simt_kernel(const __grid_constant__ SimtParams p) {
+  constexpr bool VEC = FORM != kElements;
   __shared__ __align__(16) float sp[TK][TP], sq[TK][TP];
-  const int64_t per = tiles_i * tiles_j, b = blockIdx.x / per, t = blockIdx.x - b * per;
+  __shared__ __align__(16) float part[FORM == kSplit ? TS : 1][TP];
+  const GemmProblem& g = p.g;
+  const int64_t tiles_j = p.tiles_j, per = p.tiles_i * tiles_j, blk = FORM == kSplit ? blockIdx.x / p.split : blockIdx.x;
+  const int rank = FORM == kSplit ? (int)cluster_rank() : 0;
+  const int64_t kb = rank * p.k_per, ke = FORM == kSplit && kb + p.k_per < g.K ? kb + p.k_per : g.K;
+  const int64_t b = blk / per, t = blk - b * per;
   const int64_t i0 = (t / tiles_j) * TS, j0 = (t % tiles_j) * TS;
   const int ti = threadIdx.x / 16, tj = threadIdx.x % 16;
-  SliceLoader<T> lp(g.P, b, i0, g.I, g.K), lq(g.Q, b, j0, g.J, g.K);
+  SliceLoader<T> lp(g.P, b, i0, g.I, kb, ke), lq(g.Q, b, j0, g.J, kb, ke);
   float acc[8][4] = {}, vp[kLoads], vq[kLoads];
   lp.load(vp);
   lq.load(vq);
-  for (int64_t k0 = 0; k0 < g.K; k0 += TK) {
+  for (int64_t k0 = kb; k0 < ke; k0 += TK) {
     lp.store(sp, vp);
     lq.store(sq, vq);
     __syncthreads();
-    if (k0 + TK < g.K) {
+    if (k0 + TK < ke) {
       lp.load(vp);
       lq.load(vq);
     }
-    const int n = g.K - k0 < TK ? (int)(g.K - k0) : TK;
+    const int n = ke - k0 < TK ? (int)(ke - k0) : TK;
 #pragma unroll 4
     for (int k = 0; k < n; ++k) {
       const float4 a = *reinterpret_cast<const float4*>(&sp[k][ti * 8]), c = *reinterpret_cast<const float4*>(&sp[k][ti * 8 + 4]);
@@ -99,6 +120,35 @@ __global__ void __launch_bounds__(kSimtThreads) gemm_simt_kernel(const GemmProbl
         for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], qv[j], acc[i][j]);
     }
     __syncthreads();
+  }
+  if constexpr (FORM == kSplit) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      *reinterpret_cast<float4*>(&part[ti * 8 + r][tj * 4]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+    __syncwarp();
+    cluster_sync();
+    const int share = TS / p.split;
+    for (int u = threadIdx.x; u < share * (TS / 4); u += kSimtThreads) {
+      const int r = rank * share + u / (TS / 4), c = u % (TS / 4) * 4;
+      if (i0 + r >= g.I || j0 + c >= g.J) continue;
+      const uint32_t at = smem_u32(&part[r][c]);
+      float s[4] = {};
+      for (int q = 0; q < p.split; q += 2) {
+        float v[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[h][0]), "=f"(v[h][1]), "=f"(v[h][2]), "=f"(v[h][3])
+                       : "r"(map_rank(at, q + h))
+                       : "memory");
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[0][e], s[e] += v[1][e];
+      }
+      for (int e = 0; e < 4 && j0 + c + e < g.J; ++e) epilogue_store<T>(g.e, b, i0 + r, j0 + c + e, s[e]);
+    }
+    __syncwarp();
+    cluster_sync();  // a CTA's sums stay until they have been read
+    return;
   }
   const int64_t i = i0 + ti * 8, j = j0 + (VEC ? tj * 4 : tj);
   constexpr int JS = VEC ? 1 : 16;  // columns between a thread's four
@@ -161,25 +211,54 @@ __global__ void __launch_bounds__(kSimtThreads) gemm_simt_kernel(const GemmProbl
 }
 
 template <typename T>
-cudaError_t launch_t(const GemmProblem& g, cudaStream_t s) {
-  const int64_t ti = (g.I + TS - 1) / TS, tj = (g.J + TS - 1) / TS, total = g.batch * ti * tj;
-  if (total > 0x7fffffff) return cudaErrorInvalidConfiguration;
+cudaError_t launch_t(const GemmProblem& g, int sms, cudaStream_t s) {
+  SimtParams p{};
+  p.g = g;
+  p.tiles_i = (g.I + TS - 1) / TS, p.tiles_j = (g.J + TS - 1) / TS;
+  const int64_t tiles = g.batch * p.tiles_i * p.tiles_j;
+  p.split = simt_split(g, sms);
+  p.k_per = (g.K + p.split - 1) / p.split;
+  if (tiles * p.split > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const unsigned grid = (unsigned)(tiles * p.split);
+  if (p.split > 1) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kSimtThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, gemm_simt_kernel<T, kSplit>, p);
+  }
   auto fours = [](const GemmView& v) {
     return !v.p || (v.js == 1 && reinterpret_cast<uintptr_t>(v.p) % (4 * sizeof(T)) == 0 && v.is % 4 == 0 && v.bs % 4 == 0);
   };
-  const unsigned grid = (unsigned)total;
-  if (fours(g.e.y) && fours(g.e.pre) && fours(g.e.res)) gemm_simt_kernel<T, true><<<grid, kSimtThreads, 0, s>>>(g, ti, tj);
-  else gemm_simt_kernel<T, false><<<grid, kSimtThreads, 0, s>>>(g, ti, tj);
+  if (fours(g.e.y) && fours(g.e.pre) && fours(g.e.res)) gemm_simt_kernel<T, kUnits><<<grid, kSimtThreads, 0, s>>>(p);
+  else gemm_simt_kernel<T, kElements><<<grid, kSimtThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace
 
+// CTAs that share a tile's k: up to 8, of at least 64 each, while they all fit at once.
+int simt_split(const GemmProblem& g, int sms) {
+  const int64_t tiles = g.batch * ((g.I + TS - 1) / TS) * ((g.J + TS - 1) / TS);
+  int split = 1;
+  while (split < 8 && tiles * split <= sms && g.K >= split * 128) split *= 2;
+  return split;
+}
+
 cudaError_t launch_gemm_simt(const GemmProblem& g, cudaStream_t s) {
+  int sms = 0;
+  const cudaError_t e = device_sms(&sms);
+  if (e != cudaSuccess) return e;
   switch (g.dtype) {
-    case B2C_F32: return launch_t<float>(g, s);
-    case B2C_BF16: return launch_t<__nv_bfloat16>(g, s);
-    default: return launch_t<__half>(g, s);
+    case B2C_F32: return launch_t<float>(g, sms, s);
+    case B2C_BF16: return launch_t<__nv_bfloat16>(g, sms, s);
+    default: return launch_t<__half>(g, sms, s);
   }
 }
 

@@ -6,8 +6,8 @@
 // P with unit stride along k: a warp takes 4 rows, its lanes run along k (16
 // bytes a lane where alignment allows), so Q's values, read through L1, serve
 // 4 rows. P with unit stride along the rows: a lane takes 8 rows, the 8 warps
-// of a CTA take every 8th k, and Q's slice is staged in shared memory as
-// float32 for broadcasts.
+// of a CTA take every 8th k (with 64 rows a CTA instead of 256, a quarter of a
+// warp does), and Q's slice is staged in shared memory as float32 for broadcasts.
 //
 // Where there are too few rows to fill the GPU, k is split over the warps of
 // a CTA and over a cluster of up to 8 CTAs; the partial sums are joined in
@@ -23,7 +23,6 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kSkinnyThreads = kWarps * 32;
 constexpr int kRows = 4;        // rows of a warp, unit stride along k
-constexpr int kRowBlock = 256;  // rows of a CTA, unit stride along the rows
 constexpr int kSlice = 256;     // k staged at a time there
 
 struct SkinnyParams {
@@ -127,16 +126,18 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_k_kernel(const __grid_c
   if (p.split > 1) cluster_barrier();  // peers' shared memory stays until it has been read
 }
 
-template <typename T, int JT, bool VEC>
+// ROWS: rows of a CTA, 8 a lane.
+template <typename T, int JT, bool VEC, int ROWS>
 __global__ void __launch_bounds__(kSkinnyThreads) skinny_row_kernel(const __grid_constant__ SkinnyParams p) {
   __shared__ __align__(16) float xs[kSlice][JT];
-  __shared__ float red[kWarps][kRowBlock];
-  __shared__ float part[JT][kRowBlock];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int LR = ROWS / 8, KG = 32 / LR;  // lanes along the rows, k of a warp at a time
+  __shared__ float red[kWarps * KG][ROWS];
+  __shared__ float part[JT][ROWS];
+  const int lane = threadIdx.x % LR, kg = threadIdx.x / LR;  // lane of a row group, row group
   const uint32_t rank = p.split > 1 ? ctarank() : 0;
-  const int64_t blk = blockIdx.x / p.split, b = blk / p.row_blocks, i0 = (blk - b * p.row_blocks) * kRowBlock;
+  const int64_t blk = blockIdx.x / p.split, b = blk / p.row_blocks, i0 = (blk - b * p.row_blocks) * ROWS;
   const int64_t k0 = rank * p.k_per, k1 = min(k0 + p.k_per, p.g.K);
-  const int64_t il = i0 + (VEC ? lane * 8 : lane);  // this lane's rows: 8 neighbours, or every 32nd
+  const int64_t il = i0 + (VEC ? lane * 8 : lane);  // this lane's rows: 8 neighbours, or every LR-th
   const T* P = static_cast<const T*>(p.g.P.p) + b * p.g.P.bs;
   const T* Q = static_cast<const T*>(p.g.Q.p) + b * p.g.Q.bs + p.j0 * p.g.Q.rs;
   const int nj = (int)min((int64_t)JT, p.g.J - p.j0);
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_row_kernel(const __grid
         xs[k][j] = k < n && j < nj ? to_f32(Q[j * p.g.Q.rs + (ks + k) * p.g.Q.ks]) : 0.f;
     __syncthreads();
 #pragma unroll 4
-    for (int k = warp; k < n; k += kWarps) {
+    for (int k = kg; k < n; k += kWarps * KG) {
       const T* at = P + (ks + k) * p.g.P.ks;
       float w[8];
       if constexpr (VEC) {
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_row_kernel(const __grid
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) w[c] = il + 32 * c < p.g.I ? to_f32(at[(il + 32 * c) * p.g.P.rs]) : 0.f;
+        for (int c = 0; c < 8; ++c) w[c] = il + LR * c < p.g.I ? to_f32(at[(il + LR * c) * p.g.P.rs]) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
@@ -179,17 +180,19 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_row_kernel(const __grid
   for (int j = 0; j < JT; ++j) {
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < 8; ++c) red[warp][VEC ? lane * 8 + c : lane + 32 * c] = acc[c][j];
+    for (int c = 0; c < 8; ++c) red[kg][VEC ? lane * 8 + c : lane + LR * c] = acc[c][j];
     __syncthreads();
-    float t = 0.f;
+    if (threadIdx.x < ROWS) {
+      float t = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) t += red[w][threadIdx.x];
-    part[j][threadIdx.x] = t;
+      for (int w = 0; w < kWarps * KG; ++w) t += red[w][threadIdx.x];
+      part[j][threadIdx.x] = t;
+    }
   }
   if (p.split > 1) cluster_barrier();
   else __syncthreads();
   // each CTA of the cluster finishes its share of the rows
-  const int share = kRowBlock / p.split;
+  const int share = ROWS / p.split;
   for (int t = threadIdx.x; t < share * JT; t += kSkinnyThreads) {
     const int j = t / share, r = rank * share + t % share;
     if (i0 + r < p.g.I && j < nj) {
@@ -227,8 +230,8 @@ cudaError_t launch_j(SkinnyParams p, int sms, cudaStream_t s) {
   const bool rows_inner = g.P.rs < g.P.ks && g.I > 1;
   p.split = 1;
   if (!rows_inner) {
-    // About 14 warps an SM keep HBM busy (8192 x 8192 bf16 against one token: 38 us with CTAs of 8 warps, of which an SM
-    // gets 3 or 4, 24 us with CTAs of 2): rows are shared by more warps until there are that many, then k by a cluster.
+    // A dozen warps an SM, in CTAs as small as that allows: rows are shared by more warps until there are that many,
+    // then k by a cluster.
     const int64_t groups = g.batch * ((g.I + kRows - 1) / kRows), want = 12 * (int64_t)sms;
     p.warp_split = 1;
     while (p.warp_split < kWarps && groups * p.warp_split < want && g.K > p.warp_split * 256) p.warp_split *= 2;
@@ -242,13 +245,19 @@ cudaError_t launch_j(SkinnyParams p, int sms, cudaStream_t s) {
     return vec ? launch_cluster(skinny_k_kernel<T, JT, true>, p, ctas, p.warps, s)
                : launch_cluster(skinny_k_kernel<T, JT, false>, p, ctas, p.warps, s);
   }
-  p.row_blocks = (g.I + kRowBlock - 1) / kRowBlock;
+  // 256 rows a CTA, or 64 where that leaves SMs idle
+  const int rows = g.batch * ((g.I + 255) / 256) * 8 < sms ? 64 : 256;
+  p.row_blocks = (g.I + rows - 1) / rows;
   const int64_t blocks = g.batch * p.row_blocks;
   while (p.split < 8 && blocks * p.split < 2 * (int64_t)sms && g.K > p.split * 64) p.split *= 2;
   p.k_per = ((g.K + p.split - 1) / p.split + 7) / 8 * 8;
   const bool vec = g.P.rs == 1 && on16(g.P, g.P.ks) && g.I % PER == 0;
-  return vec ? launch_cluster(skinny_row_kernel<T, JT, true>, p, blocks * p.split, kWarps, s)
-             : launch_cluster(skinny_row_kernel<T, JT, false>, p, blocks * p.split, kWarps, s);
+  const int64_t ctas = blocks * p.split;
+  if (rows == 64)
+    return vec ? launch_cluster(skinny_row_kernel<T, JT, true, 64>, p, ctas, kWarps, s)
+               : launch_cluster(skinny_row_kernel<T, JT, false, 64>, p, ctas, kWarps, s);
+  return vec ? launch_cluster(skinny_row_kernel<T, JT, true, 256>, p, ctas, kWarps, s)
+             : launch_cluster(skinny_row_kernel<T, JT, false, 256>, p, ctas, kWarps, s);
 }
 
 template <typename T>

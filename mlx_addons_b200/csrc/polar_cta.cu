@@ -71,18 +71,23 @@ __device__ __forceinline__ uint64_t block_desc(uint32_t addr, int inner) {
 }
 
 template <int PLANES>
-__device__ __forceinline__ void store_unit(unsigned char* buf, int plane_bytes, int off, const float (&v)[8]) {
-  __align__(16) __half2 h[4], l[4];
+__device__ __forceinline__ void halves(const float (&v)[8], __half2 (&h)[PLANES][4]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+    h[0][k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
     if constexpr (PLANES == 2) {
-      const float2 f = __half22float2(h[k]);
-      l[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
+      const float2 f = __half22float2(h[0][k]);
+      h[1][k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
     }
   }
-  *reinterpret_cast<uint4*>(buf + off) = *reinterpret_cast<const uint4*>(h);
-  if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(buf + plane_bytes + off) = *reinterpret_cast<const uint4*>(l);
+}
+template <int PLANES>
+__device__ __forceinline__ void store_unit(unsigned char* buf, int plane_bytes, int off, const float (&v)[8]) {
+  __align__(16) __half2 h[PLANES][4];
+  halves<PLANES>(v, h);
+#pragma unroll
+  for (int pl = 0; pl < PLANES; ++pl)
+    *reinterpret_cast<uint4*>(buf + pl * plane_bytes + off) = *reinterpret_cast<const uint4*>(h[pl]);
 }
 
 // hi + lo of 8 columns.
@@ -124,22 +129,11 @@ __device__ __forceinline__ void peer_load8(const float* p, int q, float (&v)[8])
 __device__ __forceinline__ void peer_store_float(float* p, int q, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_rank(smem_u32(p), q)), "f"(v) : "memory");
 }
-template <int PLANES>
-__device__ __forceinline__ void peer_store_unit(unsigned char* buf, int plane_bytes, int off, int q, const float (&v)[8]) {
-  __align__(16) __half2 h[4], l[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-    const float2 f = __half22float2(h[k]);
-    l[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
-  }
-#pragma unroll
-  for (int pl = 0; pl < PLANES; ++pl) {
-    const uint4 w = *reinterpret_cast<const uint4*>(pl ? l : h);
-    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(map_rank(smem_u32(buf + pl * plane_bytes + off), q)),
-                 "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                 : "memory");
-  }
+__device__ __forceinline__ void peer_store16(unsigned char* p, int q, const void* v) {
+  const uint4 w = *reinterpret_cast<const uint4*>(v);
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(map_rank(smem_u32(p), q)), "r"(w.x), "r"(w.y),
+               "r"(w.z), "r"(w.w)
+               : "memory");
 }
 
 // 8 elements of a row, zeros past its end.
@@ -378,11 +372,13 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
         if (r >= p.kk || c8 * 8 + 8 <= m * p.side || c8 * 8 >= m * p.side + p.side) continue;
         float v[8] = {};
         const float* at = partial + r * p.ppitch + c8 * 8;
-        for (int q = 0; q < p.cl; ++q) {
-          float w[8];
-          peer_load8(at, q, w);
+        // from this CTA's own part on, so that the CTAs read from different ones, two at a time
+        for (int q = 0; q < p.cl; q += 2) {
+          float w[2][8];
+          peer_load8(at, (rank + q) & (p.cl - 1), w[0]);
+          peer_load8(at, (rank + q + 1) & (p.cl - 1), w[1]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += w[e];
+          for (int e = 0; e < 8; ++e) v[e] += w[0][e] + w[1][e];
         }
         float d = 0.f;
         if constexpr (kSplitDiag) {
@@ -391,12 +387,16 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
             if (c8 * 8 + e == r) d = v[e] * (kUnitS / k.k1), v[e] = 0.f;
         }
         const bool diag = kSplitDiag && r - c8 * 8 >= 0 && r - c8 * 8 < 8;
-        for (int q = 0; q < p.cl; ++q) {
-          peer_store_unit<PLANES>(S, s_plane, unit_off(r, c8), q, v);
+        __align__(16) __half2 h[PLANES][4];
+        halves<PLANES>(v, h);
+        for (int i = 0; i < p.cl; ++i) {
+          const int q = (rank + i) & (p.cl - 1);
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl) peer_store16(S + pl * s_plane + unit_off(r, c8), q, h[pl]);
           if (diag) peer_store_float(&sdiag[r], q, d);
         }
       }
-      asm volatile("fence.proxy.async;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");
       __syncwarp();
       cluster_sync();
     } else {

@@ -2,10 +2,10 @@
 // one launch: a cooperative grid of one CTA an SM walks the three products of
 // each step (S, P, X'), with a barrier of the grid between them.
 //
-// With a launch for each product, 15 of them take 11 us each however small
-// they are: about 3 for the launch and its set-up and 5 for an epilogue whose
-// instructions all come from memory, since a kernel runs its epilogue once. Here both are
-// paid once (3 x 1000 x 517 float32: 275 us as launches).
+// With a launch for each product, 17 launches take about 10 us each however
+// small they are: about 3 for the launch and its set-up and 5 for an epilogue whose
+// instructions all come from memory, since a kernel runs its epilogue once. Here
+// both are paid once (256 x 256 bf16: 115 us against 182, 8 x 256 x 1024 bf16: 148 against 231).
 //
 // Roles in a CTA as in gemm_tc.cu: a thread of loads, one of products, eight
 // epilogue warps, which also meet the barrier: their stores, then a fence that
@@ -427,12 +427,18 @@ cudaError_t launch_g(const GridMaps& maps, const GridParams& p, int grid, size_t
 
 }  // namespace
 
-// Up to two rounds of 128 x 128 tiles of X: beyond that the products are long
-// enough for launches of their own, in pairs of CTAs, whose tiles read half as
-// much (one 2048 x 2048 bf16: 392 us as launches).
+// Where the launches cost more than what their pairs of CTAs save, whose tiles
+// read half as much. With one plane (bf16) that is up to two rounds of 128 x 128
+// tiles of X (2048 x 2048: 328 us against 396 as launches), and eight of a side
+// up to 1024 (64 x 512 x 512: 651 against 757; but 2 x 2048 x 2048: 540 against 482).
+// With two planes the products take three times as long: up to one round of a
+// side up to 256 (256 x 256: 149 against 166, 8 x 200 x 260: 160 against 184; but
+// 1000 x 517: 238 against 216, 64 x 256 x 256: 421 against 338).
 bool polar_grid_fits(const PolarParams& p, int sms) {
-  const int64_t tiles = p.batch * ((p.m + 127) / 128) * ((p.n + 127) / 128);
-  return tiles <= 2 * (int64_t)sms && p.steps <= kMaxStepsG;
+  const int64_t tiles = p.batch * ((p.m + 127) / 128) * ((p.n + 127) / 128), side = p.m < p.n ? p.m : p.n;
+  const bool one = p.dtype == B2C_BF16;
+  const int rounds = one ? (side <= 1024 ? 8 : 2) : side <= 256 ? 1 : 0;
+  return tiles <= rounds * (int64_t)sms && p.steps <= kMaxStepsG;
 }
 
 cudaError_t launch_polar_grid(const PolarParams& in, const PolarScratch& w, int sms, cudaStream_t s) {

@@ -77,6 +77,20 @@ def test_many_tiles(M, K, N, batch, ta, tb, dtype):
     check(Y, y, ey, "Y", K)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,batch", [(145, 449, 148, 0), (65, 128, 64, 0), (129, 255, 97, 0), (256, 1024, 255, 0), (33, 700, 40, 9),
+                                         (77, 150, 30, 31), (13, 2100, 192, 0), (4, 3001, 70, 0), (7, 640, 64, 5)])
+def test_sums_split_over_a_cluster(M, K, N, batch, dtype):
+    """Few tiles and a long k, in every order of the operands."""
+    for ta, tb in [(False, False), (False, True), (True, False), (True, True)]:
+        A, B, bias, R = _problem(M, K, N, dtype, (batch,) if batch else (), shared=not batch, trans_a=ta, trans_b=tb)
+        Y, pre = la.gemm(A, B, bias, "gelu_tanh", R, alpha=-0.5, beta=2.0, return_pre=True)
+        y, p, ey, ep = gemm64(A, B, bias, "gelu_tanh", R, -0.5, 2.0)
+        check(pre, p, ep, "pre", K)
+        check(Y, y, ey, "Y", K)
+        assert torch.equal(la.gemm(A, B, bias, "gelu_tanh", R, alpha=-0.5, beta=2.0), Y)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N", [(1, 96), (70, 40), (160, 144)])
