@@ -50,27 +50,50 @@ __device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
   return v;
 }
 
+// How P's rows are read: any way, in 16-byte units, or units that stay out of L1,
+// which then holds Q (533 MB of P with 9 columns: 178 us a pass of 8 against 245;
+// where L2 holds P, 64 MB, units that go through L1 are faster, 34 us against 41).
+enum SkinnyLoads { kAny, kUnits, kStream };
+template <bool STREAM>
+__device__ __forceinline__ uint4 load16(const void* p) {
+  if constexpr (STREAM) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+  }
+  return __ldg(reinterpret_cast<const uint4*>(p));
+}
+
 // Eight k of one row: neighbours (VEC, whole 16-byte units) or every 32nd.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool STREAM>
 __device__ __forceinline__ void load_k8(const T* row, int64_t ks, int64_t k, int64_t end, bool in, float (&v)[8]) {
   if constexpr (VEC) {
     constexpr int PER = 16 / sizeof(T);
 #pragma unroll
     for (int q = 0; q < 8 / PER; ++q) {
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (in && k + q * PER < end) w = __ldg(reinterpret_cast<const uint4*>(row + k + q * PER));
+      if (in && k + q * PER < end) w = load16<STREAM>(row + k + q * PER);
       const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
       for (int c = 0; c < PER; ++c) v[q * PER + c] = to_f32(e[c]);
     }
   } else {
+    // every load is issued, past the end that of the first k again: none waits for a branch
+    const T* at = row + k * ks;
+    const int left = (int)min((end - k + 31) / 32, (int64_t)8);
+    T t[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) v[c] = in && k + 32 * c < end ? to_f32(row[(k + 32 * c) * ks]) : 0.f;
+    for (int c = 0; c < 8; ++c) t[c] = at[c < left ? c * 32 * ks : 0];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v[c] = in && c < left ? to_f32(t[c]) : 0.f;
   }
 }
 
-template <typename T, int JT, bool VEC>
+template <typename T, int JT, int LOADS>
 __global__ void __launch_bounds__(kSkinnyThreads) skinny_k_kernel(const __grid_constant__ SkinnyParams p) {
+  constexpr bool VEC = LOADS != kAny;
   __shared__ float part[kWarps * kRows * JT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t rank = p.split > 1 ? ctarank() : 0;
@@ -88,11 +111,11 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_k_kernel(const __grid_c
   for (int64_t k = k0 + sub * 256 + (VEC ? lane * 8 : lane); k < k1; k += ws * 256) {
     float w[kRows][8];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) load_k8<T, VEC>(P + (i0 + r) * p.g.P.rs, p.g.P.ks, k, k1, i0 + r < p.g.I, w[r]);
+    for (int r = 0; r < kRows; ++r) load_k8<T, VEC, LOADS == kStream>(P + (i0 + r < p.g.I ? i0 + r : 0) * p.g.P.rs, p.g.P.ks, k, k1, i0 + r < p.g.I, w[r]);
 #pragma unroll
     for (int j = 0; j < JT; ++j) {
       float x[8];
-      load_k8<T, VEC>(Q + j * p.g.Q.rs, p.g.Q.ks, k, k1, j < nj, x);
+      load_k8<T, VEC, false>(Q + (j < nj ? j : 0) * p.g.Q.rs, p.g.Q.ks, k, k1, j < nj, x);
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
@@ -165,8 +188,11 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_row_kernel(const __grid
           for (int c = 0; c < PER; ++c) w[q * PER + c] = to_f32(e[c]);
         }
       } else {
+        T t[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) w[c] = il + LR * c < p.g.I ? to_f32(at[(il + LR * c) * p.g.P.rs]) : 0.f;
+        for (int c = 0; c < 8; ++c) t[c] = at[(il + LR * c < p.g.I ? il + LR * c : i0) * p.g.P.rs];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) w[c] = il + LR * c < p.g.I ? to_f32(t[c]) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
@@ -242,8 +268,10 @@ cudaError_t launch_j(SkinnyParams p, int sms, cudaStream_t s) {
     p.row_blocks = (g.I + rows - 1) / rows;
     const int64_t ctas = g.batch * p.row_blocks * p.split;
     const bool vec = g.P.ks == 1 && g.Q.ks == 1 && on16(g.P, g.P.rs) && on16(g.Q, g.Q.rs) && g.K % PER == 0;
-    return vec ? launch_cluster(skinny_k_kernel<T, JT, true>, p, ctas, p.warps, s)
-               : launch_cluster(skinny_k_kernel<T, JT, false>, p, ctas, p.warps, s);
+    const bool stream = JT > 1 && g.batch * g.I * g.K * sizeof(T) > (96u << 20);
+    return !vec     ? launch_cluster(skinny_k_kernel<T, JT, kAny>, p, ctas, p.warps, s)
+           : stream ? launch_cluster(skinny_k_kernel<T, JT, kStream>, p, ctas, p.warps, s)
+                    : launch_cluster(skinny_k_kernel<T, JT, kUnits>, p, ctas, p.warps, s);
   }
   // 256 rows a CTA, or 64 where that leaves SMs idle
   const int rows = g.batch * ((g.I + 255) / 256) * 8 < sms ? 64 : 256;

@@ -433,12 +433,14 @@ cudaError_t launch_g(const GridMaps& maps, const GridParams& p, int grid, size_t
 // up to 1024 (64 x 512 x 512: 651 against 757; but 2 x 2048 x 2048: 540 against 482).
 // With two planes the products take three times as long: up to one round of a
 // side up to 256 (256 x 256: 149 against 166, 8 x 200 x 260: 160 against 184; but
-// 1000 x 517: 238 against 216, 64 x 256 x 256: 421 against 338).
+// 1000 x 517: 238 against 216, 64 x 256 x 256: 421 against 338). A long side makes few
+// and long products of S, which only launches of their own split.
 bool polar_grid_fits(const PolarParams& p, int sms) {
-  const int64_t tiles = p.batch * ((p.m + 127) / 128) * ((p.n + 127) / 128), side = p.m < p.n ? p.m : p.n;
+  const int64_t tiles = p.batch * ((p.m + 127) / 128) * ((p.n + 127) / 128);
+  const int64_t side = p.m < p.n ? p.m : p.n, along = p.m < p.n ? p.n : p.m;
   const bool one = p.dtype == B2C_BF16;
   const int rounds = one ? (side <= 1024 ? 8 : 2) : side <= 256 ? 1 : 0;
-  return tiles <= rounds * (int64_t)sms && p.steps <= kMaxStepsG;
+  return tiles <= rounds * (int64_t)sms && along <= (one ? 4096 : 1024) && p.steps <= kMaxStepsG;
 }
 
 cudaError_t launch_polar_grid(const PolarParams& in, const PolarScratch& w, int sms, cudaStream_t s) {
