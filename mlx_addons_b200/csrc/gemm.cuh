@@ -1,5 +1,5 @@
 // Matrix products with an epilogue: types and device helpers shared by
-// gemm_simt.cu, gemm_tc.cu, gemm_dact.cu and polar.cu.
+// the gemm_*.cu and polar*.cu files.
 //
 // Every product is written as D[i, j] = sum_k P[i, k] Q[j, k] on two operands
 // with free strides; the caller of b2c_gemm has P = A, Q = B^T, or the other

@@ -7,7 +7,7 @@
 // in its tensor memory. The pairs are persistent, one CTA an SM, and tensor
 // memory holds two accumulators, so the epilogue of a tile runs under the MMAs
 // of the next. Where D is too small for that, single CTAs compute 128 x BN
-// tiles, several to an SM, and k may be split over a cluster of up to 8 of
+// tiles, several to an SM, and k may be split over a cluster of up to 4 of
 // them, whose partial sums are joined in order through distributed shared
 // memory.
 //
