@@ -46,8 +46,12 @@ __device__ __forceinline__ void load8(const void* p, int64_t off, int64_t cs, in
       for (int k = 0; k < PER; ++k) v[u * PER + k] = to_f32(e[k]);
     }
   } else {
+    // every load is issued, past the end that of c again: none waits for a branch
+    T t[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + 32 * k < N ? to_f32(q[(c + 32 * k) * cs]) : 0.f;
+    for (int k = 0; k < 8; ++k) t[k] = q[(c + 32 * k < N ? c + 32 * k : c) * cs];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + 32 * k < N ? to_f32(t[k]) : 0.f;
   }
 }
 

@@ -50,8 +50,12 @@ __global__ void __launch_bounds__(256) gemm_pack_kernel(const PackParams p) {
     if constexpr (F32) {
       const float* s = static_cast<const float*>(p.src) + src;
       __align__(16) uint16_t h[8], m[8], l[8];
+      // every load is issued, past the end that of the first again: none waits for a branch
+      float x[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) thirds(c < n ? s[c * p.is] : 0.f, h[c], m[c], l[c]);
+      for (int c = 0; c < 8; ++c) x[c] = s[c < n ? c * p.is : 0];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) thirds(c < n ? x[c] : 0.f, h[c], m[c], l[c]);
       *reinterpret_cast<uint4*>(p.dst + dst) = *reinterpret_cast<const uint4*>(h);
       *reinterpret_cast<uint4*>(p.dst + p.plane + dst) = *reinterpret_cast<const uint4*>(m);
       *reinterpret_cast<uint4*>(p.dst + 2 * p.plane + dst) = *reinterpret_cast<const uint4*>(l);
@@ -59,7 +63,9 @@ __global__ void __launch_bounds__(256) gemm_pack_kernel(const PackParams p) {
       const uint16_t* s = static_cast<const uint16_t*>(p.src) + src;
       __align__(16) uint16_t h[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) h[c] = c < n ? s[c * p.is] : (uint16_t)0;
+      for (int c = 0; c < 8; ++c) h[c] = s[c < n ? c * p.is : 0];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) h[c] = c < n ? h[c] : (uint16_t)0;
       *reinterpret_cast<uint4*>(p.dst + dst) = *reinterpret_cast<const uint4*>(h);
     }
   }

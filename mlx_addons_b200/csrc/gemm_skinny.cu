@@ -268,10 +268,11 @@ cudaError_t launch_j(SkinnyParams p, int sms, cudaStream_t s) {
     p.row_blocks = (g.I + rows - 1) / rows;
     const int64_t ctas = g.batch * p.row_blocks * p.split;
     const bool vec = g.P.ks == 1 && g.Q.ks == 1 && on16(g.P, g.P.rs) && on16(g.Q, g.Q.rs) && g.K % PER == 0;
-    const bool stream = JT > 1 && g.batch * g.I * g.K * sizeof(T) > (96u << 20);
-    return !vec     ? launch_cluster(skinny_k_kernel<T, JT, kAny>, p, ctas, p.warps, s)
-           : stream ? launch_cluster(skinny_k_kernel<T, JT, kStream>, p, ctas, p.warps, s)
-                    : launch_cluster(skinny_k_kernel<T, JT, kUnits>, p, ctas, p.warps, s);
+    if constexpr (sizeof(T) == 4 && JT > 1)  // 16-bit products of this form are small
+      if (vec && g.batch * g.I * g.K * 4 > (96 << 20))
+        return launch_cluster(skinny_k_kernel<T, JT, kStream>, p, ctas, p.warps, s);
+    return vec ? launch_cluster(skinny_k_kernel<T, JT, kUnits>, p, ctas, p.warps, s)
+               : launch_cluster(skinny_k_kernel<T, JT, kAny>, p, ctas, p.warps, s);
   }
   // 256 rows a CTA, or 64 where that leaves SMs idle
   const int rows = g.batch * ((g.I + 255) / 256) * 8 < sms ? 64 : 256;

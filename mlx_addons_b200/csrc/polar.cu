@@ -65,8 +65,12 @@ __device__ __forceinline__ void load_unit(const PolarIn& in, const T* row, int64
       for (int k = 0; k < PER; ++k) v[q * PER + k] = to_f32(e[k]);
     }
   } else {
+    // every load is issued, past the end that of c again: none waits for a branch
+    T t[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < in.n ? to_f32(row[(c + k) * in.cs]) : 0.f;
+    for (int k = 0; k < 8; ++k) t[k] = row[(c + k < in.n ? c + k : c) * in.cs];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < in.n ? to_f32(t[k]) : 0.f;
   }
 }
 

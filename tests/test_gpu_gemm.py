@@ -349,3 +349,32 @@ def test_training_step(dtype):
         unit = 2.0**-12 if dtype == BF16 else 2.0**-23
         bound = orth_bound([x[None] for x in its], 5, MUON, unit, dtype)
         assert float(torch.linalg.matrix_norm(u.double() - ref)) <= float(bound)
+
+
+@pytest.mark.parametrize("K", [8, 64])
+def test_offsets_beyond_32_bits(K):
+    """More outputs than 31 bits count, by the FP32 units and by the tensor cores, and the epilogue's gradient on them."""
+    M, N = 70001, 31000
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    g = _gen(K)
+    A, B = _rand(g, M, K, dtype=BF16), _rand(g, K, N, dtype=BF16, scale=1 / math.sqrt(K))
+    Y, pre = la.gemm(A, B, None, "gelu", return_pre=True)
+    rows = torch.tensor([0, 1, 34000, 69270, 69273, 69999, 70000], device=DEV)
+    y, p, ey, ep = gemm64(A[rows], B, None, "gelu")
+    check(pre[rows], p, ep, "pre", K)
+    check(Y[rows], y, ey, "Y", K)
+    dA = la.gemm_grad(Y, A, B, pre, "gelu")[0]
+    # the same rows alone: every sum runs over N in an order that the sizes choose, so up to its own rounding
+    ref = la.gemm_grad(Y[rows], A[rows], B, pre[rows], "gelu")[0].double()
+    rel = float((dA[rows].double() - ref).norm() / ref.norm())
+    assert rel <= 2 * (2.0**-8 + 2.0**-23 * (math.sqrt(N) + 32))
+
+
+@pytest.mark.parametrize("M", [2, 4, 11])
+def test_thin_products_of_long_streams(M):
+    """Weights that no cache holds, read as they lie and transposed."""
+    g = _gen(M)
+    A, W = _rand(g, M, 5300), _rand(g, 5200, 5300, scale=1 / math.sqrt(5300))
+    for B in (W.mT, _rand(g, 5300, 5200, scale=1 / math.sqrt(5300))):
+        check(la.gemm(A, B), *_plain(A, B), what="Y", K=5300)

@@ -60,7 +60,7 @@ def test_products(monkeypatch, M, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("shape", [(50, 40, 64), (2, 300, 500)])
+@pytest.mark.parametrize("shape", [(50, 40, 64), (20, 100, 600), (2, 140, 500), (2, 300, 5000)])
 def test_orthogonalisation(monkeypatch, shape, dtype):
     g = torch.Generator(device=DEV).manual_seed(3)
     G = torch.randn(*shape, generator=g, device=DEV).to(dtype)

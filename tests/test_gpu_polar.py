@@ -253,3 +253,18 @@ def test_many_matrices(dtype):
     out = la.orthogonalize(G)
     pick = torch.tensor([0, 1, 65534, 65535, 65536, 69999], device=DEV)
     _check(out[pick], G[pick])
+
+
+def test_offsets_beyond_32_bits():
+    """More elements than 31 bits count, in small matrices and in one of a product's tiles."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    G = torch.randn(540000, 64, 64, device=DEV, dtype=BF16)
+    out = la.orthogonalize(G)
+    pick = torch.tensor([0, 524287, 524288, 524289, 539999], device=DEV)
+    _check(out[pick], G[pick])
+    del out
+    G = G.reshape(9000, 240, 1024)
+    out = la.orthogonalize(G)
+    pick = torch.tensor([0, 8737, 8738, 8999], device=DEV)
+    _check(out[pick], G[pick])
