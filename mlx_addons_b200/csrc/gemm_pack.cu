@@ -112,8 +112,10 @@ cudaError_t launch_pack(int dtype, const GemmOperand& o, const PackPlan& plan, v
   const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
   const bool vec = p.is == 1 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0 && p.os % 4 == 0 && p.bs % 4 == 0;
   // rows that follow one another without a gap are one row
-  if (p.is == 1 && p.os == p.inner && p.pitch == p.inner) p.inner *= p.outer, p.pitch = p.inner, p.os = p.inner, p.outer = 1;
-  if (p.outer == 1 && p.bs == p.inner && p.pitch == p.inner) p.inner *= p.batch, p.pitch = p.inner, p.batch = 1;
+  if (p.is == 1 && p.pitch == p.inner) {
+    if (p.os == p.inner) p.inner *= p.outer, p.pitch = p.inner, p.outer = 1;
+    if (p.outer == 1 && p.bs == p.inner) p.inner *= p.batch, p.pitch = p.inner, p.batch = 1;
+  }
   if (dtype != B2C_F32) gemm_pack_kernel<false, false><<<grid, 256, 0, s>>>(p);
   else if (vec) gemm_pack_kernel<true, true><<<grid, 256, 0, s>>>(p);
   else gemm_pack_kernel<true, false><<<grid, 256, 0, s>>>(p);

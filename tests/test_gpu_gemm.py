@@ -136,6 +136,21 @@ def test_strides(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_expanded_operands(dtype):
+    """Strides of 0 in every place, their batch stride that of whole rows among them."""
+    g = _gen(5)
+    for b, M, K, N in [(4, 1, 1024, 1024), (3, 40, 256, 512), (5, 200, 136, 264), (2, 24, 2048, 640)]:
+        t, B = _rand(g, b, K, dtype=dtype), _rand(g, b, K, N, dtype=dtype, scale=1 / K)
+        for A in (t[:, :1].unsqueeze(1).expand(b, M, K), t.unsqueeze(1).expand(b, M, K),
+                  _rand(g, b, M, 1, dtype=dtype).expand(b, M, K), _rand(g, 1, M, K, dtype=dtype).expand(b, M, K),
+                  _rand(g, b * M, K, dtype=dtype).as_strided((b, M, K), (K, K, 1))):
+            Y = la.gemm(A, B)
+            check(Y, *_plain(A, B), what=(A.stride(), M), K=K)
+            Z = la.gemm(B.mT, A.mT)
+            check(Z, *_plain(B.mT, A.mT), what=(A.stride(), M, "right"), K=K)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_empty(dtype):
     z = lambda *s: torch.zeros(*s, device=DEV, dtype=dtype)  # noqa: E731
     assert la.gemm(z(0, 5), z(5, 3)).shape == (0, 3)
