@@ -72,11 +72,11 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(what, fn, args, ws_fn, ws_args, dev):
+def _call(what, fn, args, ws_fn, ws_args, dev, scratch=False):
     """fn(*args, workspace, bytes, stream); a call that needs scratch says so
-    before it launches anything."""
+    before it launches anything, unless it is known to need some."""
     stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    rc = fn(*args, None, 0, stream)
+    rc = _lib.B2C_ERR_WORKSPACE if scratch else fn(*args, None, 0, stream)
     if rc == _lib.B2C_ERR_WORKSPACE:
         n = ws_fn(*ws_args)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -224,7 +224,7 @@ def gemm_grad(dY, A, B, pre=None, activation: Optional[str] = None, *, alpha: fl
         with _guard(dev):
             _call("b2c_gemm_dact", lib.b2c_gemm_dact,
                   (_DTYPES[At.dtype], dy, p, act, float(beta), _addr(dP) if act else None, _addr(dbias), _addr(dR), batch,
-                   rows, N), lib.b2c_gemm_dact_workspace_size, (batch, rows, N), dev)
+                   rows, N), lib.b2c_gemm_dact_workspace_size, (batch, rows, N), dev, need_bias)
     dA, _ = _gemm_dev(dP, B3.mT, None, 0, None, float(alpha), 1.0, False)
     dB, _ = _gemm_dev(A3.mT, dP, None, 0, None, float(alpha), 1.0, False)
     if len(lead) > 1 or (lead and shared):
