@@ -152,40 +152,58 @@ __global__ void __launch_bounds__(kSimtThreads) gemm_simt_kernel(const __grid_co
   }
   const int64_t i = i0 + ti * 8, j = j0 + (VEC ? tj * 4 : tj);
   constexpr int JS = VEC ? 1 : 16;  // columns between a thread's four
+  const GemmEpilogue& e = g.e;
+  const bool alone = !e.bias && !e.pre.p && !e.res.p && e.act == B2C_ACT_NONE;
+  const int rows = g.I - i < 8 ? (int)(g.I - i) : 8;
   if (VEC && j + 4 <= g.J) {
-    const GemmEpilogue& e = g.e;
+    T* y = static_cast<T*>(e.y.p) + b * e.y.bs + i * e.y.is + j;
+    Four<T> u;
+    if (alone) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r, y += e.y.is) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) u.v[c] = from_f32<T>(e.alpha * acc[r][c]);
+        if (r < rows) *reinterpret_cast<Four<T>*>(y) = u;
+      }
+      return;
+    }
+    T* pre = static_cast<T*>(e.pre.p) + b * e.pre.bs + i * e.pre.is + j;
+    const T* res = static_cast<const T*>(e.res.p) + b * e.res.bs + i * e.res.is + j;
     float bias[4] = {};
     if (e.bias && !e.bias_on_i)
 #pragma unroll
       for (int c = 0; c < 4; ++c) bias[c] = to_f32(static_cast<const T*>(e.bias)[j + c]);
+    // all addends are asked for before anything is stored
+    Four<T> x[8];
+    if (e.res.p)
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      if (i + r >= g.I) break;
+      for (int r = 0; r < 8; ++r)
+        if (r < rows) x[r] = *reinterpret_cast<const Four<T>*>(res + r * e.res.is);
+#pragma unroll
+    for (int r = 0; r < 8; ++r, y += e.y.is, pre += e.pre.is) {
+      if (r >= rows) break;
       if (e.bias && e.bias_on_i) bias[0] = bias[1] = bias[2] = bias[3] = to_f32(static_cast<const T*>(e.bias)[i + r]);
       float v[4];
-      Four<T> u;
 #pragma unroll
       for (int c = 0; c < 4; ++c) v[c] = fmaf(e.alpha, acc[r][c], bias[c]);
       if (e.pre.p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) u.v[c] = from_f32<T>(v[c]);
-        *reinterpret_cast<Four<T>*>(static_cast<T*>(e.pre.p) + b * e.pre.bs + (i + r) * e.pre.is + j) = u;
+        *reinterpret_cast<Four<T>*>(pre) = u;
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) v[c] = act_f32<sizeof(T) == 2>(v[c], e.act);
       if (e.res.p) {
-        u = *reinterpret_cast<const Four<T>*>(static_cast<const T*>(e.res.p) + b * e.res.bs + (i + r) * e.res.is + j);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = fmaf(e.beta, to_f32(u.v[c]), v[c]);
+        for (int c = 0; c < 4; ++c) v[c] = fmaf(e.beta, to_f32(x[r].v[c]), v[c]);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) u.v[c] = from_f32<T>(v[c]);
-      *reinterpret_cast<Four<T>*>(static_cast<T*>(e.y.p) + b * e.y.bs + (i + r) * e.y.is + j) = u;
+      *reinterpret_cast<Four<T>*>(y) = u;
     }
     return;
   }
-  const GemmEpilogue& e = g.e;
-  if (!VEC && !e.bias && !e.pre.p && !e.res.p && e.act == B2C_ACT_NONE && e.y.js == 1) {
+  if (!VEC && alone && e.y.js == 1) {
     // a product alone: nothing but the stores (350 MB of rows of 10755 float32, k = 3: 115 us, 254 by the loop below)
     T* y = static_cast<T*>(e.y.p) + b * e.y.bs + i * e.y.is + j;
 #pragma unroll
@@ -197,7 +215,6 @@ __global__ void __launch_bounds__(kSimtThreads) gemm_simt_kernel(const __grid_co
   }
   // a row's addends are asked for before the row above is stored
   const int cols = j >= g.J ? 0 : (int)((g.J - j + JS - 1) / JS < 4 ? (g.J - j + JS - 1) / JS : 4);
-  const int rows = g.I - i < 8 ? (int)(g.I - i) : 8;
   if (cols == 0) return;
   const T* res = static_cast<const T*>(e.res.p) + b * e.res.bs + i * e.res.is + j * e.res.js;
   T* y = static_cast<T*>(e.y.p) + b * e.y.bs + i * e.y.is + j * e.y.js;
