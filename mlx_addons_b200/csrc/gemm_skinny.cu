@@ -188,11 +188,8 @@ __global__ void __launch_bounds__(kSkinnyThreads) skinny_row_kernel(const __grid
           for (int c = 0; c < PER; ++c) w[q * PER + c] = to_f32(e[c]);
         }
       } else {
-        T t[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) t[c] = at[(il + LR * c < p.g.I ? il + LR * c : i0) * p.g.P.rs];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) w[c] = il + LR * c < p.g.I ? to_f32(t[c]) : 0.f;
+        for (int c = 0; c < 8; ++c) w[c] = il + LR * c < p.g.I ? to_f32(at[(il + LR * c) * p.g.P.rs]) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
