@@ -27,10 +27,7 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 
 def _native(x, what, name):
     """Any accepted array as a torch tensor of one of the three types."""
-    if isinstance(x, torch.Tensor):
-        t, kind = x, "torch"
-    else:
-        t, kind = _pkg._as_tensor(x, name)
+    t, kind = _pkg._as_tensor(x, name)
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: {what} requires a gradient, which {name} does not record; detach it or call under "
                          "torch.no_grad() (gemm_grad computes the gradients of gemm)")
