@@ -17,6 +17,7 @@ import sys
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad as _fwad
 
 from .. import _lib
 
@@ -28,9 +29,10 @@ _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _l
 def _native(x, what, name):
     """Any accepted array as a torch tensor of one of the three types."""
     t, kind = _pkg._as_tensor(x, name)
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name}: {what} requires a gradient, which {name} does not record; detach it or call under "
-                         "torch.no_grad() (gemm_grad computes the gradients of gemm)")
+    # no_grad() leaves forward-mode tangents on, so these are refused there too
+    if (t.requires_grad and torch.is_grad_enabled()) or (_fwad._current_level >= 0 and _fwad.unpack_dual(t).tangent is not None):
+        raise ValueError(f"{name}: {what} requires a gradient, which {name} does not record; detach it, or for reverse "
+                         "mode call under torch.no_grad() (gemm_grad computes the gradients of gemm)")
     if t.dtype not in _DTYPES:
         if t.is_complex():
             raise ValueError(f"{name}: {what} is complex")
@@ -146,7 +148,7 @@ def gemm(A, B, bias=None, activation: Optional[str] = None, residual=None, *, al
     ``gemm_grad`` needs of the activation.
 
     float32 products are as exact as float32 arithmetic; 16-bit operands are
-    multiplied exactly and summed in 32 bits. Records no gradient."""
+    multiplied exactly and summed in 32 bits. Records no gradient, in neither mode: operands that carry one are refused."""
     name = "gemm"
     act = _activation(activation, name)
     At, kind = _native(A, "A", name)

@@ -139,3 +139,16 @@ def test_c_orthogonalize_refuses(lib):
     assert call(coef=three(9.0, -6.0, 0.0)) == bad  # 4.24 inside [0, 1], 3 at its end
     assert call(coef=three(1.5, -0.5, 0.0), m=256, n=256) == _lib.B2C_ERR_WORKSPACE  # fine; and no scratch was given
     assert call(m=0) == _lib.B2C_OK and call(batch=0) == _lib.B2C_OK
+
+
+def test_dual_numbers_are_refused():
+    """A tangent of forward-mode differentiation would be lost like a gradient."""
+    fwad = torch.autograd.forward_ad
+    with fwad.dual_level():
+        w = fwad.make_dual(torch.zeros(3, 2), torch.ones(3, 2))
+        for call in (lambda: la.gemm(f(2, 3), w), lambda: la.gemm(t(2, 3), t(3, 2), residual=w[:2]),
+                     lambda: la.gemm_grad(f(2, 2), f(2, 3), w), lambda: la.orthogonalize(w)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+                call()
