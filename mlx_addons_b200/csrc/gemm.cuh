@@ -6,6 +6,8 @@
 // way round where B's columns are the longer side.
 #pragma once
 
+#include <cstdlib>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -155,6 +157,13 @@ inline cudaError_t device_sms(int* sms) {
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   return e == cudaSuccess ? cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) : e;
+}
+
+// Test only: which wait runs out (read per call). 1: one before the first product; in the
+// grid-wide orthogonalisation also 2: one in its last product, 3: the last barrier of its grid.
+inline int injected_timeout() {
+  const char* t = getenv("B2C_GEMM_INJECT_TIMEOUT");
+  return t ? atoi(t) : 0;
 }
 
 // dP = dY act'(pre) (rounded to the type once), and the column sums of the

@@ -26,8 +26,6 @@
 // without that the truncations, all towards zero, add up along k. A slice in
 // shared memory holds all planes, each loaded once for all its products.
 #include <cmath>
-#include <cstdlib>
-#include <cstring>
 
 #include "b2c_kernels.cuh"
 #include "gemm_tile.cuh"
@@ -533,11 +531,6 @@ Form choose_form(const TcProblem& t, int kblocks, int planes, int nseg, int sms)
   return best;
 }
 
-bool inject_timeout() {
-  const char* t = getenv("B2C_GEMM_INJECT_TIMEOUT");
-  return t && strcmp(t, "1") == 0;
-}
-
 }  // namespace
 
 bool tc_direct(const GemmOperand& o, int64_t batch, int64_t rows, int64_t K, TcOperand* out) {
@@ -600,7 +593,7 @@ cudaError_t launch_gemm_tc(const TcProblem& t, cudaStream_t s) {
   p.pre_vec = vec16(t.e.pre, along_i, osize, 0);
   p.res_vec = vec16(t.e.res, along_i, rsize, t.res_plane);
   p.bias_vec = (reinterpret_cast<uintptr_t>(t.e.bias) & 15) == 0;
-  p.inject = inject_timeout();
+  p.inject = injected_timeout() == 1;
   p.chained = t.chained;
   CUtensorMap mp, mq;
   if (!encode(&mp, t.P, t.f16, planes, t.batch, t.I, t.K, BM) ||

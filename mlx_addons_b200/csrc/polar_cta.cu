@@ -22,8 +22,6 @@
 //
 // Bound by the phases of a step in turn (product, conversion of the sums to
 // the next operand, barrier): two CTAs share an SM and fill each other's gaps.
-#include <cstdlib>
-#include <cstring>
 
 #include "b2c_kernels.cuh"
 #include "gemm_tc.cuh"
@@ -566,11 +564,6 @@ __global__ void __launch_bounds__(NT, 512 / NT) polar_cta_kernel(const __grid_co
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
 }
 
-bool inject_timeout() {
-  const char* t = getenv("B2C_GEMM_INJECT_TIMEOUT");
-  return t && strcmp(t, "1") == 0;
-}
-
 template <typename T, int PLANES, int NT, bool CL>
 cudaError_t launch_n(const CtaParams& p, size_t smem, unsigned grid, cudaStream_t s) {
   auto kern = polar_cta_kernel<T, PLANES, NT, CL>;
@@ -667,7 +660,7 @@ cudaError_t launch_polar_cta(const PolarParams& in, int sms, cudaStream_t s) {
   p.along_l = p.sl <= p.sr || p.side == 1;
   p.steps = in.steps;
   p.eps = in.eps;
-  p.inject = inject_timeout();
+  p.inject = injected_timeout() == 1;
   p.lanes_per_row = 1;
   while (p.lanes_per_row < 32 && p.lanes_per_row * 8 < (p.L < p.chunk ? p.L : p.chunk)) p.lanes_per_row *= 2;
   const int64_t per = in.dtype == B2C_F32 ? 4 : 8;

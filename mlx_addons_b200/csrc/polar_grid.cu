@@ -11,9 +11,10 @@
 // epilogue warps, which also meet the barrier: their stores, then a fence that
 // orders them before the other CTAs' TMA loads, a counter in memory, and the
 // word to the loading thread.
+//
+// Every wait is bounded. A CTA whose wait runs out leaves NaN in its own tiles of
+// the result, whichever product it was in; the tiles of a CTA that finished stand.
 #include <cmath>
-#include <cstdlib>
-#include <cstring>
 
 #include "b2c_kernels.cuh"
 #include "gemm_tile.cuh"
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   float* staging = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, tfull0 = empty0 + 8 * kMaxStages,
                  tempty0 = tfull0 + 16, go = tempty0 + 16, never = go + 8;
-  const uint64_t limit = p.inject ? 1000000ull : kWaitNs;
+  const uint64_t limit = p.inject == 1 ? 1000000ull : kWaitNs;
   volatile int* gu = &gave_up;
   if (tid == 0) {
     gave_up = 0;
@@ -260,19 +261,26 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     float* stage = staging + warp * kStageFloats;
     uint32_t buf = 0, tphase = 0;
-    if (p.inject && blockIdx.x == 0) bar_wait(never, 0, gu, limit, &g_grid_fault);
-    for (int f = 0; f < phases; ++f) {
+    if (p.inject == 1 && blockIdx.x == 0) bar_wait(never, 0, gu, limit, &g_grid_fault);
+    for (int f = 0;;) {
       const int st = f / 3, ph = f - 3 * st;
-      if (f == phases - 1 && tid == 0) set_last<PLANES>(cur, p);
-      if (epi_any(*gu != 0)) break;
-      const int kblocks = p.phase[ph].kblocks, BN = p.phase[ph].BN;
       const bool last = f == phases - 1;
+      if (last && tid == 0) set_last<PLANES>(cur, p);
+      // A CTA that gives up goes on to its tiles of the last product and stores NaN for them: the others either give
+      // up at the next barrier, where it is missed, and do the same for theirs, or finish theirs without it.
+      bool ok = !epi_any(*gu != 0);
+      if (!ok && !last) {
+        f = phases - 1;
+        continue;
+      }
+      const int kblocks = p.phase[ph].kblocks, BN = p.phase[ph].BN;
+      if (p.inject == 2 && last && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, 1000000ull, &g_grid_fault));
       for (int64_t t = blockIdx.x; t < p.phase[ph].tiles; t += gridDim.x) {
         const Tile o = phase_tile(p.phase[ph], t);
         float acc[2][32];
-        bool ok = true;
-        for (int kb = 0; kb < (JOIN ? kblocks : 1); ++kb) {
-          ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_grid_fault));
+        for (int kb = 0; kb < (JOIN ? kblocks : 1) && ok; ++kb) {
+          ok = __all_sync(kFull, bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_grid_fault));
+          if (!ok) break;
           fence_after();
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -289,7 +297,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           if (lane == 0) bar_arrive_cluster(tempty0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
-        if (!ok) break;
+        if (!ok) {
+          if (!last) break;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) acc[0][c] = acc[1][c] = __int_as_float(0x7fffffff);
+        }
         // one copy of the epilogue's code: the sums move up instead of the index
 #pragma unroll 1
         for (int q = 0; q < BN / 64; ++q) {
@@ -300,7 +312,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           for (int c = 0; c < 32; ++c) acc[0][c] = acc[1][c];
         }
       }
-      if (last || epi_any(*gu != 0)) break;
+      if (last) break;
+      if (epi_any(*gu != 0)) {
+        f = phases - 1;
+        continue;
+      }
       // ---- barrier of the grid ----
       __threadfence();
       asm volatile("fence.proxy.async;" ::: "memory");
@@ -313,7 +329,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           unsigned int seen;
           asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(p.counter) : "memory");
           if (seen >= target) break;
-          if (now_ns() - t0 > (p.inject ? 3000000ull : kBarrierNs)) {
+          if (now_ns() - t0 > (p.inject == 1 ? 3000000ull : kBarrierNs) || (p.inject == 3 && blockIdx.x == 0 && f == phases - 2)) {
             *gu = 1;
             atomicOr(&g_grid_fault, 1u);
             break;
@@ -322,9 +338,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         asm volatile("fence.proxy.async;" ::: "memory");
         // the loading thread has taken the word before (its CTA may have had no tile, and nothing else keeps it in step)
         while (heard < f && !*gu)
-          if (now_ns() - t0 > 2 * kBarrierNs) *gu = 1;
+          if (now_ns() - t0 > 2 * kBarrierNs) *gu = 1, atomicOr(&g_grid_fault, 1u);
         bar_arrive_cluster(go);
       }
+      ++f;
     }
   } else if (warp == kEpi) {
     // ---- loads ----
@@ -384,25 +401,13 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   }
   __syncwarp();
   __syncthreads();
-  if (gave_up) {
-    // this CTA's part of the result is NaN; it never meets the grid again, so no other CTA passes either
-    settle();
-    __syncthreads();
-    const int64_t total = p.batch * p.mn;
-    for (int64_t e = (int64_t)blockIdx.x * kThreadsG + tid; e < total; e += (int64_t)gridDim.x * kThreadsG)
-      static_cast<T*>(p.out)[e] = from_f32<T>(__int_as_float(0x7fffffff));
-  }
+  if (gave_up) settle();
   fence_before();
   __syncthreads();
   if (warp == kEpi) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
   }
-}
-
-bool inject_timeout() {
-  const char* t = getenv("B2C_GEMM_INJECT_TIMEOUT");
-  return t && strcmp(t, "1") == 0;
 }
 
 template <int PLANES, typename T>
@@ -462,7 +467,7 @@ cudaError_t launch_polar_grid(const PolarParams& in, const PolarScratch& w, int 
   p.out = in.out;
   p.out_rs = in.out_rs, p.out_cs = in.out_cs;
   p.counter = w.counter;
-  p.inject = inject_timeout();
+  p.inject = injected_timeout();
   const int64_t elt = in.dtype == B2C_F32 ? 4 : 2, other = in.out_cs == 1 ? in.out_rs : in.out_cs;
   p.last_vec = (reinterpret_cast<uintptr_t>(in.out) & 15) == 0 && p.mn * elt % 16 == 0 && other * elt % 16 == 0;
   for (int ph = 0; ph < 3; ++ph) {
