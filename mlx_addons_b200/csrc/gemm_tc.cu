@@ -24,7 +24,8 @@
 // cores truncate when they add to an accumulator, so such a product's
 // accumulator is joined in float32 registers after every slice (JOIN):
 // without that the truncations, all towards zero, add up along k. A slice in
-// shared memory holds all planes, each loaded once for all its products.
+// shared memory holds all planes, each loaded once for all its products. One
+// plane is joined too, but rarely and over a long k alone (kJoinAfter).
 #include <cmath>
 
 #include "b2c_kernels.cuh"
@@ -36,23 +37,33 @@ __device__ unsigned int g_gemm_fault;
 
 namespace {
 
+// The tensor cores cut off what they add to an accumulator: a sum of terms of one sign loses 9e-8 of itself with every
+// 16 products (all-positive bf16 and f16, k = 131,072 in one accumulator: 7.2e-4, more than half a step of f16). So
+// one plane, too, is joined in float32 registers every kJoinSlices where an accumulator would take more than kJoinAfter
+// slices (8,192 k, up to which it loses 5e-5 at the most, a tenth of half a step of f16). Joining every product takes
+// up to 1.1 times as long (8192 x 4096 x 16384 bf16: 695 and 767 us).
+constexpr int kJoinAfter = 128, kJoinSlices = 32;
+
 // Warps of a pair's CTA: its epilogue warps, then a warpgroup of loads,
 // products and two idle warps. Joined sums stay in registers, 64 a thread with
 // sixteen epilogue warps (eight, with 128, took 1.3 times as long over a tile).
-template <int PLANES>
+template <bool JOIN>
 struct Pair {
-  static constexpr bool JOIN = PLANES > 1;
   static constexpr int EPI = JOIN ? 16 : 8;
   static constexpr int NT = (EPI + 4) * 32;
   // registers where JOIN: 640 x 96 at launch = 128 x 64 + 512 x 104 after the split
   static constexpr int FEW = 64, MANY = 104;
 };
+// Blocks of staging: one for each epilogue warp, or, with one plane joined over a long k, one for two of them, which take turns
+// at the end of a tile, so that the ring holds six slices instead of four (4096 x 32768 x 4096 bf16: 815 and 915 us; 785 without joining).
+__host__ __device__ constexpr int pair_staging(int planes) { return planes > 1 ? 16 : 8; }
+
 // ---------------------------------------------------------------------------
 // pairs of CTAs
 // ---------------------------------------------------------------------------
 
-template <int PLANES, typename OUT>
-__global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
+template <int PLANES, bool JOIN, typename OUT>
+__global__ void __launch_bounds__(Pair<JOIN>::NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ TcParams p) {
   extern __shared__ unsigned char raw[];
@@ -60,8 +71,8 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
-  constexpr bool JOIN = PLANES > 1;
-  constexpr int EPI = Pair<PLANES>::EPI, GROUPS = EPI / 4, SLICES = 8 / GROUPS;  // slices: 32 columns of a warp's rows
+  constexpr int STAGES = pair_staging(PLANES);
+  constexpr int EPI = Pair<JOIN>::EPI, GROUPS = EPI / 4, SLICES = 8 / GROUPS;  // slices: 32 columns of a warp's rows
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
@@ -95,15 +106,15 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
   previous_done();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
   volatile int* gu = &gave_up;
-  const int per = JOIN ? 1 : p.kblocks;  // slices of one accumulator
+  const int per = PLANES > 1 ? 1 : JOIN ? kJoinSlices : p.kblocks;  // slices of one accumulator
 
   if (warp < EPI) {
-    if constexpr (JOIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Pair<PLANES>::MANY));
+    if constexpr (JOIN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Pair<JOIN>::MANY));
     // ---- epilogue: warps w, w + 4, ... share the rows 32 (w % 4).. and deal out the columns ----
     const int quad = warp & 3, group = warp >> 2;
     const uint32_t lead_tempty0 = map_rank(tempty0, 0);
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    float* stage = staging + warp * kStageFloats;
+    float* stage = staging + warp % STAGES * kStageFloats;
     uint32_t buf = 0, tphase = 0;
     bool ok = true;
     const float bad = __int_as_float(0x7fffffff);
@@ -119,7 +130,7 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
         for (int q = 0; q < SLICES; ++q)
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[q][c] = 0.f;
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+        for (int kb = 0; kb < p.kblocks; kb += per) {
           ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
           fence_after();
 #pragma unroll
@@ -134,6 +145,7 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
           if (lane == 0) bar_arrive_cluster(lead_tempty0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
+        if (STAGES < EPI && warp >= STAGES) asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32) : "memory");
         // one copy of the epilogue's code: the sums move up instead of the index
 #pragma unroll 1
         for (int q = 0; q < SLICES; ++q) {
@@ -147,6 +159,9 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
 #pragma unroll
             for (int m = 1; m < SLICES; ++m) acc[m - 1][c] = acc[m][c];
         }
+        // the first half of the warps lets the second one in, and stays out until that is done
+        if (STAGES < EPI && warp < STAGES) asm volatile("bar.sync 1, %0;" ::"n"(EPI * 32) : "memory");
+        if (STAGES < EPI) asm volatile("bar.sync 2, %0;" ::"n"(EPI * 32) : "memory");
       } else {
         ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
         fence_after();
@@ -169,7 +184,7 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
       }
     }
   } else {
-    if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Pair<PLANES>::FEW));
+    if constexpr (JOIN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Pair<JOIN>::FEW));
     if (warp == EPI) {
       // ---- loads ----
       const bool lead = elect_one();
@@ -197,7 +212,8 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
         for (int k0 = 0; k0 < p.kblocks; k0 += per) {
           if (!bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
           fence_after();
-          for (int kb = 0; kb < per; ++kb) {
+          const int n = p.kblocks - k0 < per ? p.kblocks - k0 : per;
+          for (int kb = 0; kb < n; ++kb) {
             if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
             fence_after();
             if (lead) {
@@ -230,17 +246,16 @@ __global__ void __launch_bounds__(Pair<PLANES>::NT, 1)
 
 // JOIN: one CTA an SM with eight epilogue warps, so that a slice's planes fit
 // twice; otherwise two CTAs with four.
-template <int PLANES>
+template <bool JOIN>
 struct Solo {
-  static constexpr bool JOIN = PLANES > 1;
   static constexpr int EPI = JOIN ? 8 : 4;
   static constexpr int NT = (EPI + 2) * 32;
   static constexpr int CTAS = JOIN ? 1 : 2;
   static constexpr int SMEM = JOIN ? kSmemMax - 1024 : 113 * 1024;
 };
 
-template <int PLANES, typename OUT>
-__global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
+template <int PLANES, bool JOIN, typename OUT>
+__global__ void __launch_bounds__(Solo<JOIN>::NT, Solo<JOIN>::CTAS)
     gemm_solo_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ TcParams p) {
   extern __shared__ unsigned char raw[];
@@ -248,8 +263,8 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 5];  // the last: nothing arrives on it
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
-  constexpr bool JOIN = PLANES > 1;
-  constexpr int EPI = Solo<PLANES>::EPI, GROUPS = EPI / 4, SLICES = JOIN ? 4 / GROUPS : 1;
+  constexpr int EPI = Solo<JOIN>::EPI, GROUPS = EPI / 4, SLICES = JOIN ? 4 / GROUPS : 1;
+  constexpr int per = PLANES > 1 ? 1 : kJoinSlices;  // slices of one accumulator where JOIN
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = p.split, rank = split > 1 ? (int)cluster_rank() : 0;
   unsigned char* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
@@ -301,7 +316,7 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
 #pragma unroll
         for (int c = 0; c < 32; ++c) acc[q][c] = 0.f;
       uint32_t buf = 0, tphase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += per) {
         ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_gemm_fault));
         fence_after();
 #pragma unroll
@@ -361,16 +376,18 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
     const Multiplier<1, PLANES> mul(p, smem_u32(ring));
     uint32_t s = 0, phase = 0, buf = 0, tphase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (JOIN && !bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
+      // an accumulator's first and last slice
+      const bool fresh = JOIN ? (kb - kb0) % per == 0 : kb == kb0, done = kb == kb1 - 1 || (JOIN && (kb - kb0) % per == per - 1);
+      if (JOIN && fresh && !bar_wait(tempty0 + 8 * buf, tphase ^ 1, gu, limit, &g_gemm_fault)) break;
       if (!bar_wait(full0 + 8 * s, phase, gu, limit, &g_gemm_fault)) break;
       fence_after();
       if (lead) {
-        mul.slice(s, tmem + buf * p.BN, JOIN || kb == kb0);
+        mul.slice(s, tmem + buf * p.BN, fresh);
         commit<1>(empty0 + 8 * s);
-        if (JOIN || kb == kb1 - 1) commit<1>(tfull0 + 8 * buf);
+        if (done) commit<1>(tfull0 + 8 * buf);
       }
       if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
-      if (JOIN && ++buf == 2) buf = 0, tphase ^= 1;
+      if (JOIN && done && ++buf == 2) buf = 0, tphase ^= 1;
     }
   }
   __syncwarp();
@@ -379,10 +396,10 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
   // each CTA of the cluster finishes its share of the rows
   const int nrows = BM / split, r0 = rank * nrows;
   const Block mine{o.b, o.i + r0, o.j, partial + r0 * pitch, pitch, 31 - __clz(nrows), 31 - __clz(p.BN)};
-  finish<OUT, true, 1>(p, mine, o.mirror, tid, Solo<PLANES>::NT);
+  finish<OUT, true, 1>(p, mine, o.mirror, tid, Solo<JOIN>::NT);
   if (o.mirror) {
     __syncthreads();
-    mirror_units<OUT>(p, mine, tid, Solo<PLANES>::NT);
+    mirror_units<OUT>(p, mine, tid, Solo<JOIN>::NT);
   }
   __syncwarp();
   if (split > 1) cluster_sync();  // peers' sums stay until they have been read
@@ -399,6 +416,8 @@ __global__ void __launch_bounds__(Solo<PLANES>::NT, Solo<PLANES>::CTAS)
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+
+int slices_of_cta(int kblocks, int split) { return (kblocks + split - 1) / split; }
 
 template <typename Kern>
 cudaError_t launch_in_clusters(Kern kern, int64_t ctas, int cluster, int threads, size_t smem, cudaStream_t s,
@@ -427,14 +446,14 @@ cudaError_t launch_in_clusters(Kern kern, int64_t ctas, int cluster, int threads
   return cudaLaunchKernelEx(&cfg, kern, mp, mq, p);
 }
 
-template <int PLANES, typename OUT>
+template <int PLANES, bool JOIN, typename OUT>
 cudaError_t launch_pair(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
-  constexpr int NT = Pair<PLANES>::NT;
-  const int staging = Pair<PLANES>::EPI * kStageFloats * 4;
+  constexpr int NT = Pair<JOIN>::NT;
+  const int staging = pair_staging(PLANES) * kStageFloats * 4;
   const int stages = (kSmemMax - 1024 - 512 - staging) / p.stage_bytes;
   p.stages = stages > kMaxStages ? kMaxStages : stages;
   const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + staging;
-  auto kern = gemm_pair_kernel<PLANES, OUT>;
+  auto kern = gemm_pair_kernel<PLANES, JOIN, OUT>;
   static int cache[64];
   int occ = 0;
   cudaError_t e = kernel_occupancy(kern, NT, smem, cache, &occ);
@@ -443,13 +462,13 @@ cudaError_t launch_pair(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p
   return launch_in_clusters(kern, want < cap ? want : cap, 2, NT, smem, s, mp, mq, p);
 }
 
-template <int PLANES, typename OUT>
+template <int PLANES, bool JOIN, typename OUT>
 cudaError_t launch_solo(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p, int sms, cudaStream_t s) {
-  constexpr int NT = Solo<PLANES>::NT;
+  constexpr int NT = Solo<JOIN>::NT;
   const int sums = BM * (p.BN + 4) * 4;
   const int per = (p.kblocks + p.split - 1) / p.split;
   // all of an SM's shared memory where it gets one CTA anyway: a slice takes about 2,000 clocks to arrive
-  const int room = p.tiles * p.split <= sms ? kSmemMax - 1024 : Solo<PLANES>::SMEM;
+  const int room = p.tiles * p.split <= sms ? kSmemMax - 1024 : Solo<JOIN>::SMEM;
   int stages = (room - 1024 - 512) / p.stage_bytes;
   if (stages > kMaxStages) stages = kMaxStages;
   p.stages = stages > per ? per : stages;
@@ -457,8 +476,8 @@ cudaError_t launch_solo(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p
   if (smem < (size_t)sums) smem = sums;
   smem += 1024;
   p.tmem_cols = 32;
-  while (p.tmem_cols < (PLANES > 1 ? 2 : 1) * p.BN) p.tmem_cols *= 2;
-  auto kern = gemm_solo_kernel<PLANES, OUT>;
+  while (p.tmem_cols < (JOIN ? 2 : 1) * p.BN) p.tmem_cols *= 2;
+  auto kern = gemm_solo_kernel<PLANES, JOIN, OUT>;
   static int cache[64];
   int occ = 0;
   cudaError_t e = kernel_occupancy(kern, NT, smem, cache, &occ);
@@ -468,8 +487,15 @@ cudaError_t launch_solo(const CUtensorMap& mp, const CUtensorMap& mq, TcParams p
 
 template <bool PAIR, int PLANES, typename OUT>
 cudaError_t launch_form(const CUtensorMap& mp, const CUtensorMap& mq, const TcParams& p, int sms, cudaStream_t s) {
-  if constexpr (PAIR) return launch_pair<PLANES, OUT>(mp, mq, p, sms, s);
-  else return launch_solo<PLANES, OUT>(mp, mq, p, sms, s);
+  if (PLANES > 1 || slices_of_cta(p.kblocks, p.split) > kJoinAfter) {
+    if constexpr (PAIR) return launch_pair<PLANES, true, OUT>(mp, mq, p, sms, s);
+    else return launch_solo<PLANES, true, OUT>(mp, mq, p, sms, s);
+  }
+  if constexpr (PLANES == 1) {
+    if constexpr (PAIR) return launch_pair<PLANES, false, OUT>(mp, mq, p, sms, s);
+    else return launch_solo<PLANES, false, OUT>(mp, mq, p, sms, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 template <bool PAIR>
@@ -512,7 +538,7 @@ Form choose_form(const TcProblem& t, int kblocks, int planes, int nseg, int sms)
     if (!t.sym && BN > 32 && BN / 2 >= t.J) break;
     const int64_t tj = (t.J + BN - 1) / BN, tiles = t.batch * (t.sym ? ti * (ti + 1) / 2 : ti * tj);
     for (int split = 1; split <= 4 && split <= kblocks; split *= 2) {
-      const double ctas = (double)tiles * split, on_sm = ceil(ctas / sms), at_once = fmin(on_sm, planes > 1 ? 1.0 : 2.0);
+      const double ctas = (double)tiles * split, on_sm = ceil(ctas / sms), at_once = fmin(on_sm, planes > 1 || slices_of_cta(kblocks, split) > kJoinAfter ? 1.0 : 2.0);
       const double load = planes * (16384.0 + BN * 128.0) / rate(ctas), mul = nseg * 4.0 * fmax(BN / 2.0, (128 + BN) / 4.0);
       const double slice = fmax(500.0, at_once * fmax(load, mul));
       const double c = ceil(on_sm / at_once) * ((kblocks + split - 1) / split * slice + 8000 + BN * 20) +
