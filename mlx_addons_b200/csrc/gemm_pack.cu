@@ -27,14 +27,17 @@ __device__ __forceinline__ uint16_t bf16_finite(float x) {
 }
 __device__ __forceinline__ float bf16_value(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 
-// x as hi + mid + lo, each bf16: the remainders are exact, so the three hold
-// all 24 bits. A non-finite x is its hi plane alone.
+// x as hi + 2^-8 mid + 2^-16 lo, each bf16: the remainders are exact, so the three
+// hold all 24 bits. Without the powers of two the last bits of a small x (below 2^-110)
+// would fall under 2^-133, bf16's smallest value; with them float32's own smallest,
+// 2^-149, is 2^-133 in lo. |mid| and |lo| stay within |hi|, so nothing overflows that hi
+// would not. A non-finite x is its hi plane alone.
 __device__ __forceinline__ void thirds(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
   if (isfinite(x)) {
     hi = bf16_finite(x);
     const float r = x - bf16_value(hi);
-    mid = bf16_finite(r);
-    lo = bf16_finite(r - bf16_value(mid));
+    mid = bf16_finite(r * 256.f);
+    lo = bf16_finite(fmaf(bf16_value(mid), -0.00390625f, r) * 65536.f);
   } else {
     hi = __bfloat16_as_ushort(__float2bfloat16_rn(x));
     mid = lo = 0;

@@ -9,7 +9,7 @@ namespace b2c {
 // How a 16-bit array stands for the values of an operand, addend or output.
 //   kOne      one array of bf16 or f16
 //   kHalves   two f16 planes, value = hi + lo (22 bits and the sign of lo)
-//   kThirds   three bf16 planes, value = hi + mid + lo (all 24 bits)
+//   kThirds   three bf16 planes, value = hi + 2^-8 mid + 2^-16 lo (all 24 bits)
 enum TcKind { kOne = 0, kHalves = 1, kThirds = 2 };
 
 // One operand, as the tensor cores read it: 16-bit, one of its axes with unit

@@ -593,7 +593,8 @@ __device__ __forceinline__ void settle() {
   }
 }
 
-// The plane pairs of a product, smallest first.
+// The plane pairs of a product, smallest first; shift: by how many bits the sum
+// so far goes down before the first product of a pair is added.
 template <int PLANES>
 struct Segs;
 template <>
@@ -601,18 +602,22 @@ struct Segs<1> {
   static constexpr int N = 1;
   static __host__ __device__ constexpr int p(int) { return 0; }
   static __host__ __device__ constexpr int q(int) { return 0; }
+  static __host__ __device__ constexpr int shift(int) { return 0; }
 };
 template <>
 struct Segs<2> {  // lo hi, hi lo, hi hi
   static constexpr int N = 3;
   static __host__ __device__ constexpr int p(int g) { return g == 0; }
   static __host__ __device__ constexpr int q(int g) { return g == 1; }
+  static __host__ __device__ constexpr int shift(int) { return 0; }
 };
 template <>
 struct Segs<3> {  // lo hi, mid mid, hi lo, mid hi, hi mid, hi hi
   static constexpr int N = 6;
   static __host__ __device__ constexpr int p(int g) { return g == 0 ? 2 : g == 1 || g == 3 ? 1 : 0; }
   static __host__ __device__ constexpr int q(int g) { return g == 2 ? 2 : g == 1 || g == 4 ? 1 : 0; }
+  // mid is held times 2^8, lo times 2^16: the first three products are 2^16 times what they stand for, the next two 2^8
+  static __host__ __device__ constexpr int shift(int g) { return g == 3 || g == 5 ? 8 : 0; }
 };
 
 // One slice: every plane of this CTA's rows of P, then of Q.
@@ -661,7 +666,10 @@ struct Multiplier {
     for (int g = 0; g < S::N; ++g) {
       const uint64_t a = dp + s * stage + S::p(g) * (kABytes >> 4), q = dq + s * stage + S::q(g) * plane_q;
 #pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk) mma<CG>(d, a + kk * step_p, q + kk * step_q, idesc, g || kk ? 1u : !fresh);
+      for (int kk = 0; kk < BK / 16; ++kk) {
+        if (S::shift(g) && kk == 0) mma<CG, 8>(d, a, q, idesc, 1u);
+        else mma<CG>(d, a + kk * step_p, q + kk * step_q, idesc, g || kk ? 1u : !fresh);
+      }
     }
   }
 };
