@@ -124,7 +124,9 @@ __device__ __forceinline__ float act_slope_f32(float x, int act) {
     }
     case B2C_ACT_GELU_TANH: {
       const float s = sigmoid_f32<FAST>(2.f * kGeluC * (x + kGeluK * x * x * x));
-      return s + x * s * (1.f - s) * 2.f * kGeluC * (1.f + 3.f * kGeluK * x * x);
+      // beyond 16 the second term is zero in 32 bits, but its factors overflow there
+      const float c = fminf(fmaxf(x, -16.f), 16.f);
+      return s + c * s * (1.f - s) * 2.f * kGeluC * (1.f + 3.f * kGeluK * c * c);
     }
     case B2C_ACT_SILU: {
       const float s = sigmoid_f32<FAST>(x);
