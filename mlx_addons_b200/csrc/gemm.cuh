@@ -70,29 +70,36 @@ constexpr float kRsqrt2 = 0.7071067811865476f;
 constexpr float kRsqrt2Pi = 0.3989422804014327f;  // 1 / sqrt(2 pi)
 
 // Activations come in two forms: FAST for 16-bit results, on the exponential
-// and reciprocal units (a few 2^-22 relative, far below a 16-bit rounding),
-// and one on the accurate functions for float32.
+// and reciprocal units, and one on the accurate functions for float32. The fast
+// ones are within 2^-16 of their value wherever it is a normal number (most of it the exponent's
+// rounding far out), a thirtieth of half a step of f16.
 template <bool FAST>
 __device__ __forceinline__ float exp_f32(float x) {
   return FAST ? __expf(x) : expf(x);
 }
+// By exp(-|x|), which leaves the divisor in [1, 2] and the lower tail its relative accuracy.
 template <bool FAST>
 __device__ __forceinline__ float sigmoid_f32(float x) {
-  return FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
+  const float t = exp_f32<FAST>(-fabsf(x)), r = FAST ? __fdividef(1.f, 1.f + t) : 1.f / (1.f + t);
+  return x < 0.f ? t * r : r;
 }
 
 // Normal distribution function; bell receives exp(-x^2 / 2). The fast form is
-// Abramowitz and Stegun's 7.1.26 for erfc(|x| / sqrt 2), off by 1.5e-7 at most.
+// Phi(-|x|) = bell t (c0 + c1 t + ... + c6 t^6) with t = 1 / (1 + p |x|): the c are the
+// minimax fit of the relative error over |x| <= 14 (a linear programme on 1,400 points),
+// p the one that makes it smallest; 7e-7 of the value, 1.0e-6 as evaluated in 32 bits.
 template <bool FAST>
 __device__ __forceinline__ float normal_cdf(float x, float& bell) {
   bell = exp_f32<FAST>(-0.5f * x * x);
   if constexpr (!FAST) return 0.5f * (1.f + erff(x * kRsqrt2));
-  const float t = __fdividef(1.f, fmaf(0.3275911f * kRsqrt2, fabsf(x), 1.f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  const float tail = 0.5f * q * t * bell;
+  const float t = __fdividef(1.f, fmaf(0.362480336f, fabsf(x), 1.f));
+  float q = fmaf(0.0481144309f, t, -0.179940585f);
+  q = fmaf(q, t, 0.175411849f);
+  q = fmaf(q, t, 0.0294815642f);
+  q = fmaf(q, t, 0.139324177f);
+  q = fmaf(q, t, 0.142915497f);
+  q = fmaf(q, t, 0.144693461f);
+  const float tail = q * t * bell;
   return x < 0.f ? tail : 1.f - tail;
 }
 

@@ -1,10 +1,10 @@
-"""Slopes of the activations far from zero."""
+"""Tails of the activations and of their slopes, relative to their values."""
 
 import pytest
 import torch
 
 import mlx_addons_b200.linalg as la
-from tests._exact import HALF
+from tests._exact import HALF, act64
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,12 @@ TINY = {F32: 2.0**-150, BF16: 2.0**-134, F16: 2.0**-25}
 def _need_cuda():
     if not torch.cuda.is_available():
         pytest.skip("no CUDA device")
+
+
+def _act64(x, name):
+    if name == "gelu":  # log_ndtr keeps its relative accuracy in the lower tail
+        return x * torch.special.log_ndtr(x).exp()
+    return act64(x, name) if name != "gelu_tanh" else x * torch.sigmoid(2 * 0.7978845608028654 * (x + 0.044715 * x**3))
 
 
 def _slope64(z, name):
@@ -37,8 +43,29 @@ def _slope64(z, name):
     return cdf + rest, cdf + rest.abs()
 
 
+def _outputs(x, act):
+    """act(x) for a column x through the FP32 units and, as rows of 64 against the identity, through the tensor cores."""
+    one = torch.ones(1, 1, device=DEV, dtype=x.dtype)
+    eye = torch.eye(64, device=DEV, dtype=x.dtype)
+    return la.gemm(x, one, activation=act), la.gemm(x.reshape(-1, 64), eye, activation=act).reshape(-1, 1)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_16_bit_values(dtype, act):
+    """Every output within half a step of its own and 2^-14 of its value, down to the type's smallest. 2^-14 is an eighth
+    of a half step of float16: exp(-x^2 / 2) takes its exponent, up to 88, from a product rounded to 2^-24 of it (about
+    2^-17 of the result), which leaves the approximations of Phi and of the sigmoid the rest."""
+    x = torch.linspace(-12.5, 12.5, 64 * 2048, device=DEV).to(dtype).reshape(-1, 1)
+    ref = _act64(x.double(), act)
+    for y in _outputs(x, act):
+        over = (y.double() - ref).abs() - (HALF[dtype] * (1 + 2.0**-14) + 2.0**-14) * ref.abs() - TINY[dtype]
+        at = int(over.argmax())
+        assert float(over.max()) <= 0, (float(x[at]), float(y[at]), float(ref[at]))
+
+
 def _check_slopes(got, x, act, scale):
-    """dP is rounded once; evaluating the terms costs 2^-14 of them in 16 bits and 2^-17 in 32 (exp of up to 88
+    """dP is rounded once; evaluating the terms costs 2^-14 of them in 16 bits, as above, and 2^-17 in 32 (exp of up to 88
     from an argument rounded to 2^-24 of it); in 32 bits Phi comes from 1 + erf, rounded to 2^-24 in itself."""
     ref, terms = _slope64(x.double(), act)
     own = 2.0**-17 if x.dtype == F32 else 2.0**-14
@@ -63,3 +90,12 @@ def test_slopes_far_out(dtype, act):
     want = _check_slopes(dA, pre, act, 3.0)
     n = float(want.sum())  # 3 for each positive one
     assert abs(n - 3 * len(far)) < 1e-9 and float(db) == round(n) and float(dB) == round(n)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_slopes_in_the_tail(dtype, act):
+    """Slopes over the range where they vary, within roundings of their two terms."""
+    x = torch.linspace(-12.5, 12.5, 64 * 512, device=DEV).to(dtype).reshape(-1, 1)
+    one = torch.ones(1, 1, device=DEV, dtype=dtype)
+    _check_slopes(la.gemm_grad(torch.ones_like(x), x, one, x, act)[0], x, act, 1.0)
