@@ -144,6 +144,9 @@ int b2c_qr(const float *A, float *Q, float *R, int64_t batch, int k,
 #define B2C_ACT_GELU_TANH 3 /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
 #define B2C_ACT_SILU 4      /* x / (1 + exp(-x)) */
 
+/* In the products below every address is a multiple of its element's size and a
+ * workspace, where one is needed, of 16 bytes; other addresses are refused. */
+
 /* A batch of matrices with free strides, in elements: element (b, r, c) at
  * ptr[b * batch_stride + r * row_stride + c * col_stride]. Strides may be 0
  * (a broadcast axis) but not negative. */

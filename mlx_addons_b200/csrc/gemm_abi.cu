@@ -2,6 +2,7 @@
 // Newton-Schulz orthogonalisation (declared in include/b2c.h).
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 
 #include "b2c_kernels.cuh"
 #include "gemm_tc.cuh"
@@ -30,6 +31,13 @@ int cuda_err(cudaError_t e, const char* name) {
 }
 
 bool dtype_ok(int dtype) { return dtype >= B2C_F32 && dtype <= B2C_F16; }
+bool on(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// Whether all of these addresses are multiples of an element's size.
+bool aligned(int dtype, std::initializer_list<const void*> all) {
+  for (const void* p : all)
+    if (!on(p, dtype == B2C_F32 ? 4 : 2)) return false;
+  return true;
+}
 bool strides_ok(const b2c_matrix& m) { return m.batch_stride >= 0 && m.row_stride >= 0 && m.col_stride >= 0; }
 
 GemmProblem problem(int dtype, const b2c_matrix* A, const b2c_matrix* B, int64_t batch, int64_t M, int64_t K, int64_t N) {
@@ -142,6 +150,8 @@ int b2c_gemm(int dtype, const b2c_matrix* A, const b2c_matrix* B, const void* bi
   if (batch == 0 || M == 0 || N == 0) return set_error(B2C_OK, "");
   if (!Y || (K > 0 && (!A->ptr || !B->ptr)) || (R && !R->ptr))
     return err(B2C_ERR_INVALID_ARGUMENT, name, "A, B, R and Y must point to data");
+  if (!aligned(dtype, {A->ptr, B->ptr, bias, R ? R->ptr : nullptr, Y, pre}))
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "an address is not aligned to its elements");
   GemmProblem g = problem(dtype, A, B, batch, M, K, N);
   g.e.y = GemmView{Y, M * N, N, 1};
   g.e.pre = GemmView{pre, M * N, N, 1};
@@ -151,7 +161,7 @@ int b2c_gemm(int dtype, const b2c_matrix* A, const b2c_matrix* B, const void* bi
   g.e.beta = beta;
   g.e.act = activation;
   const GemmChoice c = choose(g);
-  if (c.ws() && (!workspace || workspace_bytes < c.ws() || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+  if (c.ws() && (!workspace || workspace_bytes < c.ws() || !on(workspace, 16)))
     return err(B2C_ERR_WORKSPACE, name, "workspace missing, too small or not on 16 bytes");
   const cudaError_t e = launch_gemm(c, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
@@ -180,6 +190,8 @@ int b2c_gemm_dact(int dtype, const b2c_matrix* dY, const b2c_matrix* pre, int ac
   if (empty && !dbias) return set_error(B2C_OK, "");
   if (!empty && (!dY->ptr || (activation != B2C_ACT_NONE && !pre->ptr)))
     return err(B2C_ERR_INVALID_ARGUMENT, name, "dY and pre must point to data");
+  if (!aligned(dtype, {dY->ptr, activation != B2C_ACT_NONE ? pre->ptr : nullptr, dP, dbias, dR}))
+    return err(B2C_ERR_INVALID_ARGUMENT, name, "an address is not aligned to its elements");
   DactParams p{};
   p.dtype = dtype;
   p.act = activation;
@@ -198,7 +210,8 @@ int b2c_gemm_dact(int dtype, const b2c_matrix* dY, const b2c_matrix* pre, int ac
   p.N = N;
   p.ws = static_cast<float*>(workspace);
   const size_t need = dbias ? dact_ws_floats(batch, M, N) * sizeof(float) : 0;
-  if (need && (!workspace || workspace_bytes < need)) return err(B2C_ERR_WORKSPACE, name, "workspace too small");
+  if (need && (!workspace || workspace_bytes < need || !on(workspace, 16)))
+    return err(B2C_ERR_WORKSPACE, name, "workspace missing, too small or not on 16 bytes");
   const cudaError_t e = launch_gemm_dact(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);
 }
@@ -244,6 +257,7 @@ int b2c_orthogonalize(int dtype, const b2c_matrix* G, void* out, int64_t batch, 
   }
   if (batch == 0 || m == 0 || n == 0) return set_error(B2C_OK, "");
   if (!G->ptr || !out) return err(B2C_ERR_INVALID_ARGUMENT, name, "G and out must point to data");
+  if (!aligned(dtype, {G->ptr, out})) return err(B2C_ERR_INVALID_ARGUMENT, name, "an address is not aligned to its elements");
   PolarParams p = polar_params(dtype, G, batch, m, n);
   p.out = out;
   p.coef = coef;
@@ -251,7 +265,7 @@ int b2c_orthogonalize(int dtype, const b2c_matrix* G, void* out, int64_t batch, 
   p.eps = eps;
   p.ws = workspace;
   const size_t need = polar_ws_bytes(p);
-  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+  if (need && (!workspace || workspace_bytes < need || !on(workspace, 16)))
     return err(B2C_ERR_WORKSPACE, name, "workspace missing, too small or not on 16 bytes");
   const cudaError_t e = launch_polar(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? set_error(B2C_OK, "") : cuda_err(e, name);

@@ -152,3 +152,28 @@ def test_dual_numbers_are_refused():
                 call()
             with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
                 call()
+
+
+def test_c_entries_refuse_misaligned_addresses(lib):
+    """An address that is not a multiple of its element's size, or scratch that is not on 16 bytes, would fault the GPU."""
+    bad, ws = _lib.B2C_ERR_INVALID_ARGUMENT, _lib.B2C_ERR_WORKSPACE
+    muon = (ctypes.c_double * 3)(3.4445, -4.775, 2.0315)
+
+    def gemm(dtype, A=16, B=16, bias=None, R=None, Y=16, pre=None):
+        return lib.b2c_gemm(dtype, _m(A, 0, 2, 1), _m(B, 0, 2, 1), bias, None if R is None else _m(R, 0, 2, 1), Y, pre, 1, 2, 2, 2,
+                            1.0, 1.0, 0, None, 0, None)
+
+    def dact(dtype, dY=16, pre=16, dP=16, db=None, dR=None, w=16, n=1 << 20):
+        return lib.b2c_gemm_dact(dtype, _m(dY, 0, 2, 1), _m(pre, 0, 2, 1), 2, 1.0, dP, db, dR, 1, 2, 2, w, n, None)
+
+    def orth(dtype, G=16, out=16, w=16, m=4):
+        return lib.b2c_orthogonalize(dtype, _m(G, 0, m, 1), out, 1, m, m, muon, 1, 1e-7, w, 1 << 30, None)
+
+    for dtype, off in ((0, 17), (0, 18), (1, 17), (2, 17)):
+        for call, names in ((gemm, ("A", "B", "bias", "R", "Y", "pre")), (dact, ("dY", "pre", "dP", "db", "dR")),
+                            (orth, ("G", "out"))):
+            for name in names:
+                assert call(dtype, **{name: off}) == bad, (dtype, off, name)
+                assert b"align" in lib.b2c_last_error()
+    for w in (17, 20, 24):
+        assert dact(0, db=16, w=w) == ws and orth(0, w=w, m=300) == ws
