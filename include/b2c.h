@@ -174,8 +174,9 @@ int b2c_gemm(int dtype, const b2c_matrix *A, const b2c_matrix *B, const void *bi
              void *pre, int64_t batch, int64_t M, int64_t K, int64_t N, float alpha, float beta, int activation,
              void *workspace, size_t workspace_bytes, void *stream);
 
-/* Scratch bytes of b2c_gemm for these operands (their alignment and strides
- * count; A->ptr and B->ptr are not read). */
+/* Scratch bytes of b2c_gemm for these operands. Their strides and the alignment
+ * of their addresses count (nothing is read there), so pass the addresses of
+ * the call, or NULL for a size that suits any. */
 size_t b2c_gemm_workspace_size(int dtype, const b2c_matrix *A, const b2c_matrix *B, int64_t batch, int64_t M,
                                int64_t K, int64_t N);
 

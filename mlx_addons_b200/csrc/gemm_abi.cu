@@ -132,7 +132,12 @@ size_t b2c_gemm_workspace_size(int dtype, const b2c_matrix* A, const b2c_matrix*
   if (!dtype_ok(dtype) || !A || !B || !strides_ok(*A) || !strides_ok(*B) || batch <= 0 || M <= 0 || K <= 0 || N <= 0 ||
       M > kMaxDim || K > kMaxDim || N > kMaxDim)
     return 0;
-  return choose(problem(dtype, A, B, batch, M, K, N)).ws();
+  // an operand without an address may get one that TMA cannot read, and then needs a copy
+  GemmProblem g = problem(dtype, A, B, batch, M, K, N);
+  const void* odd = reinterpret_cast<const void*>((uintptr_t)1);
+  if (!g.P.p) g.P.p = odd;
+  if (!g.Q.p) g.Q.p = odd;
+  return choose(g).ws();
 }
 
 int b2c_gemm(int dtype, const b2c_matrix* A, const b2c_matrix* B, const void* bias, const b2c_matrix* R, void* Y,

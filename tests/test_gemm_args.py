@@ -177,3 +177,14 @@ def test_c_entries_refuse_misaligned_addresses(lib):
                 assert b"align" in lib.b2c_last_error()
     for w in (17, 20, 24):
         assert dact(0, db=16, w=w) == ws and orth(0, w=w, m=300) == ws
+
+
+def test_c_workspace_size_without_addresses(lib):
+    """Asked for before the operands have addresses, the size covers any that they may get."""
+    for dtype in (0, 1, 2):
+        for s in ((0, 512, 1), (0, 1, 512), (0, 520, 1), (0, 513, 1)):
+            def size(a, b):
+                return lib.b2c_gemm_workspace_size(dtype, _m(a, *s), _m(b, *s), 1, 512, 512, 512)
+            any_ = size(None, None)
+            assert any_ == size(2 if dtype else 4, 2 if dtype else 4) > 0
+            assert all(size(a, b) <= any_ for a in (None, 8, 16) for b in (None, 8, 16))
