@@ -182,9 +182,9 @@ def test_c_entries_refuse_misaligned_addresses(lib):
 def test_c_workspace_size_without_addresses(lib):
     """Asked for before the operands have addresses, the size covers any that they may get."""
     for dtype in (0, 1, 2):
-        for s in ((0, 512, 1), (0, 1, 512), (0, 520, 1), (0, 513, 1)):
+        for s in ((0, 1024, 1), (0, 1, 1024), (0, 1032, 1), (0, 1025, 1)):
             def size(a, b):
-                return lib.b2c_gemm_workspace_size(dtype, _m(a, *s), _m(b, *s), 1, 512, 512, 512)
+                return lib.b2c_gemm_workspace_size(dtype, _m(a, *s), _m(b, *s), 1, 1024, 1024, 1024)
             any_ = size(None, None)
             assert any_ == size(2 if dtype else 4, 2 if dtype else 4) > 0
             assert all(size(a, b) <= any_ for a in (None, 8, 16) for b in (None, 8, 16))
