@@ -253,8 +253,8 @@ int b2c_orthogonalize(int dtype, const b2c_matrix* G, void* out, int64_t batch, 
   for (int t = 0; t < steps; ++t) {
     const double *c = coefficients + 3 * t;
     for (int i = 0; i < 3; ++i) {
-      if (!std::isfinite(c[i])) return err(B2C_ERR_INVALID_ARGUMENT, name, "coefficients must be finite");
       coef[3 * t + i] = (float)c[i];
+      if (!std::isfinite(coef[3 * t + i])) return err(B2C_ERR_INVALID_ARGUMENT, name, "coefficients must be finite float32 values");
     }
     hi = polar_poly_bound(c[0], c[1], c[2], hi);
     if (!(hi <= kMaxSigma))

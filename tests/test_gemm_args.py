@@ -188,3 +188,16 @@ def test_c_workspace_size_without_addresses(lib):
             any_ = size(None, None)
             assert any_ == size(2 if dtype else 4, 2 if dtype else 4) > 0
             assert all(size(a, b) <= any_ for a in (None, 8, 16) for b in (None, 8, 16))
+
+
+@pytest.mark.parametrize("coef", [(1e200, -2e200, 1e200), (1e39, -1e39, 0.0), (0.0, 0.0, 1e60), (1e39, 0.0, -1e39)])
+def test_c_coefficients_beyond_float32(lib, coef):
+    """They pass the bound at 1, where they cancel, and leave float32 in the kernels."""
+    c = (ctypes.c_double * 3)(*coef)
+    assert lib.b2c_orthogonalize(0, _m(16, 0, 256, 1), 16, 1, 256, 256, c, 1, 1e-7, None, 0, None) == _lib.B2C_ERR_INVALID_ARGUMENT
+
+
+def test_c_coefficients_after_a_polynomial_of_zeros(lib):
+    """Nothing can grow from zero, but a factor beyond float32 makes NaN of it."""
+    c = (ctypes.c_double * 6)(0, 0, 0, 1e39, 0, 0)
+    assert lib.b2c_orthogonalize(0, _m(16, 0, 256, 1), 16, 1, 256, 256, c, 2, 1e-7, None, 0, None) == _lib.B2C_ERR_INVALID_ARGUMENT
