@@ -71,7 +71,8 @@ _HOST_CHUNK_BYTES = 32 << 20
 
 def _as_tensor(x, name):
     if isinstance(x, torch.Tensor):
-        return x.resolve_neg(), "torch"  # the kernels read memory, which a lazily negated view holds with the other sign
+        # the kernels read memory, which a lazily negated view holds with the other sign
+        return x.resolve_neg() if x.is_neg() else x, "torch"
     if isinstance(x, np.ndarray):
         return torch.from_numpy(np.ascontiguousarray(x)), "numpy"
     if hasattr(x, "__dlpack__"):

@@ -57,7 +57,7 @@ def _on_device(tensors):
 
 def _guard(dev):
     """The device as the current one, at no cost where it is."""
-    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _NO_GUARD if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _matrix(t):
