@@ -167,8 +167,9 @@ typedef struct b2c_matrix {
  *   Y    (batch, M, N) contiguous output
  *   pre  (batch, M, N) contiguous output, or NULL
  * Other outputs may not overlap the inputs. K = 0 gives A B = 0. Non-finite
- * inputs give non-finite outputs where the sums meet them, for float32 NaN in
- * the place of inf too. Each of M, K, N is at most 2^30. No counterpart in
+ * inputs give non-finite outputs where the sums meet them; for float32, where the
+ * size takes the product to the tensor cores, NaN in the place of inf too, also
+ * where a sum of finite terms leaves float32's range. Each of M, K, N is at most 2^30. No counterpart in
  * the reference. */
 int b2c_gemm(int dtype, const b2c_matrix *A, const b2c_matrix *B, const void *bias, const b2c_matrix *R, void *Y,
              void *pre, int64_t batch, int64_t M, int64_t K, int64_t N, float alpha, float beta, int activation,
@@ -222,7 +223,8 @@ int b2c_host_device_pointer(const void *host_ptr, void **device_ptr);
 
 /* Reads and clears the device fault flags of this library on the current
  * device (synchronises it): *fault = 0 when every kernel finished its work;
- * nonzero = a CTA gave up on a bounded wait (one second) and left the matrix
+ * nonzero = a CTA gave up on a bounded wait (one second; two, and up to four in
+ * the cooperative form, in the products and the orthogonalisation) and left the matrix
  * it was on and every later matrix of that CTA (batch indices i, i + grid,
  * ...) unfinished: their x and logdet are NaN, their L incomplete (NaN from
  * the task-graph kernel). These kernels wait at all: the tensor-core form of

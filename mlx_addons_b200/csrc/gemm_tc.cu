@@ -549,7 +549,7 @@ Form choose_form(const TcProblem& t, int kblocks, int planes, int nseg, int sms)
   if (t.I > BM && t.J > 128) {
     const int64_t ti2 = (t.I + 255) / 256, tj2 = (t.J + 255) / 256;
     const int64_t tiles = t.batch * (t.sym ? ti2 * (ti2 + 1) / 2 : ti2 * tj2);
-    // with several planes the ring holds two or three slices, and their arrival is not hidden
+    // with two planes the ring holds two slices, with three one: their arrival is hardly hidden
     const double slice = planes > 1 ? planes * 2000.0 : fmax(32768.0 / rate(2.0 * tiles), 4.0 * 128);
     const double c = ceil(2.0 * tiles / sms) * kblocks * slice + 11000;
     if (c < best.clocks) best = Form{1, 256, 1, c};

@@ -20,6 +20,10 @@
 // float32: 82 us, with a grid for each product 173; a step costs 4 to 6 us more
 // than one CTA's). Idle SMs join in the same way.
 //
+// The sums of S, P and P X stay in one accumulator: at most 192 additions of 16 products, each cut off at the
+// accumulator's last place, the 128 of the small planes before the 64 that matter (10,000 x 64 x 64 float32: 8e-7 from
+// the 64-bit iteration, float32 products 1.0e-6).
+//
 // Bound by the phases of a step in turn (product, conversion of the sums to
 // the next operand, barrier): two CTAs share an SM and fill each other's gaps.
 

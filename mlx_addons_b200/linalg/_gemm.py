@@ -139,7 +139,7 @@ def _back(out, kind, host):
 
 def gemm(A, B, bias=None, activation: Optional[str] = None, residual=None, *, alpha: float = 1.0, beta: float = 1.0,
          return_pre: bool = False):
-    """act(alpha * A @ B + bias) + beta * residual in one kernel.
+    """act(alpha * A @ B + bias) + beta * residual, the epilogue in the product's kernel.
 
     A (..., M, K); B (K, N), or (..., K, N) with A's leading dimensions; bias
     (N,); residual of the result's shape (an expanded view will do);
@@ -147,8 +147,14 @@ def gemm(A, B, bias=None, activation: Optional[str] = None, residual=None, *, al
     With ``return_pre`` returns (Y, pre), pre = alpha A B + bias being what
     ``gemm_grad`` needs of the activation.
 
-    float32 products are as exact as float32 arithmetic; 16-bit operands are
-    multiplied exactly and summed in 32 bits. Records no gradient, in neither mode: operands that carry one are refused."""
+    float32 products are as exact as float32 arithmetic, for values of any size;
+    16-bit operands are multiplied exactly and summed in 32 bits. A NaN or an
+    infinity stays in the rows and columns that it meets; in larger float32
+    products, which the tensor cores compute from three bf16 planes an operand, an
+    infinity (and a sum that leaves float32's range) gives NaN where float32
+    arithmetic gives inf. The planes, and copies of 16-bit operands whose
+    rows do not start on 16 bytes, take a pass of their own and scratch from torch's
+    allocator: 6 and 2 bytes an element. Records no gradient, in neither mode: operands that carry one are refused."""
     name = "gemm"
     act = _activation(activation, name)
     At, kind = _native(A, "A", name)

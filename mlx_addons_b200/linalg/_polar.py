@@ -37,8 +37,8 @@ def orthogonalize(G, steps: int = 5, coefficients=_COEFFICIENTS, eps: float = 1e
     needs it; (1.875, -1.25, 0.375) converges to 1 in more steps. The
     polynomials may not let a singular value grow past 3.5.
 
-    float32 and float16 inputs are computed as exactly as float32 products
-    allow, larger bfloat16 ones with 11-bit factors (8 times finer than bfloat16);
+    float32 and float16 inputs are computed with 22-bit factors, which comes
+    closer to the exact iteration than float32 products do, larger bfloat16 ones with 11-bit factors (8 times finer than bfloat16);
     sums and norms are held in 32 bits or more and the result is rounded once to
     G's type. A matrix of zeros gives zeros; one with a NaN or an infinity
     gives NaN. Records no gradient, in neither mode: operands that carry one are refused."""

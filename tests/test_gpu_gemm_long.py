@@ -17,7 +17,7 @@ import pytest
 import torch
 
 import mlx_addons_b200.linalg as la
-from tests._exact import HALF
+from tests._exact import HALF, MUON, orth64, orth_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,17 @@ def test_orthogonalisation_of_a_very_long_side():
     ref = (X @ X.mT) @ X
     mean = float((got.double() * ref).sum() / (ref * ref).sum() - 1)
     assert abs(mean) <= (128 * 17 + n / 2048 + 16) * 2.0**-24 + 2.0**-16, mean
+
+
+@pytest.mark.parametrize("shape", [(300, 40000), (1000, 20000), (20000, 1000), (2, 260, 70001), (140, 300000)])
+def test_orthogonalisations_of_long_sides(shape):
+    """bfloat16, all steps, within the bound of their factors and sums, and the same bits again."""
+    g = torch.Generator(device=DEV).manual_seed(shape[-1])
+    G = torch.randn(*shape, generator=g, device=DEV).add_(0.3).to(BF16)  # with a mean, so that sums of one sign are among S
+    out = la.orthogonalize(G)
+    ref, its = orth64(G)
+    flat = lambda t: t.reshape((-1,) + tuple(t.shape[-2:]))  # noqa: E731
+    err = torch.linalg.matrix_norm(flat(out.double() - ref))
+    bound = orth_bound([flat(x) for x in its], 5, MUON, 2.0**-12, BF16)
+    assert bool((err <= bound).all()), (err.tolist(), bound.tolist())
+    assert torch.equal(la.orthogonalize(G), out)
