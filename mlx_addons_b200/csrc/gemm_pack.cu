@@ -31,16 +31,22 @@ __device__ __forceinline__ float bf16_value(uint16_t v) { return __uint_as_float
 // hold all 24 bits. Without the powers of two the last bits of a small x (below 2^-110)
 // would fall under 2^-133, bf16's smallest value; with them float32's own smallest,
 // 2^-149, is 2^-133 in lo. |mid| and |lo| stay within |hi|, so nothing overflows that hi
-// would not. A non-finite x is its hi plane alone.
+// would not.
+//
+// An infinity or a NaN lies in lo, which meets the other operand's hi alone, with a
+// 1 of its sign in hi: in hi it would meet planes that are zero, and infinity times 0
+// is NaN. hi is zero for a zero alone, so that an infinity makes NaN of that and of nothing else.
 __device__ __forceinline__ void thirds(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
   if (isfinite(x)) {
     hi = bf16_finite(x);
+    if ((hi & 0x7fff) == 0 && x != 0.f) hi |= 1;
     const float r = x - bf16_value(hi);
     mid = bf16_finite(r * 256.f);
     lo = bf16_finite(fmaf(bf16_value(mid), -0.00390625f, r) * 65536.f);
   } else {
-    hi = __bfloat16_as_ushort(__float2bfloat16_rn(x));
-    mid = lo = 0;
+    lo = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+    hi = (lo & 0x8000) | 0x3f80;
+    mid = 0;
   }
 }
 
