@@ -40,7 +40,7 @@ def orthogonalize(G, steps: int = 5, coefficients=_COEFFICIENTS, eps: float = 1e
     float32 and float16 inputs are computed with 22-bit factors, which comes
     closer to the exact iteration than float32 products do, larger bfloat16 ones with 11-bit factors (8 times finer than bfloat16);
     sums and norms are held in 32 bits or more and the result is rounded once to
-    G's type. A matrix of zeros gives zeros; one with a NaN or an infinity
+    G's type. A matrix of zeros gives zeros (NaN where eps is 0); one with a NaN or an infinity
     gives NaN. Records no gradient, in neither mode: operands that carry one are refused."""
     name = "orthogonalize"
     Gt, kind = _native(G, "G", name)

@@ -11,12 +11,14 @@ than a 16-bit step, so their roundings hide a bias instead of averaging out: a r
 takes the rounded value away before the output is rounded, which leaves the
 error itself, to half a step of its own."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import mlx_addons_b200.linalg as la
+from mlx_addons_b200 import _lib
 from tests._exact import HALF, MUON, orth64, orth_bound
 
 pytestmark = pytest.mark.gpu
@@ -111,3 +113,27 @@ def test_orthogonalisations_of_long_sides(shape):
     bound = orth_bound([flat(x) for x in its], 5, MUON, 2.0**-12, BF16)
     assert bool((err <= bound).all()), (err.tolist(), bound.tolist())
     assert torch.equal(la.orthogonalize(G), out)
+
+
+@pytest.mark.parametrize("M,K,N", [(300, 40000, 200), (40, 70000, 1000), (2048, 10000, 2304)])
+def test_a_wait_that_runs_out(monkeypatch, M, K, N):
+    """B2C_GEMM_INJECT_TIMEOUT=1 in the joined form: NaN for what is lost, the device flag, and a normal next call."""
+    def fault():
+        f = ctypes.c_uint(7)
+        assert _lib.load().b2c_take_device_fault(ctypes.byref(f)) == 0
+        return f.value
+
+    g = torch.Generator(device=DEV).manual_seed(M)
+    A, B = _positive(g, M, K, dtype=BF16), _positive(g, K, N, dtype=BF16)
+    fault()
+    want = la.gemm(A, B)
+    torch.cuda.synchronize()
+    assert fault() == 0
+    monkeypatch.setenv("B2C_GEMM_INJECT_TIMEOUT", "1")
+    bad = la.gemm(A, B)
+    torch.cuda.synchronize()
+    monkeypatch.delenv("B2C_GEMM_INJECT_TIMEOUT")
+    assert fault() != 0 and fault() == 0
+    lost = torch.isnan(bad)
+    assert bool(lost.any()) and torch.equal(bad[~lost], want[~lost])
+    assert torch.equal(la.gemm(A, B), want) and fault() == 0
