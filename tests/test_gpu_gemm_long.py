@@ -19,7 +19,7 @@ import torch
 
 import mlx_addons_b200.linalg as la
 from mlx_addons_b200 import _lib
-from tests._exact import HALF, MUON, orth64, orth_bound
+from tests._exact import ACTS, HALF, MUON, check, gemm64, orth64, orth_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,24 @@ def test_a_wait_that_runs_out(monkeypatch, M, K, N):
     lost = torch.isnan(bad)
     assert bool(lost.any()) and torch.equal(bad[~lost], want[~lost])
     assert torch.equal(la.gemm(A, B), want) and fault() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("M,K,N", [(300, 33001, 200), (20, 66000, 264), (1700, 8328, 1608), (1601, 8300, 1793), (2304, 16384, 2048)])
+def test_epilogues_of_long_sums(M, K, N, dtype):
+    """The joined forms with every part of the epilogue, in all orders of the operands, ragged and not."""
+    g = torch.Generator(device=DEV).manual_seed(K)
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    bias, R = rand(N).to(dtype), rand(M, N).to(dtype)
+    for i, (ta, tb) in enumerate([(False, True), (True, False), (False, False), (True, True)]):
+        A = rand(K, M).to(dtype).mT if ta else rand(M, K).to(dtype)
+        B = (rand(N, K) / math.sqrt(K)).to(dtype).mT if tb else (rand(K, N) / math.sqrt(K)).to(dtype)
+        act = ACTS[1 + i]
+        Y, pre = la.gemm(A, B, bias, act, R, alpha=0.75, beta=-1.5, return_pre=True)
+        y, p, ey, ep = gemm64(A, B, bias, act, R, 0.75, -1.5)
+        check(pre, p, ep, "pre", K)
+        check(Y, y, ey, "Y", K)
+        assert torch.equal(la.gemm(A, B, bias, act, R, alpha=0.75, beta=-1.5), Y)
+    A, B = rand(3, 140, 33000).to(dtype), (rand(3, 33000, 150) / 180).to(dtype)
+    y, _, ey, _ = gemm64(A, B)
+    check(la.gemm(A, B), y, ey, "batch", 33000)
