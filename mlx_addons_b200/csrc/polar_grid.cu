@@ -262,25 +262,19 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     float* stage = staging + warp * kStageFloats;
     uint32_t buf = 0, tphase = 0;
     if (p.inject == 1 && blockIdx.x == 0) bar_wait(never, 0, gu, limit, &g_grid_fault);
-    for (int f = 0;;) {
+    for (int f = 0; f < phases; ++f) {
       const int st = f / 3, ph = f - 3 * st;
-      const bool last = f == phases - 1;
-      if (last && tid == 0) set_last<PLANES>(cur, p);
-      // A CTA that gives up goes on to its tiles of the last product and stores NaN for them: the others either give
-      // up at the next barrier, where it is missed, and do the same for theirs, or finish theirs without it.
-      bool ok = !epi_any(*gu != 0);
-      if (!ok && !last) {
-        f = phases - 1;
-        continue;
-      }
+      if (f == phases - 1 && tid == 0) set_last<PLANES>(cur, p);
+      if (epi_any(*gu != 0)) break;
       const int kblocks = p.phase[ph].kblocks, BN = p.phase[ph].BN;
-      if (p.inject == 2 && last && blockIdx.x == 0) ok = __all_sync(kFull, bar_wait(never, 0, gu, 1000000ull, &g_grid_fault));
+      const bool last = f == phases - 1;
+      if (p.inject == 2 && last && blockIdx.x == 0) bar_wait(never, 0, gu, 1000000ull, &g_grid_fault);
       for (int64_t t = blockIdx.x; t < p.phase[ph].tiles; t += gridDim.x) {
         const Tile o = phase_tile(p.phase[ph], t);
         float acc[2][32];
-        for (int kb = 0; kb < (JOIN ? kblocks : 1) && ok; ++kb) {
-          ok = __all_sync(kFull, bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_grid_fault));
-          if (!ok) break;
+        bool ok = true;
+        for (int kb = 0; kb < (JOIN ? kblocks : 1); ++kb) {
+          ok = __all_sync(kFull, ok && bar_wait(tfull0 + 8 * buf, tphase, gu, limit, &g_grid_fault));
           fence_after();
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -297,11 +291,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           if (lane == 0) bar_arrive_cluster(tempty0 + 8 * buf);
           if (++buf == 2) buf = 0, tphase ^= 1;
         }
-        if (!ok) {
-          if (!last) break;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) acc[0][c] = acc[1][c] = __int_as_float(0x7fffffff);
-        }
+        if (!ok) break;
         // one copy of the epilogue's code: the sums move up instead of the index
 #pragma unroll 1
         for (int q = 0; q < BN / 64; ++q) {
@@ -312,11 +302,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           for (int c = 0; c < 32; ++c) acc[0][c] = acc[1][c];
         }
       }
-      if (last) break;
-      if (epi_any(*gu != 0)) {
-        f = phases - 1;
-        continue;
-      }
+      if (last || epi_any(*gu != 0)) break;
       // ---- barrier of the grid ----
       __threadfence();
       asm volatile("fence.proxy.async;" ::: "memory");
@@ -341,7 +327,6 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           if (now_ns() - t0 > 2 * kBarrierNs) *gu = 1, atomicOr(&g_grid_fault, 1u);
         bar_arrive_cluster(go);
       }
-      ++f;
     }
   } else if (warp == kEpi) {
     // ---- loads ----
@@ -401,7 +386,20 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   }
   __syncwarp();
   __syncthreads();
-  if (gave_up) settle();
+  if (gave_up) {
+    settle();
+    __syncthreads();
+    // NaN for this CTA's tiles of the last product, which no other CTA writes: the others either give up at the next
+    // barrier, where this one is missed, and do the same for theirs, or finish theirs without it
+    const GridPhase& g = p.phase[2];
+    for (int64_t t = blockIdx.x; t < g.tiles; t += gridDim.x) {
+      const Tile o = phase_tile(g, t);
+      for (int e = tid; e < BM * g.BN; e += kThreadsG) {
+        const int64_t i = o.i + e / g.BN, j = o.j + e % g.BN;
+        if (i < g.I && j < g.J) static_cast<T*>(p.out)[o.b * p.mn + i * p.out_rs + j * p.out_cs] = from_f32<T>(__int_as_float(0x7fffffff));
+      }
+    }
+  }
   fence_before();
   __syncthreads();
   if (warp == kEpi) {
