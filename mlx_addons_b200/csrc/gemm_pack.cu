@@ -36,18 +36,34 @@ __device__ __forceinline__ float bf16_value(uint16_t v) { return __uint_as_float
 // An infinity or a NaN lies in lo, which meets the other operand's hi alone, with a
 // 1 of its sign in hi: in hi it would meet planes that are zero, and infinity times 0
 // is NaN. hi is zero for a zero alone, so that an infinity makes NaN of that and of nothing else.
-__device__ __forceinline__ void thirds(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
+__device__ __noinline__ void thirds(float x, uint16_t& hi, uint16_t& mid, uint16_t& lo) {
   if (isfinite(x)) {
     hi = bf16_finite(x);
     if ((hi & 0x7fff) == 0 && x != 0.f) hi |= 1;
-    const float r = x - bf16_value(hi);
-    mid = bf16_finite(r * 256.f);
-    lo = bf16_finite(fmaf(bf16_value(mid), -0.00390625f, r) * 65536.f);
+    const float r = (x - bf16_value(hi)) * 256.f;
+    mid = bf16_finite(r);
+    lo = bf16_finite((r - bf16_value(mid)) * 256.f);
   } else {
     lo = __bfloat16_as_ushort(__float2bfloat16_rn(x));
     hi = (lo & 0x8000) | 0x3f80;
     mid = 0;
   }
+}
+// Zeros, and values whose bf16 is neither zero nor infinite, go two at a time and without the cases above (an
+// operand of 300 x 256 x 256: 28 us; with those cases for every value 37).
+__device__ __forceinline__ bool common(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  return u == 0 || u - 0x8001u < 0x7f7f8000u - 0x8001u;
+}
+__device__ __forceinline__ uint32_t bf16x2(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void thirds2(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = bf16x2(a, b);
+  const float ra = (a - __uint_as_float(hi << 16)) * 256.f, rb = (b - __uint_as_float(hi & 0xffff0000u)) * 256.f;
+  mid = bf16x2(ra, rb);
+  lo = bf16x2((ra - __uint_as_float(mid << 16)) * 256.f, (rb - __uint_as_float(mid & 0xffff0000u)) * 256.f);
 }
 
 // VEC: rows of unit stride that start on 16 bytes, whole units of 8 in two or
@@ -78,9 +94,22 @@ __global__ void __launch_bounds__(256) gemm_pack_kernel(const PackParams p) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) x[c] = c < n ? x[c] : 0.f;
       }
-      __align__(16) uint16_t h[8], m[8], l[8];
+      __align__(16) uint32_t h[4], m[4], l[4];
+      bool all = true;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) thirds(x[c], h[c], m[c], l[c]);
+      for (int c = 0; c < 8; ++c) all &= common(x[c]);
+      if (all) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) thirds2(x[2 * c], x[2 * c + 1], h[c], m[c], l[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint16_t p0, p1, p2, q0, q1, q2;
+          thirds(x[2 * c], p0, p1, p2);
+          thirds(x[2 * c + 1], q0, q1, q2);
+          h[c] = p0 | (uint32_t)q0 << 16, m[c] = p1 | (uint32_t)q1 << 16, l[c] = p2 | (uint32_t)q2 << 16;
+        }
+      }
       *reinterpret_cast<uint4*>(p.dst + dst) = *reinterpret_cast<const uint4*>(h);
       *reinterpret_cast<uint4*>(p.dst + p.plane + dst) = *reinterpret_cast<const uint4*>(m);
       *reinterpret_cast<uint4*>(p.dst + 2 * p.plane + dst) = *reinterpret_cast<const uint4*>(l);

@@ -63,3 +63,15 @@ def test_subnormal_values(M, K, N):
     B = _rand(6, K, N, scale=2.0**120)
     y, _, ey, _ = gemm64(A, B)
     check(la.gemm(A, B), y, ey, "Y", K)
+
+
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_the_largest_values(M, K, N):
+    """float32's largest, and others whose nearest bf16 would be infinite, among ordinary ones of that size and zeros."""
+    top = torch.finfo(torch.float32).max
+    A, B = _rand(7, M, K, scale=2.0**125).clamp(-top, top), _rand(8, K, N, scale=2.0**-127 / math.sqrt(K))
+    A[:, ::5], A[1, ::7], A[:, 3] = top, -top * (1 - 2.0**-9), 0.0
+    A[2] = torch.where(torch.arange(K, device=DEV) % 2 == 0, top, -top)
+    y, _, ey, _ = gemm64(A, B)
+    check(la.gemm(A, B), y, ey, "Y", K)
+    check(la.gemm(B.mT, A.mT), y.mT, ey.mT, "transposed", K)
