@@ -168,8 +168,8 @@ typedef struct b2c_matrix {
  *   pre  (batch, M, N) contiguous output, or NULL
  * Other outputs may not overlap the inputs. K = 0 gives A B = 0. Non-finite
  * inputs give what IEEE arithmetic gives, in the rows and columns that they meet.
- * A float32 sum whose terms leave float32's range is inf, or, where the size takes the
- * product to the tensor cores, inf or NaN. Each of M, K, N is at most 2^30. No counterpart in
+ * A float32 sum whose terms add up, by size, beyond float32's range may be inf, or, where
+ * the size takes the product to the tensor cores, NaN. Each of M, K, N is at most 2^30. No counterpart in
  * the reference. */
 int b2c_gemm(int dtype, const b2c_matrix *A, const b2c_matrix *B, const void *bias, const b2c_matrix *R, void *Y,
              void *pre, int64_t batch, int64_t M, int64_t K, int64_t N, float alpha, float beta, int activation,

@@ -150,8 +150,8 @@ def gemm(A, B, bias=None, activation: Optional[str] = None, residual=None, *, al
     float32 products are as exact as float32 arithmetic, for values of any size;
     16-bit operands are multiplied exactly and summed in 32 bits. A NaN or an
     infinity stays in the rows and columns that it meets, where it gives what IEEE
-    arithmetic gives; a float32 sum whose terms leave float32's range may
-    give NaN in the place of inf. Larger float32 products read three bf16 planes an
+    arithmetic gives; a float32 sum whose terms add up, by size, beyond
+    float32's range may give NaN in the place of inf. Larger float32 products read three bf16 planes an
     operand, 16-bit ones whose rows do not start on 16 bytes a copy: these take a
     pass of their own and scratch from torch's allocator, 6 and 2 bytes an element. Records no gradient, in neither mode: operands that carry one are refused."""
     name = "gemm"
